@@ -89,6 +89,30 @@ int reco_neumf_gather(const float* Eu_g, const float* Ei_g, const float* Eu_m, c
                       int32_t* oob, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * K-f  embedding lookup with a scale, and the gradient of the table (HBM-bound)
+ * forward and backward of nn.Embedding      src/helpers/ncf_model.py:207-208,220-221
+ * (the reference trains its tables in the notebooks; the scoring handles above have no gradient)
+ * ---------------------------------------------------------------------------------------- */
+/* element types of the K-f / K-g operands; their arithmetic is fp32 throughout, rounded to the type once, when a result is stored */
+#define RECO_DT_F32   0
+#define RECO_DT_BF16  1
+#define RECO_DT_F16   2
+
+/* out[t, :] = scale * table[ids[t], :]; table [rows, dim] of `dtype` with row stride ld (values), out [n, dim] dense.  Any width and
+ * alignment (rows that start on 16 bytes move 16 bytes per lane).  Out-of-range ids are clamped and counted in *oob (nullable). */
+int reco_embedding(const void* table, int64_t rows, int64_t ld, int dim, int dtype, const int64_t* ids, int64_t n, float scale,
+                   void* out, int32_t* oob, void* stream);
+
+/* out[v, :] = scale * sum of grad[t, :] over the t with ids[t] = v (clamped like the lookup's; 0 where there is none), summed in fp32
+ * in an order that depends on n and rows alone (no atomic adds: the same bits on every run).  Every row of out [rows, dim] is
+ * written.  padding: a row that takes no gradient (its terms are not read, its row is 0), or -1.  grad [n, dim] of `dtype` with row
+ * stride ldg; out dense, 16-byte aligned, of the same type.  n = 0 writes zeros.  n < 2^31, rows < 2^31 - 1.
+ * ws: reco_embedding_grad_workspace_bytes(n, rows, dim), 16-byte aligned; calls that overlap need one each. */
+size_t reco_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int dim);
+int reco_embedding_grad(const int64_t* ids, int64_t n, const void* grad, int64_t ldg, int dim, int dtype, int64_t rows, float scale,
+                        int64_t padding, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * K-c  Linear layer as an fp32 MFMA GEMM with fused epilogue
  *   C[m, n] = act( sum_k A[row(m), k] * W[n, k] + bias[n] )
  * replaces nn.Linear + Sigmoid/ReLU/clamp   src/autorec/utils/model.py:25-33,
@@ -360,6 +384,7 @@ int reco_topk_rows_seen(const float* scores, int64_t src_rows, int64_t N, int64_
  *   RECO_PROF_CSR     the segment kernel of reco_csr_linear_f32 (its reduce launch: RECO_PROF_CSR_REDUCE)
  *   RECO_PROF_TOPK    the scan / lane kernel of reco_topk_rows* (its merge launch: RECO_PROF_TOPK_MERGE)
  *   RECO_PROF_ENCODER the fused layer-2/3 kernel of reco_mlp2_f32
+ *   RECO_PROF_EMBEDDING  the launches of reco_embedding / reco_embedding_grad
  * reco_profile_collect_kinds synchronises the recorded events and returns per-launch milliseconds and kinds in launch order
  * (host pointers; kind_out nullable), then rearms.  reco_profile_collect returns the RECO_PROF_TOWER launches only.
  * ---------------------------------------------------------------------------------------- */
@@ -372,6 +397,7 @@ int reco_topk_rows_seen(const float* scores, int64_t src_rows, int64_t N, int64_
 #define RECO_PROF_TOPK           7
 #define RECO_PROF_TOPK_MERGE     8
 #define RECO_PROF_ENCODER        9
+#define RECO_PROF_EMBEDDING     10
 int reco_profile_enable(int max_launches);                                    /* every kind */
 int reco_profile_enable_kinds(int max_launches, unsigned kind_mask);          /* only kinds k with bit (1u << k) set: an event pair
                                                                                  costs a few microseconds of stream time */

@@ -101,6 +101,135 @@ def neumf_gather(eu_g, ei_g, eu_m, ei_m, user, item, check_ids=True, gmf_out=Non
 
 
 # ----------------------------------------------------------------------------------------------
+# K-f embedding lookup and its gradient
+# ----------------------------------------------------------------------------------------------
+DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+
+
+def _rows(t, name):
+    """A 2-D float32 / bfloat16 / float16 GPU tensor whose rows are dense: a column block of a wider row-major buffer is read in
+    place, anything else is copied."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if not t.is_cuda:
+        raise ValueError("%s must live on the GPU" % name)
+    if t.dtype not in DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    if t.dim() != 2:
+        raise ValueError("%s must be 2-D, got shape %s" % (name, tuple(t.shape)))
+    t = t.detach()
+    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _number(v, name):
+    if isinstance(v, torch.Tensor) or isinstance(v, bool):
+        raise TypeError("%s must be a number, got %s" % (name, type(v).__name__))
+    return float(v)
+
+
+def _padding(padding_idx, rows):
+    """nn.Embedding's rule: an index into the table, negative ones from its end; -1 for none."""
+    if padding_idx is None:
+        return -1
+    if not -rows <= padding_idx < rows:
+        raise ValueError("padding_idx must be within the %d rows of the table, got %d" % (rows, padding_idx))
+    return int(padding_idx) % rows
+
+
+def _no_captured_graph(what, instead):
+    """Autograd inside a HIP graph is refused: leaves that an eager graph has touched are accumulated on that graph's stream, and
+    a captured backward pass that waits for it ends the process.  The functional gradient is what a captured step calls."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s cannot record an autograd graph while its stream is being captured: use torch.no_grad() and call %s "
+                           "in the captured work" % (what, instead))
+
+
+def _embedding(ids, table, scale, check_ids):
+    out = torch.empty((ids.numel(), table.shape[1]), dtype=table.dtype, device=table.device)
+    if out.numel() == 0:
+        return out
+    oob = torch.zeros(1, dtype=torch.int32, device=table.device) if check_ids else None
+    with torch.cuda.device(table.device):
+        check(_lib.lib().reco_embedding(_p(table), table.shape[0], _ld(table), table.shape[1], DTYPES[table.dtype], _p(ids), ids.numel(),
+                                        scale, _p(out), _p(oob), _stream(table.device)))
+    if check_ids and int(oob.item()):
+        raise IndexError("index out of range in self")
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding, check_ids):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.padding = table.shape[0], scale, padding
+        return _embedding(ids, _rows(table, "table"), scale, check_ids)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _no_captured_graph("embedding's backward pass", "embedding_grad")
+        (ids,) = ctx.saved_tensors
+        return embedding_grad(ids, grad, ctx.rows, ctx.scale, ctx.padding if ctx.padding >= 0 else None), None, None, None, None
+
+
+def embedding(ids, table, scale=1.0, padding_idx=None, check_ids=True):
+    """scale * table[ids] (nn.Embedding forward, ncf_model.py:207-208), differentiable in the table (see embedding_grad).
+
+    ids: integers of any shape; table [rows, dim] float32 / bfloat16 / float16 (the product is taken in 32 bits and rounded once);
+    padding_idx: a row that takes no gradient.  Out-of-range ids raise IndexError; check_ids=False skips that report (one
+    device-to-host sync), they are then clamped, here and in the gradient.  Inside a HIP graph: under no_grad, check_ids=False.
+    """
+    scale = _number(scale, "scale")
+    t = _rows(table, "table")
+    padding = _padding(padding_idx, t.shape[0])
+    shape = ids.shape if isinstance(ids, torch.Tensor) else None
+    if shape is not None and ids.dim() != 1:
+        ids = ids.reshape(-1)
+    ids = _i64(ids, "ids", t.device)
+    if torch.is_grad_enabled() and table.requires_grad:
+        _no_captured_graph("embedding", "embedding_grad")
+        out = _Embedding.apply(table, ids, scale, padding, check_ids)
+    else:
+        out = _embedding(ids, t, scale, check_ids)
+    return out if shape is None or len(shape) == 1 else out.view(shape + (t.shape[1],))
+
+
+def embedding_grad(ids, grad, rows, scale=1.0, padding_idx=None):
+    """The gradient of embedding()'s table [rows, dim], dense, in grad's type: scale * the sum of grad's rows per id, taken in 32 bits
+    in an order that depends on the sizes alone (the same bits on every run), 0 for rows that no id names and for padding_idx.
+
+    ids: integers of any shape, clamped to the table; grad: ids' shape + [dim].  May be captured into a HIP graph.
+    """
+    scale, rows = _number(scale, "scale"), int(rows)
+    if isinstance(grad, torch.Tensor) and grad.dim() != 2 and grad.dim() > 0:
+        grad = grad.reshape(-1, grad.shape[-1]) if grad.numel() else grad.new_empty((0, grad.shape[-1]))
+    grad = _rows(grad, "grad")
+    if isinstance(ids, torch.Tensor) and ids.dim() != 1:
+        ids = ids.reshape(-1)
+    ids = _i64(ids, "ids", grad.device)
+    n, dim = grad.shape
+    if ids.numel() != n:
+        raise ValueError("grad has %d rows for %d ids" % (n, ids.numel()))
+    padding = _padding(padding_idx, rows)
+    out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
+    if out.numel() == 0:
+        return out
+    L = _lib.lib()
+    nbytes = L.reco_embedding_grad_workspace_bytes(n, rows, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
+    with torch.cuda.device(grad.device):
+        check(L.reco_embedding_grad(_p(ids), n, _p(grad), _ld(grad), dim, DTYPES[grad.dtype], rows, scale, padding, _p(out), _p(ws), nbytes,
+                                    _stream(grad.device)))
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
 # K-c Linear / AutoRec
 # ----------------------------------------------------------------------------------------------
 def linear(x, weight, bias=None, act=None, lo=0.0, hi=0.0, out=None, x_transposed=False, bias_per_row=False, precision=None):

@@ -1,0 +1,266 @@
+"""embedding / embedding_grad on the GPU against the same sums in 64 bits.
+
+Tolerances.  A product scale * x is rounded to 32 bits once (2^-24 relative) and to the type once (half a step, finfo.eps / 2; half
+of the smallest subnormal where f16 has no more digits).  A sum of k terms in 32 bits, in any order, is within k * 2^-24 * sum|x| of
+the exact one; the scale adds one rounding more.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+U = 2.0 ** -24
+
+
+def _ops():
+    from recommender_amd import ops
+    return ops
+
+
+def _tol(exact, dtype, abs_sum=None, k=None):
+    t = exact.abs() * (torch.finfo(dtype).eps / 2 + 2 * U) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -140)
+    if abs_sum is not None:
+        t = t + (k + 2) * U * abs_sum * (1 + torch.finfo(dtype).eps)
+    return t
+
+
+def _close(got, exact, tol, what):
+    err = (got.double() - exact).abs()
+    bad = ~(err <= tol)
+    assert not bool(bad.any()), "%s: %d of %d outside, worst %g over %g" % (what, int(bad.sum()), bad.numel(), float(err.max()), float(tol.max()))
+
+
+def _reference(ids, grad, rows, scale, padding):
+    """(gradient, sum of |terms|, terms per row) in 64 bits."""
+    keep = torch.ones_like(ids, dtype=torch.bool) if padding is None else ids != padding
+    ids, g = ids[keep], grad.double()[keep] * scale
+    total = torch.zeros((rows, grad.shape[1]), dtype=torch.float64, device=grad.device).index_add_(0, ids, g)
+    size = torch.zeros_like(total).index_add_(0, ids, g.abs())
+    return total, size, torch.bincount(ids, minlength=rows).double()[:, None]
+
+
+def _check_grad(ids, grad, rows, scale=1.0, padding=None):
+    got = _ops().embedding_grad(ids, grad, rows, scale, padding)
+    exact, size, k = _reference(ids, grad, rows, scale, padding)
+    assert got.shape == exact.shape and got.dtype == grad.dtype
+    _close(got, exact, _tol(exact, grad.dtype, size, k), "gradient")
+    assert torch.equal(got, _ops().embedding_grad(ids, grad, rows, scale, padding)), "two runs differ"
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,n", [(1, 1, 1), (7, 3, 5), (3533, 32, 100), (50, 50, 257), (1000, 127, 64), (300, 512, 33), (11, 2048, 9), (97, 64, 5000)])
+def test_lookup(dtype, rows, dim, n):
+    g = torch.Generator(device="cuda").manual_seed(rows + dim + n)
+    table = torch.randn(rows, dim, device="cuda", generator=g).to(dtype)
+    ids = torch.randint(0, rows, (n,), device="cuda", generator=g)
+    for scale in (1.0, math.sqrt(dim), -0.3):
+        got = _ops().embedding(ids, table, scale)
+        exact = table.double()[ids] * float(np.float32(scale))
+        _close(got, exact, _tol(exact, dtype), "lookup x %g" % scale)
+    assert torch.equal(_ops().embedding(ids, table), table[ids])
+
+
+def test_lookup_shapes_and_strides():
+    ops = _ops()
+    wide = torch.randn(40, 31, device="cuda")
+    ids = torch.tensor([[3, 0, 39], [5, 5, 1]])                               # host ids, two dimensions
+    for t in (wide[:, :16], wide[:, 3:20], wide.t()[:31, :8], wide[::3, 1:2], wide[:, 4:4 + 16].to(torch.float16)):
+        got = ops.embedding(ids.clamp(max=t.shape[0] - 1).int(), t)
+        assert got.shape == (2, 3, t.shape[1]) and torch.equal(got, t[ids.clamp(max=t.shape[0] - 1).cuda()])
+    assert ops.embedding(torch.empty(0, dtype=torch.int64), wide).shape == (0, 31)
+    assert ops.embedding(torch.empty((0, 4), dtype=torch.int64), wide).shape == (0, 4, 31)
+    assert ops.embedding([3, 4], wide).shape == (2, 31)
+
+
+def test_ids_out_of_range():
+    ops = _ops()
+    table = torch.randn(10, 8, device="cuda", requires_grad=True)
+    bad = torch.tensor([0, 10, -1, 2 ** 40, -2 ** 40, 9], device="cuda")
+    with pytest.raises(IndexError):
+        ops.embedding(bad, table)
+    out = ops.embedding(bad, table, check_ids=False)
+    clamped = bad.clamp(0, 9)
+    assert torch.equal(out, table.detach()[clamped])
+    up = torch.randn_like(out)
+    grad, = torch.autograd.grad(out, table, up)
+    want = _ops().embedding_grad(clamped, up, 10)
+    assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,n", [
+    (1, 1, 1), (1, 5, 3000), (2, 3, 9), (6038, 64, 4096), (6038, 64, 4097), (2047, 16, 20000), (2048, 24, 20000), (60401, 50, 70001),
+    (1000000, 8, 5000), (5000000, 4, 30000), (13, 300, 777), (300, 513, 1200), (5, 128, 9000)])
+def test_gradient(dtype, rows, dim, n):
+    g = torch.Generator(device="cuda").manual_seed(rows + 31 * dim + n)
+    grad = torch.randn(n, dim, device="cuda", generator=g).to(dtype)
+    even = torch.randint(0, rows, (n,), device="cuda", generator=g)
+    popular = torch.exp(torch.rand(n, device="cuda", generator=g) * math.log(rows)).long().clamp(1, rows) - 1
+    _check_grad(even, grad, rows, scale=math.sqrt(dim))
+    _check_grad(popular, grad, rows, padding=0)
+    _check_grad(torch.full((n,), rows - 1, device="cuda"), grad, rows, scale=-0.7)                  # one id takes everything
+    assert int(torch.count_nonzero(_check_grad(torch.full((n,), rows - 1, device="cuda"), grad, rows, padding=rows - 1))) == 0
+    _check_grad(torch.arange(n, device="cuda") * 7 % rows, grad, rows, padding=rows // 2)
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 8192, 100000])
+@pytest.mark.parametrize("share", [0.1, 0.9])
+def test_gradient_runs_cross_chunks(n, share):
+    """Sorted runs of every length from 1 to a share of the list, so that they begin and end at every place of a chunk."""
+    lengths = []
+    k = 1
+    while sum(lengths) < n * (1 - share):
+        lengths.append(k)
+        k = k % 150 + 1
+    ids = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))[: int(n * (1 - share))]
+    ids = torch.cat([ids, torch.full((n - ids.numel(),), len(lengths))])
+    ids = ids[torch.randperm(n, generator=torch.Generator().manual_seed(n))].cuda()
+    grad = torch.randn(n, 20, device="cuda")
+    _check_grad(ids, grad, len(lengths) + 3)
+
+
+def test_gradient_adds_in_order_of_position():
+    """A lone large term swallows the small ones before it and not those behind it: the order is that of the positions, within one chunk."""
+    grad = torch.ones(8, 1, device="cuda")
+    grad[3] = 2.0 ** 24
+    want = torch.zeros((), dtype=torch.float32)
+    for v in grad.cpu()[:, 0]:
+        want = want + v
+    got = _ops().embedding_grad(torch.zeros(8, dtype=torch.int64, device="cuda"), grad, 1)
+    assert float(got) == float(want)
+
+
+def test_gradient_strided_expanded_and_special_values():
+    ops = _ops()
+    ids = torch.tensor([1, 1, 4, 0], device="cuda")
+    wide = torch.randn(4, 40, device="cuda")
+    for g in (wide[:, :16], wide[:, 5:12], wide.t()[:4, :4], torch.ones(1, 6, device="cuda").expand(4, 6), torch.ones((), device="cuda").expand(4, 3)):
+        _check_grad(ids, g, 6)
+    bad = torch.ones(4, 8, device="cuda")
+    bad[0, 0], bad[2, 1], bad[3, 2] = float("nan"), float("inf"), float("-inf")
+    got = ops.embedding_grad(ids, bad, 6, padding_idx=0)
+    assert torch.isnan(got[1, 0]) and got[4, 1] == float("inf") and int(torch.count_nonzero(got[0])) == 0 and not torch.isnan(got[2:]).any()
+    bad[:, :] = float("nan")
+    assert int(torch.count_nonzero(ops.embedding_grad(torch.zeros(4, dtype=torch.int64, device="cuda"), bad, 3, padding_idx=0))) == 0
+    empty = ops.embedding_grad(torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, 7, device="cuda", dtype=torch.bfloat16), 5)
+    assert empty.shape == (5, 7) and int(torch.count_nonzero(empty)) == 0
+
+
+@pytest.mark.parametrize("dim", [1, 3, 5, 8])
+@pytest.mark.parametrize("rows", [1, 3, 5, 1001])
+@pytest.mark.parametrize("n", [3, 5000])
+def test_gradient_writes_its_table_and_nothing_else(rows, dim, n):
+    """Every byte of the table is written, the bytes behind it are not (through the C entry, into a larger buffer)."""
+    import ctypes
+    from recommender_amd import _lib
+    ops = _ops()
+    for dtype in TYPES:
+        buf = torch.full((rows * dim + 64,), 7.0, dtype=dtype, device="cuda")
+        ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+        grad = torch.ones(n, dim, dtype=dtype, device="cuda")
+        nbytes = _lib.lib().reco_embedding_grad_workspace_bytes(n, rows, dim)
+        ws = torch.full((nbytes + 256,), 0xAB, dtype=torch.uint8, device="cuda")
+        _lib.check(_lib.lib().reco_embedding_grad(ops._p(ids), n, ops._p(grad), dim, dim, ops.DTYPES[dtype], rows, 1.0, -1, ops._p(buf), ops._p(ws),
+                                                  nbytes, ops._stream(buf.device)))
+        want = torch.zeros(rows * dim, dtype=dtype, device="cuda")
+        want[:dim] = n
+        assert torch.equal(buf[: rows * dim], want.to(dtype)) and bool((buf[rows * dim:] == 7.0).all()) and bool((ws[nbytes:] == 0xAB).all())
+
+
+def test_autograd_leaf_and_shared_table():
+    """Two lookups of one table, one of them twice differentiated through: gradients add up, as autograd's own do."""
+    ops = _ops()
+    table = torch.randn(30, 12, device="cuda", requires_grad=True)
+    a, b = torch.randint(0, 30, (5, 4), device="cuda"), torch.randint(0, 30, (9,), device="cuda")
+    ua, ub = torch.randn(5, 4, 12, device="cuda"), torch.randn(9, 12, device="cuda")
+    ((ops.embedding(a, table, 2.0) * ua).sum() + (ops.embedding(b, table, padding_idx=-1) * ub).sum()).backward()
+    want = _reference(a.reshape(-1), ua.reshape(-1, 12), 30, 2.0, None)[0] + _reference(b, ub, 30, 1.0, 29)[0]
+    _close(table.grad, want, 1e-5 * torch.ones_like(want), "leaf gradient")       # sums of at most 29 terms of size 2: 29 * 2 * 5 * 2^-24
+    with pytest.raises(RuntimeError):
+        g, = torch.autograd.grad(ops.embedding(b, table).square().sum(), table, create_graph=True)
+        g.sum().backward()
+
+
+def test_gradient_against_differences():
+    ops = _ops()
+    table = torch.randn(6, 3, device="cuda")
+    ids = torch.tensor([0, 2, 2, 5], device="cuda")
+    weight = torch.randn(4, 3, device="cuda", dtype=torch.float64)
+    f = lambda t: float((ops.embedding(ids, t, 1.5).double() * weight).sum())      # noqa: E731
+    leaf = table.clone().requires_grad_()
+    grad, = torch.autograd.grad((ops.embedding(ids, leaf, 1.5).double() * weight).sum(), leaf)
+    step = 2.0 ** -6
+    for v in range(6):
+        for d in range(3):
+            up, down = table.clone(), table.clone()
+            up[v, d] += step
+            down[v, d] -= step
+            # the function is linear; each lookup rounds by 2^-24 of at most 8 x 1.5, twice, over 2 steps, for two rows
+            assert abs((f(up) - f(down)) / (2 * step) - float(grad[v, d])) < 2 * 2 * 12 * 2.0 ** -24 / (2 * step) * 4 + 1e-6
+
+
+def test_other_stream_and_two_at_once():
+    """Calls on two streams at a time have workspaces of their own."""
+    ops = _ops()
+    n, rows, dim = 60000, 5000, 64
+    ids = [torch.randint(0, rows, (n,), device="cuda") for _ in range(2)]
+    grads = [torch.randn(n, dim, device="cuda") for _ in range(2)]
+    want = [ops.embedding_grad(i, g, rows) for i, g in zip(ids, grads)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = ops.embedding_grad(ids[k], grads[k], rows)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("n", [100, 30000])
+def test_captured_and_replayed(n):
+    ops = _ops()
+    rows, dim = 777, 40
+    table = torch.randn(rows, dim, device="cuda")
+    ids = torch.randint(0, rows, (n,), device="cuda")
+    grad = torch.randn(n, dim, device="cuda")
+    ops.embedding_grad(ids, grad, rows)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):                                    # two graphs over the same inputs
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.embedding(ids, table, 0.5, check_ids=False), ops.embedding_grad(ids, grad, rows, 0.5, 3)
+        graphs.append(g)
+        outs.append(out)
+    for k in range(4):
+        ids.copy_(torch.randint(0, rows, (n,), device="cuda"))
+        grad.normal_()
+        table.normal_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = ops.embedding(ids, table, 0.5), ops.embedding_grad(ids, grad, rows, 0.5, 3)
+        for out in outs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), k
+
+
+def test_offsets_past_32_bits():
+    """A table of more than 2^32 values (9 GB): rows at its far end are read and written there."""
+    ops = _ops()
+    rows, dim = (1 << 25) + 5, 130
+    table = torch.zeros(rows, dim, dtype=torch.float16, device="cuda")
+    far = torch.tensor([rows - 1, 3, rows - 2, rows // 2], device="cuda")
+    values = torch.randn(4, dim, device="cuda").half()
+    table[far] = values
+    assert torch.equal(ops.embedding(far, table), values)
+    del table
+    grad = ops.embedding_grad(far, values, rows)
+    assert torch.equal(grad[far], values)
+    grad[far] = 0
+    assert not any(bool(part.any()) for part in grad.split(1 << 22))
