@@ -132,6 +132,33 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
                     int act, float lo, float hi, float* C, int64_t ldc, int flags,
                     void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * K-g  softmax cross entropy over a whole catalogue, and its gradients, without its logits in memory
+ *   z[t, v] = sum_d x[t, d] w[v, d] + bias[v];   loss_t = log sum_v exp(z[t, v]) - z[t, target_t]
+ * the loss over all items that a two-tower / GMF table (src/helpers/ncf_model.py:207-211) or the AutoRec decoder
+ * (src/autorec/utils/model.py:31-33) is trained with; no counterpart in the reference, which samples negatives.
+ * x [T, D], w [V, D], bias [V] (nullable) of one `dtype`, rows dense with strides ldx / ldw.  Any sizes, strides and alignment
+ * (rows that do not start on 16 bytes, or whose width is no whole number of 16-byte groups, are copied into ws first).
+ * target int64 [T]; a row whose target equals `ignore` has no loss and no gradient whatever its x holds; other targets outside
+ * [0, V) are clamped and counted in *oob (nullable).  bias may hold -inf (items that are never offered) or the type's lowest value.
+ * reduction: RECO_XENT_NONE (loss [T]), _MEAN over the rows that count (loss [1]; NaN when none does), _SUM.  loss and state are fp32.
+ * state [2 T] is written by the forward call and read by the gradient call, which takes the same operands.
+ * dloss fp32: [T] for RECO_XENT_NONE, else [1].  dx [T, D], dw [V, D], db [V] dense, of `dtype`; NULL = not wanted.
+ * Sums run in an order that depends on the sizes alone: the same bits on every run.  Work is enqueued only; calls that overlap need a
+ * workspace each (*_workspace_bytes looks at x and w for their alignment, never through them), 16-byte aligned.
+ * ---------------------------------------------------------------------------------------- */
+#define RECO_XENT_NONE 0
+#define RECO_XENT_MEAN 1
+#define RECO_XENT_SUM  2
+size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D);
+int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
+                     const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, int32_t* oob,
+                     void* ws, size_t ws_bytes, void* stream);
+size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D);
+int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
+                          const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dloss,
+                          void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+
 /* Linear layer over a SPARSE input given as CSR -- the "masked-observed" form of the AutoRec / Hybrid encoders, whose input
  * is the 4.5 %-dense rating matrix (or its transpose) with unobserved entries fed as literal zeros:
  *   src/autorec/utils/model.py:31-33 with X from src/api/core/inference_engine.py:230 / src/api/core/data_loader.py:96-103;
@@ -385,6 +412,7 @@ int reco_topk_rows_seen(const float* scores, int64_t src_rows, int64_t N, int64_
  *   RECO_PROF_TOPK    the scan / lane kernel of reco_topk_rows* (its merge launch: RECO_PROF_TOPK_MERGE)
  *   RECO_PROF_ENCODER the fused layer-2/3 kernel of reco_mlp2_f32
  *   RECO_PROF_EMBEDDING  the launches of reco_embedding / reco_embedding_grad
+ *   RECO_PROF_XENT       all launches of one reco_linear_xent / reco_linear_xent_grad call as one entry
  * reco_profile_collect_kinds synchronises the recorded events and returns per-launch milliseconds and kinds in launch order
  * (host pointers; kind_out nullable), then rearms.  reco_profile_collect returns the RECO_PROF_TOWER launches only.
  * ---------------------------------------------------------------------------------------- */
@@ -398,6 +426,7 @@ int reco_topk_rows_seen(const float* scores, int64_t src_rows, int64_t N, int64_
 #define RECO_PROF_TOPK_MERGE     8
 #define RECO_PROF_ENCODER        9
 #define RECO_PROF_EMBEDDING     10
+#define RECO_PROF_XENT          11
 int reco_profile_enable(int max_launches);                                    /* every kind */
 int reco_profile_enable_kinds(int max_launches, unsigned kind_mask);          /* only kinds k with bit (1u << k) set: an event pair
                                                                                  costs a few microseconds of stream time */

@@ -15,8 +15,9 @@ LIB_PATH = os.environ.get("RECO_HIP_LIB") or os.path.join(_HERE, "lib", "libreco
 OK, EINVAL, EHIP, ENOMEM, EINDEX = 0, -1, -2, -3, -4
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_CLAMP, ACT_RATING = 0, 1, 2, 3, 4
 PREC_F32, PREC_SPLIT_BF16X3 = 0, 1
-PROF_TOWER, PROF_GATHER, PROF_LINEAR, PROF_LINEAR_REDUCE, PROF_CSR, PROF_CSR_REDUCE, PROF_TOPK, PROF_TOPK_MERGE, PROF_ENCODER, PROF_EMBEDDING = range(1, 11)
+PROF_TOWER, PROF_GATHER, PROF_LINEAR, PROF_LINEAR_REDUCE, PROF_CSR, PROF_CSR_REDUCE, PROF_TOPK, PROF_TOPK_MERGE, PROF_ENCODER, PROF_EMBEDDING, PROF_XENT = range(1, 12)
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+XENT_NONE, XENT_MEAN, XENT_SUM = 0, 1, 2
 ABI_VERSION = 5
 
 
@@ -43,6 +44,12 @@ _SIGNATURES = {
     "reco_embedding_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "reco_embedding_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int64, c_float, c_int64, c_void_p, c_void_p,
                                     c_size_t, c_void_p]),
+    "reco_linear_xent_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64]),
+    "reco_linear_xent": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "reco_linear_xent_grad_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64]),
+    "reco_linear_xent_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "reco_linear_f32": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                 c_int64, c_int64, c_int, c_float, c_float, c_void_p, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "reco_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),

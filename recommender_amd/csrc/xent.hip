@@ -1,0 +1,686 @@
+// K-g: softmax cross entropy of x W^T + bias over a whole catalogue, and its gradients, gfx950.
+//
+//   z[t, v] = sum_d x[t, d] W[v, d] + bias[v]             never stored whole: the vocabulary is walked in pieces
+//   others_t = log sum over v != y_t of exp(z[t, v]),     d_t = others_t - z[t, y_t]
+//   loss_t = log(1 + exp(d_t)),   q_t = 1 - p_t = 1 / (1 + exp(-d_t)),   lse_t = z[t, y_t] + loss_t
+//   G[t, v] = g_t exp(z[t, v] - lse_t),  G[t, y_t] = -g_t q_t
+//   dx = G W,   dW = G^T x,   dbias = column sums of G
+//
+// The target's own term is kept out of the sum: loss and q keep their digits where the model is sure of the target (p near one),
+// which 1 - p would lose.  Ignored rows have no loss and no gradient, whatever their x holds.
+//
+// Everything but the operands of the matrix instructions is 32 bits wide: logits, running maxima and sums, losses, accumulators.  G is
+// rounded to the operands' type to be multiplied (half a step per term, where the result takes one such rounding too); half-precision G
+// is held times 2^14, so that probabilities down to 2^-28 are normal numbers.
+//
+// This file: the form for every width.  A piece of G, [T, piece] in the operands' type, is written and read by two matrix products.
+#include "types16.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+template <typename T> struct Traits;
+template <> struct Traits<float> {
+    static constexpr int VEC = 4, KSTEP = 8, BK = 32;
+    static constexpr float G_SCALE = 1.f;
+    typedef f32x4 frag;
+};
+template <> struct Traits<__bf16> {
+    static constexpr int VEC = 8, KSTEP = 16, BK = 64;
+    static constexpr float G_SCALE = 1.f;
+    typedef bf16x8 frag;
+};
+template <> struct Traits<_Float16> {
+    static constexpr int VEC = 8, KSTEP = 16, BK = 64;
+    static constexpr float G_SCALE = 16384.f;
+    typedef f16x8 frag;
+};
+
+// acc[m, n] += sum over KSTEP k of a[m, k] b[n, k].  Lane l holds m (n) = l % 32; its k are 8 (l / 32) + 0 .. 7 of 16, in 32 bits
+// 4 (l / 32) + 0 .. 3 of 8 -- the order of k is free as long as both operands have the same.  The result: n = l % 32, m of
+// register r is 8 (r / 4) + 4 (l / 32) + r % 4.
+__device__ __forceinline__ void mma(f32x16& acc, const f32x4& a, const f32x4& b)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& acc, const bf16x8& a, const bf16x8& b) { acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
+__device__ __forceinline__ void mma(f32x16& acc, const f16x8& a, const f16x8& b) { acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); }
+
+// ---------------------------------------------------------------------------------------------
+// a 128 x 128 tile of a matrix product: 4 waves, 64 x 64 each; operands staged through LDS, the next step's in registers meanwhile
+// ---------------------------------------------------------------------------------------------
+constexpr int TB = 128;
+
+// A matrix of which 128 rows r take part: KC: element (r, k) at p[r * ld + k], else at p[k * ld + r].  Row starts are 16-byte
+// aligned; `rows` and `k_end` count whole VEC groups along the contiguous side.
+template <typename T> struct Operand {
+    const T* p;
+    int64_t ld;
+    int64_t rows;
+    const int64_t* keep;      // !KC: k rows whose keep[k] == drop are read as zeros (nullable)
+    int64_t drop;
+};
+
+template <typename T, bool KC> struct Stage {
+    static constexpr int VEC = Traits<T>::VEC, BK = Traits<T>::BK;
+    static constexpr int PITCH = KC ? BK + VEC : TB + VEC;             // 16 bytes of padding: rows start on different banks
+    static constexpr int SIZE = (KC ? TB : BK) * PITCH;
+    static constexpr int PER_ROW = (KC ? BK : TB) / VEC;               // 16-byte pieces per stored row
+    static constexpr int PIECES = 4;                                   // per thread: 1,024 in all
+    Pack<T, VEC> reg[PIECES];
+
+    __device__ __forceinline__ void load(const Operand<T>& o, int64_t r0, int64_t k0, int64_t k_end)
+    {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = threadIdx.x + 256 * i, row = c / PER_ROW, col = (c % PER_ROW) * VEC;
+            const int64_t r = r0 + (KC ? row : col), k = k0 + (KC ? col : row);
+            bool ok = r < o.rows && k < k_end;
+            if (!KC && ok && o.keep) ok = o.keep[k] != o.drop;
+            if (ok) {
+                reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(o.p + (KC ? r * o.ld + k : k * o.ld + r));
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) reg[i].v[j] = (T)0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const
+    {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = threadIdx.x + 256 * i;
+            *reinterpret_cast<Pack<T, VEC>*>(lds + (c / PER_ROW) * PITCH + (c % PER_ROW) * VEC) = reg[i];
+        }
+    }
+    // rows r .. r + 31 and one KSTEP of k from LDS
+    static __device__ __forceinline__ typename Traits<T>::frag frag(const T* lds, int r, int k)
+    {
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        typename Traits<T>::frag f;
+        if constexpr (KC) {
+            f = *reinterpret_cast<const typename Traits<T>::frag*>(lds + (r + (lane & 31)) * PITCH + k + half * VEC);
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = lds[(k + 4 * half + i) * PITCH + r + (lane & 31)];
+        } else {
+            // 16 lanes read 4 k rows of 16 values and get them transposed: lane i value i of each row
+            const T* src = lds + (k + 8 * half + ((lane & 15) >> 2)) * PITCH + r + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+            union { s16x4 h[2]; typename Traits<T>::frag f; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)src);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(src + 4 * PITCH));
+            f = u.f;
+        }
+        return f;
+    }
+};
+
+// acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end)
+template <typename T, bool AKC, bool BKC>
+__device__ __forceinline__ void tile_product(f32x16 (&acc)[2][2], const Operand<T>& A, const Operand<T>& B, int64_t m0, int64_t n0, int64_t k0,
+                                             int64_t k_end, T* la, T* lb)
+{
+    constexpr int BK = Traits<T>::BK, KSTEP = Traits<T>::KSTEP;
+    const int wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    Stage<T, AKC> sa;
+    Stage<T, BKC> sb;
+    sa.load(A, m0, k0, k_end);
+    sb.load(B, n0, k0, k_end);
+    for (int64_t k = k0; k < k_end; k += BK) {
+        __syncthreads();
+        sa.store(la);
+        sb.store(lb);
+        __syncthreads();
+        if (k + BK < k_end) {
+            sa.load(A, m0, k + BK, k_end);
+            sb.load(B, n0, k + BK, k_end);
+        }
+#pragma unroll
+        for (int s = 0; s < BK; s += KSTEP) {
+            typename Traits<T>::frag a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = Stage<T, AKC>::frag(la, wm + 32 * i, s);
+                b[i] = Stage<T, BKC>::frag(lb, wn + 32 * i, s);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma(acc[i][j], a[i], b[j]);
+        }
+    }
+}
+
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+struct Problem {
+    int64_t T, V, D;            // D: values per row as read (whole VEC groups, zeros behind the caller's width)
+    int64_t ldx, ldw;
+    const void* x;
+    const void* w;
+    const void* bias;           // nullable
+    const int64_t* target;
+    int64_t ignore;
+};
+
+__device__ __forceinline__ int64_t clamp_target(int64_t y, int64_t V) { return y < 0 ? 0 : y >= V ? V - 1 : y; }
+
+// (m, s): running maximum and sum of exp(z - m) of the logits that are not the target's
+struct Running { float m, s; };
+
+__device__ __forceinline__ Running joined(Running a, Running b)
+{
+    Running r;
+    r.m = fmaxf(a.m, b.m);
+    const float base = r.m == -INFINITY ? 0.f : r.m;            // nothing but -inf so far: the sum stays 0
+    r.s = a.s * exp2f((a.m - base) * LOG2E) + b.s * exp2f((b.m - base) * LOG2E);
+    return r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void stats_kernel(Problem p, int64_t tiles_per_split, Running* __restrict__ part, float* __restrict__ z_target)
+{
+    __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
+    __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr, 0}, X{(const T*)p.x, p.ldx, p.T, nullptr, 0};
+    const T* bias = (const T*)p.bias;
+    const int64_t n0 = (int64_t)blockIdx.x * TB;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    int64_t y[2];
+    Running run[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t t = n0 + wn + 32 * j + (lane & 31);
+        y[j] = -1;
+        if (t < p.T && p.target[t] != p.ignore) y[j] = clamp_target(p.target[t], p.V);
+        run[j] = Running{-INFINITY, 0.f};
+    }
+    const int64_t first = blockIdx.y * tiles_per_split * TB;
+    const int64_t end = first + tiles_per_split * TB < p.V ? first + tiles_per_split * TB : p.V;
+    for (int64_t m0 = first; m0 < end; m0 += TB) {
+        f32x16 acc[2][2] = {};
+        tile_product<T, true, true>(acc, W, X, m0, n0, 0, p.D, la, lb);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int64_t t = n0 + wn + 32 * j + (lane & 31);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
+                    float z = acc[i][j][r];
+                    if (bias && v < p.V) z += (float)bias[v];
+                    if (v >= p.V) z = -INFINITY;
+                    if (v == y[j]) {
+                        z_target[t] = z;
+                        z = -INFINITY;
+                    }
+                    acc[i][j][r] = z;
+                    top = fmaxf(top, z);
+                }
+            const float m = fmaxf(run[j].m, top), base = m == -INFINITY ? 0.f : m;
+            float s = run[j].s * exp2f((run[j].m - base) * LOG2E);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += exp2f((acc[i][j][r] - base) * LOG2E);
+            run[j] = Running{m, s};
+        }
+    }
+    __syncthreads();
+    Running* sh = reinterpret_cast<Running*>(la);                // [2 waves along the vocabulary][128 tokens]
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const Running o{__shfl_xor(run[j].m, 32, 64), __shfl_xor(run[j].s, 32, 64)};
+        const Running both = half ? joined(o, run[j]) : joined(run[j], o);
+        if (half == 0) sh[(wave >> 1) * TB + wn + 32 * j + lane] = both;
+    }
+    __syncthreads();
+    const int64_t t = n0 + threadIdx.x;
+    if (threadIdx.x < TB && t < p.T) part[(int64_t)blockIdx.y * p.T + t] = joined(sh[threadIdx.x], sh[TB + threadIdx.x]);
+}
+
+// One wave per row: the splits' sums joined, the row's loss, lse and q
+__global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits, const float* __restrict__ z_target,
+                                                   float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ rest, int32_t* oob)
+{
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (t >= p.T) return;
+    Running r{-INFINITY, 0.f};
+    for (int64_t s = lane; s < splits; s += 64) r = joined(r, part[s * p.T + t]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const Running o{__shfl_xor(r.m, d, 64), __shfl_xor(r.s, d, 64)};
+        r = (lane & d) ? joined(o, r) : joined(r, o);
+    }
+    if (lane) return;
+    const int64_t y = p.target[t];
+    if (y == p.ignore) {
+        loss[t] = 0.f;
+        lse[t] = 0.f;
+        rest[t] = 0.f;
+        return;
+    }
+    if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
+    const float zt = z_target[t], others = r.m + logf(r.s), d = others - zt;
+    // log(1 + e^d) from the smaller of e^d and e^-d; a target at -inf leaves the others' sum, another row of -inf alone is NaN
+    const float e = expf(-fabsf(d)), l = log1pf(e);
+    loss[t] = d > 0.f ? d + l : l;
+    lse[t] = d > 0.f ? others + l : zt + l;
+    rest[t] = d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
+    if (d != d || zt == INFINITY) loss[t] = lse[t] = rest[t] = NAN;
+}
+
+// One workgroup: number of rows that count, and the reduced loss (mean: NaN when none counts, as 0 / 0 is)
+constexpr int REDUCE_NONE = 0, REDUCE_MEAN = 1, REDUCE_SUM = 2;
+
+__device__ __forceinline__ float block_sum(float v, float* sh)
+{
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = 0.f;
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) r += sh[w];
+    __syncthreads();
+    return r;
+}
+
+__global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __restrict__ rows, int reduction, float* __restrict__ out)
+{
+    __shared__ float sh[16];
+    float sum = 0.f, count = 0.f;
+    for (int64_t t = threadIdx.x; t < p.T; t += 1024) {
+        sum += rows[t];
+        count += p.target[t] != p.ignore ? 1.f : 0.f;
+    }
+    sum = block_sum(sum, sh);
+    count = block_sum(count, sh);
+    if (threadIdx.x == 0) *out = reduction == REDUCE_MEAN ? sum / count : sum;
+}
+
+// One workgroup: every row's weight g_t as gn[t] * scale, |gn| <= 1 and scale's size a power of two (sum, mean: gn is 1 and scale
+// the incoming gradient, over the count for the mean), so that G keeps its digits in 16 bits whatever the weights' size is.
+__global__ __launch_bounds__(1024) void weights_kernel(Problem p, int reduction, const float* __restrict__ dloss, float* __restrict__ gn,
+                                                       float* __restrict__ scale)
+{
+    __shared__ float sh[16];
+    if (reduction == REDUCE_NONE) {
+        float top = 0.f;
+        for (int64_t t = threadIdx.x; t < p.T; t += 1024)
+            if (p.target[t] != p.ignore) top = fmaxf(top, fabsf(dloss[t]));
+#pragma unroll
+        for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < 16; ++w) top = fmaxf(top, sh[w]);
+        float unit = 1.f;
+        if (top > 0.f && top < INFINITY) {
+            int e;
+            (void)frexpf(top, &e);                       // top = f 2^e with f in [0.5, 1)
+            unit = ldexpf(1.f, e < -120 ? -120 : e > 127 ? 127 : e);
+        }
+        for (int64_t t = threadIdx.x; t < p.T; t += 1024) gn[t] = p.target[t] != p.ignore ? dloss[t] / unit : 0.f;
+        if (threadIdx.x == 0) *scale = unit;
+        return;
+    }
+    float count = 0.f;
+    for (int64_t t = threadIdx.x; t < p.T; t += 1024) {
+        const bool in = p.target[t] != p.ignore;
+        gn[t] = in ? 1.f : 0.f;
+        count += in ? 1.f : 0.f;
+    }
+    count = block_sum(count, sh);
+    if (threadIdx.x == 0) *scale = reduction == REDUCE_MEAN ? (count > 0.f ? *dloss / count : 0.f) : *dloss;
+}
+
+// G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero
+template <typename T>
+__global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t width, const float* __restrict__ lse, const float* __restrict__ rest,
+                                                const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
+{
+    __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
+    __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr, 0}, X{(const T*)p.x, p.ldx, p.T, nullptr, 0};
+    const T* bias = (const T*)p.bias;
+    const int64_t n0 = (int64_t)blockIdx.x * TB, m0 = v0 + (int64_t)blockIdx.y * TB;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    f32x16 acc[2][2] = {};
+    tile_product<T, true, true>(acc, W, X, m0, n0, 0, p.D, la, lb);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t t = n0 + wn + 32 * j + (lane & 31);
+        if (t >= p.T) continue;
+        const int64_t y0 = p.target[t];
+        const bool in = y0 != p.ignore;
+        const int64_t y = clamp_target(y0, p.V);
+        const float l = lse[t], q = rest[t], g = gn[t] * Traits<T>::G_SCALE;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int64_t v = m0 + wm + 32 * i + 8 * r4 + 4 * half;
+                if (v - v0 >= ldg) continue;
+                Pack<T, 4> o;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float z = acc[i][j][4 * r4 + u];
+                    if (bias && v + u < p.V) z += (float)bias[v + u];
+                    const float e = v + u == y ? -q : exp2f((z - l) * LOG2E);
+                    o.v[u] = (T)(in && v + u < p.V ? e * g : 0.f);
+                }
+                *reinterpret_cast<Pack<T, 4>*>(G + t * ldg + (v - v0)) = o;
+            }
+    }
+}
+
+// Slice blockIdx.z of out [slices][M][N] (+)= A B over its share of k, in 32 bits
+template <typename T, bool AKC, bool BKC>
+__global__ __launch_bounds__(256) void product_kernel(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t K, int64_t k_per_slice, float* out, int add)
+{
+    __shared__ __attribute__((aligned(16))) T la[Stage<T, AKC>::SIZE];
+    __shared__ __attribute__((aligned(16))) T lb[Stage<T, BKC>::SIZE];
+    const int64_t m0 = (int64_t)blockIdx.x * TB, n0 = (int64_t)blockIdx.y * TB;
+    const int64_t k0 = blockIdx.z * k_per_slice, k1 = k0 + k_per_slice < K ? k0 + k_per_slice : K;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    f32x16 acc[2][2] = {};
+    tile_product<T, AKC, BKC>(acc, A, B, m0, n0, k0, k1, la, lb);
+    out += blockIdx.z * M * N;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t m = m0 + wm + 32 * i + acc_row(r, half), n = n0 + wn + 32 * j + (lane & 31);
+                if (m < M && n < N) {
+                    float* o = out + m * N + n;
+                    *o = add ? *o + acc[i][j][r] : acc[i][j][r];
+                }
+            }
+}
+
+// out[i] = scale / G_SCALE * sum over slices, rounded to T
+template <typename T>
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int slices, int64_t n, const float* __restrict__ scale, T* __restrict__ out)
+{
+    const float f = *scale / Traits<T>::G_SCALE;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float s = 0.f;
+        for (int k = 0; k < slices; ++k) s += part[k * n + i];
+        out[i] = (T)(s * f);
+    }
+}
+
+// column sums of G, [slices][width] in 32 bits: slice blockIdx.y takes rows [y * rows_per, ...)
+template <typename T>
+__global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ G, int64_t ldg, int64_t T_rows, int64_t rows_per, int64_t width, float* __restrict__ out)
+{
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t0 = blockIdx.y * rows_per, t1 = t0 + rows_per < T_rows ? t0 + rows_per : T_rows;
+    if (v >= width) return;
+    float s = 0.f;
+    for (int64_t t = t0; t < t1; ++t) s += (float)G[t * ldg + v];
+    out[blockIdx.y * width + v] = s;
+}
+
+// rows with their width filled up to `ldo` with zeros
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ in, int64_t rows, int64_t ld, int64_t D, T* __restrict__ out, int64_t ldo)
+{
+    const int64_t n = rows * ldo;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / ldo, c = i - r * ldo;
+        out[i] = c < D ? in[r * ld + c] : (T)0.f;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void zero_kernel(T* out, int64_t n)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (T)0.f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+struct Carve {
+    char* base;
+    size_t used = 0;
+    void* take(size_t bytes)
+    {
+        void* p = base ? base + used : nullptr;
+        used += align_up(bytes, 256);
+        return p;
+    }
+};
+
+unsigned stream_blocks(int64_t n)
+{
+    const int64_t b = ceil_div64(n, 256);
+    return (unsigned)(b < 1 ? 1 : b > 4096 ? 4096 : b);
+}
+
+int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+struct Args {
+    const void* x; int64_t ldx;
+    const void* w; int64_t ldw;
+    const void* bias;
+    int dtype;
+    int64_t T, V, D;
+    const int64_t* target;
+    int64_t ignore;
+};
+
+// Rows as the kernels read them: as they are, or copied with their width filled up, where a row does not start on 16 bytes or its
+// width is no whole number of 16-byte groups.
+bool must_pack(const void* p, int64_t ld, int64_t D, int size) { return (uintptr_t)p % 16 || ld * size % 16 || D * size % 16; }
+
+struct ForwardPlan {
+    int64_t splits, tiles_per_split;
+};
+
+ForwardPlan forward_plan(int64_t T, int64_t V)
+{
+    const int64_t tiles = ceil_div64(V, TB), rows = ceil_div64(T, TB);
+    ForwardPlan f;
+    f.splits = clamp64(1024 / rows, 1, tiles);
+    f.tiles_per_split = ceil_div64(tiles, f.splits);
+    f.splits = ceil_div64(tiles, f.tiles_per_split);
+    return f;
+}
+
+struct BackwardPlan {
+    int64_t width;                    // vocabulary rows per piece, a multiple of TB
+    int64_t x_slices, w_slices, b_slices;
+    int64_t x_per, w_per, b_per;      // k per slice
+};
+
+constexpr size_t PIECE_BYTES = (size_t)64 << 20;
+
+BackwardPlan backward_plan(int64_t T, int64_t V, int64_t D, int size)
+{
+    BackwardPlan b;
+    const int64_t tiles = ceil_div64(V, TB);
+    // the piece of G, and the 32-bit rows of dW that belong to it
+    const int64_t by_g = (int64_t)(PIECE_BYTES / ((size_t)T * size)) / TB, by_w = (int64_t)(4 * PIECE_BYTES / ((size_t)D * 4)) / TB;
+    b.width = clamp64(by_g < by_w ? by_g : by_w, 1, tiles < 32768 ? tiles : 32768) * TB;
+    const int64_t dt = ceil_div64(D, TB), tt = ceil_div64(T, TB);
+    b.x_slices = clamp64(512 / (tt * dt), 1, b.width / TB);
+    b.x_per = ceil_div64(b.width / TB, b.x_slices) * TB;
+    b.x_slices = ceil_div64(b.width, b.x_per);
+    b.w_slices = clamp64(512 / (b.width / TB * dt), 1, tt);
+    b.w_per = ceil_div64(tt, b.w_slices) * TB;
+    b.w_slices = ceil_div64(T, b.w_per);
+    b.b_slices = clamp64(512 / ceil_div64(b.width, 256), 1, tt);
+    b.b_per = ceil_div64(T, b.b_slices);
+    b.b_slices = ceil_div64(T, b.b_per);
+    return b;
+}
+
+template <typename T> int pack_rows(const Args& a, Problem& p, Carve& c, bool launch, hipStream_t s)
+{
+    const int64_t padded = ceil_div64(a.D, Traits<T>::VEC) * Traits<T>::VEC;
+    p = Problem{a.T, a.V, padded, a.ldx, a.ldw, a.x, a.w, a.bias, a.target, a.ignore};
+    struct { const void** p; int64_t* ld; int64_t rows; } in[2] = {{&p.x, &p.ldx, a.T}, {&p.w, &p.ldw, a.V}};
+    for (auto& m : in) {
+        if (!must_pack(*m.p, *m.ld, a.D, sizeof(T))) continue;
+        T* to = (T*)c.take((size_t)m.rows * padded * sizeof(T));
+        if (launch) {
+            hipLaunchKernelGGL(pack_kernel<T>, dim3(stream_blocks(m.rows * padded)), dim3(256), 0, s, (const T*)*m.p, m.rows, *m.ld, a.D, to, padded);
+            RECO_CHECK_LAUNCH();
+            *m.p = to;
+            *m.ld = padded;
+        }
+    }
+    return RECO_OK;
+}
+
+template <typename T> int forward(const Args& a, int reduction, float* loss, float* state, int32_t* oob, char* ws, size_t* need, hipStream_t s)
+{
+    Carve c{ws};
+    Problem p;
+    const bool launch = ws != nullptr;
+    const ForwardPlan f = forward_plan(a.T, a.V);
+    Running* part = (Running*)c.take((size_t)f.splits * a.T * sizeof(Running));
+    float* z_target = (float*)c.take((size_t)a.T * 4);
+    float* rows = (float*)c.take((size_t)a.T * 4);
+    const int rc = pack_rows<T>(a, p, c, launch, s);
+    if (rc) return rc;
+    *need = c.used;
+    if (!launch) return RECO_OK;
+    if (reduction == REDUCE_NONE) rows = loss;
+    hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)ceil_div64(a.T, TB), (unsigned)f.splits), dim3(256), 0, s, p, f.tiles_per_split, part, z_target);
+    hipLaunchKernelGGL(rows_kernel, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, f.splits, z_target, rows, state, state + a.T, oob);
+    if (reduction != REDUCE_NONE) hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, s, p, rows, reduction, loss);
+    RECO_CHECK_LAUNCH();
+    return RECO_OK;
+}
+
+template <typename T>
+int backward(const Args& a, int reduction, const float* state, const float* dloss, void* dx, void* dw, void* db, char* ws, size_t* need, hipStream_t s)
+{
+    Carve c{ws};
+    Problem p;
+    const bool launch = ws != nullptr;
+    const BackwardPlan b = backward_plan(a.T, a.V, a.D, sizeof(T));
+    float* gn = (float*)c.take((size_t)a.T * 4);
+    float* scale = (float*)c.take(4);
+    T* G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
+    float* x_part = (float*)c.take((size_t)b.x_slices * a.T * a.D * 4);
+    float* w_part = (float*)c.take((size_t)b.w_slices * b.width * a.D * 4);
+    float* b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
+    const int rc = pack_rows<T>(a, p, c, launch, s);
+    if (rc) return rc;
+    *need = c.used;
+    if (!launch) return RECO_OK;
+    const float *lse = state, *rest = state + a.T;
+    const unsigned tt = (unsigned)ceil_div64(a.T, TB), dt = (unsigned)ceil_div64(a.D, TB);
+    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, s, p, reduction, dloss, gn, scale);
+    for (int64_t v0 = 0; v0 < a.V; v0 += b.width) {
+        const int64_t width = a.V - v0 < b.width ? a.V - v0 : b.width, ldg = ceil_div64(width, TB) * TB;
+        hipLaunchKernelGGL(g_kernel<T>, dim3(tt, (unsigned)(ldg / TB)), dim3(256), 0, s, p, v0, width, lse, rest, gn, G, ldg);
+        if (dx) {
+            // a slice without k of this (shorter) piece adds nothing; the first piece, which sets the slices, has k for all
+            const Operand<T> A{G, ldg, a.T, nullptr, 0}, B{(const T*)p.w + v0 * p.ldw, p.ldw, p.D, nullptr, 0};
+            hipLaunchKernelGGL((product_kernel<T, true, false>), dim3(tt, dt, (unsigned)b.x_slices), dim3(256), 0, s, A, B, a.T, a.D, width, b.x_per, x_part,
+                               v0 > 0);
+        }
+        if (dw) {
+            const Operand<T> A{G, ldg, ldg, nullptr, 0}, B{(const T*)p.x, p.ldx, p.D, p.target, p.ignore};
+            hipLaunchKernelGGL((product_kernel<T, false, false>), dim3((unsigned)(ldg / TB), dt, (unsigned)b.w_slices), dim3(256), 0, s, A, B, width, a.D, a.T,
+                               b.w_per, w_part, 0);
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width * a.D)), dim3(256), 0, s, w_part, (int)b.w_slices, width * a.D, scale,
+                               (T*)dw + v0 * a.D);
+        }
+        if (db) {
+            hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(width, 256), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per, width,
+                               b_part);
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, width, scale, (T*)db + v0);
+        }
+        RECO_CHECK_LAUNCH();
+    }
+    if (dx) hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, x_part, (int)b.x_slices, a.T * a.D, scale, (T*)dx);
+    RECO_CHECK_LAUNCH();
+    return RECO_OK;
+}
+
+int check_args(const char* what, const Args& a, int reduction)
+{
+    RECO_REQUIRE(a.dtype >= RECO_DT_F32 && a.dtype <= RECO_DT_F16, "%s: unknown element type %d", what, a.dtype);
+    RECO_REQUIRE(a.T > 0 && a.T < (int64_t)1 << 31 && a.V > 0 && a.V < (int64_t)1 << 31 && a.D > 0 && a.D <= 1 << 20,
+                 "%s: bad sizes: %lld rows, %lld columns, width %lld", what, (long long)a.T, (long long)a.V, (long long)a.D);
+    RECO_REQUIRE(a.x && a.w && a.target, "%s: null pointer", what);
+    RECO_REQUIRE(a.ldx >= a.D && a.ldw >= a.D, "%s: row strides %lld / %lld below the width %lld", what, (long long)a.ldx, (long long)a.ldw, (long long)a.D);
+    RECO_REQUIRE(reduction >= REDUCE_NONE && reduction <= REDUCE_SUM, "%s: unknown reduction %d", what, reduction);
+    return RECO_OK;
+}
+
+}  // namespace
+
+extern "C" size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D)
+{
+    if (T <= 0 || V <= 0 || D <= 0) return 0;
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
+    size_t need = 0;
+    (void)reco_with_type(dtype, [&](auto z) -> int { return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, &need, nullptr); });
+    return need;
+}
+
+extern "C" int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
+                                const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, int32_t* oob,
+                                void* ws, size_t ws_bytes, void* stream)
+{
+    const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
+    const int rc = check_args("linear_xent", a, reduction);
+    if (rc) return rc;
+    RECO_REQUIRE(loss && state && ws && (uintptr_t)ws % 16 == 0, "linear_xent: null or misaligned loss, state or workspace");
+    const size_t need = reco_linear_xent_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D);
+    if (ws_bytes < need) {
+        reco_set_error("linear_xent: workspace of %zu bytes, %zu needed", ws_bytes, need);
+        return RECO_ENOMEM;
+    }
+    ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
+    size_t used = 0;
+    return reco_with_type(dtype, [&](auto z) -> int { return forward<decltype(z)>(a, reduction, loss, state, oob, (char*)ws, &used, (hipStream_t)stream); });
+}
+
+extern "C" size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D)
+{
+    if (T <= 0 || V <= 0 || D <= 0) return 0;
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
+    size_t need = 0;
+    (void)reco_with_type(dtype, [&](auto z) -> int {
+        return backward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &need, nullptr);
+    });
+    return need;
+}
+
+extern "C" int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
+                                     const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dloss,
+                                     void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream)
+{
+    const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
+    const int rc = check_args("linear_xent_grad", a, reduction);
+    if (rc) return rc;
+    RECO_REQUIRE(state && dloss && ws && (uintptr_t)ws % 16 == 0, "linear_xent_grad: null or misaligned state, gradient or workspace");
+    const size_t need = reco_linear_xent_grad_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D);
+    if (ws_bytes < need) {
+        reco_set_error("linear_xent_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
+        return RECO_ENOMEM;
+    }
+    if (!dx && !dw && !db) return RECO_OK;
+    ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
+    size_t used = 0;
+    return reco_with_type(dtype, [&](auto z) -> int {
+        return backward<decltype(z)>(a, reduction, state, dloss, dx, dw, db, (char*)ws, &used, (hipStream_t)stream);
+    });
+}

@@ -474,6 +474,121 @@ def autorec_forward(x, we, be, wd, bd, clamp=None, precision=None):
 
 
 # ----------------------------------------------------------------------------------------------
+# K-g softmax cross entropy over a whole catalogue
+# ----------------------------------------------------------------------------------------------
+REDUCTIONS = {"none": _lib.XENT_NONE, "mean": _lib.XENT_MEAN, "sum": _lib.XENT_SUM}
+
+
+def _xent_args(x, weight, target, bias, reduction, ignore_index):
+    """(x, weight, target, bias) as the C ABI takes them; every extent that it assumes is checked here."""
+    if reduction not in REDUCTIONS:
+        raise ValueError("reduction must be one of %s, got %r" % (sorted(REDUCTIONS), reduction))
+    if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
+        raise TypeError("ignore_index must be an int, got %r" % (ignore_index,))
+    x, weight = _rows(x, "input"), _rows(weight, "weight")
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError("weight must be %s on %s like the input, got %s on %s" % (x.dtype, x.device, weight.dtype, weight.device))
+    if weight.shape[1] != x.shape[1]:
+        raise ValueError("mat1 and mat2 shapes cannot be multiplied (%dx%d and %dx%d)" % (tuple(x.shape) + tuple(weight.shape)[::-1]))
+    if weight.numel() == 0:
+        raise ValueError("weight must have rows and columns, got shape %s" % (tuple(weight.shape),))
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.device != x.device or tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError("bias must be a %s tensor of %d entries on %s" % (x.dtype, weight.shape[0], x.device))
+        bias = bias.detach().contiguous()
+    target = _i64(target, "target", x.device)
+    if target.numel() != x.shape[0]:
+        raise ValueError("target has %d entries for %d rows" % (target.numel(), x.shape[0]))
+    return x, weight, target, bias
+
+
+def _xent(x, weight, target, bias, reduction, ignore_index, check_ids):
+    """(loss, state) of checked operands."""
+    T, D = x.shape
+    dev = x.device
+    loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    state = torch.empty(2 * T, dtype=torch.float32, device=dev)
+    if T == 0:
+        return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), state
+    oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
+    L = _lib.lib()
+    what = (_p(x), _ld(x), _p(weight), _ld(weight))
+    nbytes = L.reco_linear_xent_workspace_bytes(*what, DTYPES[x.dtype], T, weight.shape[0], D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(L.reco_linear_xent(*what, _p(bias), DTYPES[x.dtype], T, weight.shape[0], D, _p(target), ignore_index, REDUCTIONS[reduction], _p(loss),
+                                 _p(state), _p(oob), _p(ws), nbytes, _stream(dev)))
+    if check_ids and int(oob.item()):
+        raise IndexError("index out of range in self")
+    return loss, state
+
+
+def _xent_grad(x, weight, target, bias, state, dloss, reduction, ignore_index, wanted):
+    T, D = x.shape
+    V, dev = weight.shape[0], x.device
+    out = [torch.empty(s, dtype=x.dtype, device=dev) if w else None for w, s in zip(wanted, ((T, D), (V, D), (V,)))]
+    if T == 0:
+        return [o if o is None else o.zero_() for o in out]
+    L = _lib.lib()
+    what = (_p(x), _ld(x), _p(weight), _ld(weight))
+    nbytes = L.reco_linear_xent_grad_workspace_bytes(*what, DTYPES[x.dtype], T, V, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(L.reco_linear_xent_grad(*what, _p(bias), DTYPES[x.dtype], T, V, D, _p(target), ignore_index, REDUCTIONS[reduction], _p(state), _p(dloss),
+                                      _p(out[0]), _p(out[1]), _p(out[2]), _p(ws), nbytes, _stream(dev)))
+    return out
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, reduction, ignore_index, check_ids):
+        xr, wr, target, br = _xent_args(x, weight, target, bias, reduction, ignore_index)
+        loss, state = _xent(xr, wr, target, br, reduction, ignore_index, check_ids)
+        ctx.save_for_backward(x, weight, bias, target, state)
+        ctx.reduction, ctx.ignore_index = reduction, ignore_index
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        _no_captured_graph("linear_cross_entropy's backward pass", "linear_cross_entropy_grad")
+        x, weight, bias, target, state = ctx.saved_tensors
+        bias = None if bias is None else bias.contiguous()
+        grads = _xent_grad(_rows(x, "input"), _rows(weight, "weight"), target, bias, state, dloss.contiguous(), ctx.reduction, ctx.ignore_index,
+                           ctx.needs_input_grad[:3])
+        return tuple(grads) + (None,) * 4
+
+
+def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, check_ids=True):
+    """cross_entropy(x @ weight.T + bias, target) over a whole catalogue without its [T, V] logits in memory, differentiable in x,
+    weight and bias.
+
+    x [T, D], weight [V, D], bias [V] (may hold -inf: items never offered) of one type, float32 / bfloat16 / float16; target integers
+    [T]; rows whose target is ignore_index have no loss and no gradient.  The loss is float32: [T] for reduction "none" (0 for ignored
+    rows), else a scalar ("mean" over the rows that count is NaN when there is none, as in torch).  Out-of-range targets raise
+    IndexError; check_ids=False skips that report (one device-to-host sync) and clamps them.  Inside a HIP graph: under no_grad with
+    check_ids=False, and linear_cross_entropy_grad for the gradients.
+    """
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
+        _no_captured_graph("linear_cross_entropy", "linear_cross_entropy_grad")
+        return _LinearCrossEntropy.apply(x, weight, bias, target, reduction, ignore_index, check_ids)
+    return _xent(*_xent_args(x, weight, target, bias, reduction, ignore_index), reduction, ignore_index, check_ids)[0]
+
+
+def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ignore_index=-100, grad=None):
+    """(loss, dx, dweight, dbias) in one call, without autograd (dbias is None without a bias); may be captured into a HIP graph.
+    grad: the incoming gradient, float32 of the loss' shape (None: ones).  Targets are clamped, not checked."""
+    x, weight, target, bias = _xent_args(x, weight, target, bias, reduction, ignore_index)
+    shape = (x.shape[0],) if reduction == "none" else ()
+    if grad is None:
+        grad = torch.ones(shape, dtype=torch.float32, device=x.device)
+    elif not isinstance(grad, torch.Tensor) or grad.dtype != torch.float32 or grad.device != x.device or tuple(grad.shape) != shape:
+        raise ValueError("grad must be a float32 tensor of shape %s on %s" % (shape, x.device))
+    loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False)
+    return (loss, *_xent_grad(x, weight, target, bias, state, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
+
+
+# ----------------------------------------------------------------------------------------------
 # K-d top-k
 # ----------------------------------------------------------------------------------------------
 def topk_rows(scores, k, exclude=None):
