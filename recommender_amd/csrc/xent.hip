@@ -14,41 +14,11 @@
 // is held times 2^14, so that probabilities down to 2^-28 are normal numbers.
 //
 // This file: the form for every width.  A piece of G, [T, piece] in the operands' type, is written and read by two matrix products.
-#include "types16.h"
-
-#include <type_traits>
+#include "xent_shared.h"
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
-
-template <typename T> struct Traits;
-template <> struct Traits<float> {
-    static constexpr int VEC = 4, KSTEP = 8, BK = 32;
-    static constexpr float G_SCALE = 1.f;
-    typedef f32x4 frag;
-};
-template <> struct Traits<__bf16> {
-    static constexpr int VEC = 8, KSTEP = 16, BK = 64;
-    static constexpr float G_SCALE = 1.f;
-    typedef bf16x8 frag;
-};
-template <> struct Traits<_Float16> {
-    static constexpr int VEC = 8, KSTEP = 16, BK = 64;
-    static constexpr float G_SCALE = 16384.f;
-    typedef f16x8 frag;
-};
-
-// acc[m, n] += sum over KSTEP k of a[m, k] b[n, k].  Lane l holds m (n) = l % 32; its k are 8 (l / 32) + 0 .. 7 of 16, in 32 bits
-// 4 (l / 32) + 0 .. 3 of 8 -- the order of k is free as long as both operands have the same.  The result: n = l % 32, m of
-// register r is 8 (r / 4) + 4 (l / 32) + r % 4.
-__device__ __forceinline__ void mma(f32x16& acc, const f32x4& a, const f32x4& b)
-{
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(f32x16& acc, const bf16x8& a, const bf16x8& b) { acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
-__device__ __forceinline__ void mma(f32x16& acc, const f16x8& a, const f16x8& b) { acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); }
+using namespace xent;
 
 // ---------------------------------------------------------------------------------------------
 // a 128 x 128 tile of a matrix product: 4 waves, 64 x 64 each; operands staged through LDS, the next step's in registers meanwhile
@@ -61,8 +31,7 @@ template <typename T> struct Operand {
     const T* p;
     int64_t ld;
     int64_t rows;
-    const int64_t* keep;      // !KC: k rows whose keep[k] == drop are read as zeros (nullable)
-    int64_t drop;
+    const int* keep;          // !KC: k rows whose keep[k] is negative are read as zeros (nullable)
 };
 
 template <typename T, bool KC> struct Stage {
@@ -80,7 +49,7 @@ template <typename T, bool KC> struct Stage {
             const int c = threadIdx.x + 256 * i, row = c / PER_ROW, col = (c % PER_ROW) * VEC;
             const int64_t r = r0 + (KC ? row : col), k = k0 + (KC ? col : row);
             bool ok = r < o.rows && k < k_end;
-            if (!KC && ok && o.keep) ok = o.keep[k] != o.drop;
+            if (!KC && ok && o.keep) ok = o.keep[k] >= 0;
             if (ok) {
                 reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(o.p + (KC ? r * o.ld + k : k * o.ld + r));
             } else {
@@ -156,38 +125,12 @@ __device__ __forceinline__ void tile_product(f32x16 (&acc)[2][2], const Operand<
     }
 }
 
-__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
-
-struct Problem {
-    int64_t T, V, D;            // D: values per row as read (whole VEC groups, zeros behind the caller's width)
-    int64_t ldx, ldw;
-    const void* x;
-    const void* w;
-    const void* bias;           // nullable
-    const int64_t* target;
-    int64_t ignore;
-};
-
-__device__ __forceinline__ int64_t clamp_target(int64_t y, int64_t V) { return y < 0 ? 0 : y >= V ? V - 1 : y; }
-
-// (m, s): running maximum and sum of exp(z - m) of the logits that are not the target's
-struct Running { float m, s; };
-
-__device__ __forceinline__ Running joined(Running a, Running b)
-{
-    Running r;
-    r.m = fmaxf(a.m, b.m);
-    const float base = r.m == -INFINITY ? 0.f : r.m;            // nothing but -inf so far: the sum stays 0
-    r.s = a.s * exp2f((a.m - base) * LOG2E) + b.s * exp2f((b.m - base) * LOG2E);
-    return r;
-}
-
 template <typename T>
 __global__ __launch_bounds__(256) void stats_kernel(Problem p, int64_t tiles_per_split, Running* __restrict__ part, float* __restrict__ z_target)
 {
     __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
     __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
-    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr, 0}, X{(const T*)p.x, p.ldx, p.T, nullptr, 0};
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr}, X{(const T*)p.x, p.ldx, p.T, nullptr};
     const T* bias = (const T*)p.bias;
     const int64_t n0 = (int64_t)blockIdx.x * TB;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -246,13 +189,23 @@ __global__ __launch_bounds__(256) void stats_kernel(Problem p, int64_t tiles_per
     if (threadIdx.x < TB && t < p.T) part[(int64_t)blockIdx.y * p.T + t] = joined(sh[threadIdx.x], sh[TB + threadIdx.x]);
 }
 
-// One wave per row: the splits' sums joined, the row's loss, lse and q
+// One wave per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
+// sums of W [splits][T][D_out], also dx for an incoming gradient of one, in 32 bits.
+template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits, const float* __restrict__ z_target,
-                                                   float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ rest, int32_t* oob)
+                                                   float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
+                                                   const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
 {
     const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (t >= p.T) return;
+    const int64_t y = p.target[t];
+    if (y == p.ignore) {
+        if (lane == 0) loss[t] = lse[t] = rest[t] = 0.f;
+        if (dx_unit)
+            for (int64_t d = lane; d < D_out; d += 64) dx_unit[t * D_out + d] = 0.f;
+        return;
+    }
     Running r{-INFINITY, 0.f};
     for (int64_t s = lane; s < splits; s += 64) r = joined(r, part[s * p.T + t]);
 #pragma unroll
@@ -260,26 +213,33 @@ __global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __r
         const Running o{__shfl_xor(r.m, d, 64), __shfl_xor(r.s, d, 64)};
         r = (lane & d) ? joined(o, r) : joined(r, o);
     }
-    if (lane) return;
-    const int64_t y = p.target[t];
-    if (y == p.ignore) {
-        loss[t] = 0.f;
-        lse[t] = 0.f;
-        rest[t] = 0.f;
-        return;
-    }
-    if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
     const float zt = z_target[t], others = r.m + logf(r.s), d = others - zt;
-    // log(1 + e^d) from the smaller of e^d and e^-d; a target at -inf leaves the others' sum, another row of -inf alone is NaN
+    // log(1 + e^d) from the smaller of e^d and e^-d; a target at -inf leaves the others' sum, a row of -inf alone is NaN
     const float e = expf(-fabsf(d)), l = log1pf(e);
-    loss[t] = d > 0.f ? d + l : l;
-    lse[t] = d > 0.f ? others + l : zt + l;
-    rest[t] = d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
-    if (d != d || zt == INFINITY) loss[t] = lse[t] = rest[t] = NAN;
+    const bool none = d != d || zt == INFINITY;
+    const float whole = none ? NAN : d > 0.f ? others + l : zt + l;
+    const float q = none ? NAN : d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
+    if (lane == 0) {
+        if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
+        loss[t] = none ? NAN : d > 0.f ? d + l : l;
+        lse[t] = whole;
+        rest[t] = q;
+    }
+    if (!dx_unit) return;
+    const T* w = (const T*)p.w + clamp_target(y, p.V) * p.ldw;
+    for (int64_t c = lane; c < D_out; c += 64) {
+        float sum = 0.f;
+        for (int64_t s = 0; s < splits; ++s) {
+            const float m = part[s * p.T + t].m;
+            if (m != -INFINITY) sum = fmaf(exp2f((m - whole) * LOG2E), dx_part[(s * p.T + t) * D_out + c], sum);
+        }
+        dx_unit[t * D_out + c] = fmaf(-q, (float)w[c], sum);
+    }
 }
 
-// One workgroup: number of rows that count, and the reduced loss (mean: NaN when none counts, as 0 / 0 is)
-constexpr int REDUCE_NONE = 0, REDUCE_MEAN = 1, REDUCE_SUM = 2;
+// Number of rows that count, and the reduced loss (mean: NaN when none counts, as 0 / 0 is): partial sums per workgroup, joined in
+// their order; one workgroup alone finishes by itself.
+constexpr int REDUCE_NONE = RECO_XENT_NONE, REDUCE_MEAN = RECO_XENT_MEAN, REDUCE_SUM = RECO_XENT_SUM;
 
 __device__ __forceinline__ float block_sum(float v, float* sh)
 {
@@ -293,52 +253,92 @@ __device__ __forceinline__ float block_sum(float v, float* sh)
     return r;
 }
 
-__global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __restrict__ rows, int reduction, float* __restrict__ out)
+// in: the rows' losses (of Problem p), or with p.T = 0 the `parts` (sum, count) of an earlier launch
+__global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __restrict__ rows, const float2* __restrict__ parts, int n_parts, int reduction,
+                                                      float* __restrict__ loss, float* __restrict__ count_out, float2* __restrict__ part_out)
 {
     __shared__ float sh[16];
     float sum = 0.f, count = 0.f;
-    for (int64_t t = threadIdx.x; t < p.T; t += 1024) {
-        sum += rows[t];
-        count += p.target[t] != p.ignore ? 1.f : 0.f;
+    if (parts) {
+        for (int i = threadIdx.x; i < n_parts; i += 1024) {
+            sum += parts[i].x;
+            count += parts[i].y;
+        }
+    } else {
+        for (int64_t t = (int64_t)blockIdx.x * 1024 + threadIdx.x; t < p.T; t += (int64_t)gridDim.x * 1024) {
+            sum += rows[t];
+            count += p.target[t] != p.ignore ? 1.f : 0.f;
+        }
     }
     sum = block_sum(sum, sh);
     count = block_sum(count, sh);
-    if (threadIdx.x == 0) *out = reduction == REDUCE_MEAN ? sum / count : sum;
+    if (threadIdx.x) return;
+    if (gridDim.x > 1) {
+        part_out[blockIdx.x] = float2{sum, count};
+    } else {
+        *loss = reduction == REDUCE_MEAN ? sum / count : sum;
+        *count_out = count;
+    }
 }
 
-// One workgroup: every row's weight g_t as gn[t] * scale, |gn| <= 1 and scale's size a power of two (sum, mean: gn is 1 and scale
-// the incoming gradient, over the count for the mean), so that G keeps its digits in 16 bits whatever the weights' size is.
-__global__ __launch_bounds__(1024) void weights_kernel(Problem p, int reduction, const float* __restrict__ dloss, float* __restrict__ gn,
-                                                       float* __restrict__ scale)
+// Rows' weights in two factors, gn[t] * scale: |gn| < 2 and scale a power of two where every row has a weight of its own, so that G
+// keeps its digits in 16 bits whatever the weights' size is; gn = 1 (NULL) and scale the incoming gradient, over the count for the
+// mean, where it is the same for all.
+__global__ __launch_bounds__(256) void top_kernel(Problem p, const float* __restrict__ dloss, float* __restrict__ tops)
 {
-    __shared__ float sh[16];
+    __shared__ float sh[4];
+    float top = 0.f;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < p.T; t += (int64_t)gridDim.x * 256)
+        if (p.target[t] != p.ignore) top = fmaxf(top, fabsf(dloss[t]));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) tops[blockIdx.x] = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+}
+
+// Also what the gradient kernels read per row: the target as 32 bits (-1: the row does not count), and for the narrow form the constant
+// of its exponentials (see narrow_cols_kernel).
+__global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, const float* __restrict__ dloss, const float* __restrict__ count,
+                                                      const float* __restrict__ tops, int n_tops, const float* __restrict__ lse, float g_log2,
+                                                      float* __restrict__ gn, float* __restrict__ scale, int* __restrict__ y, float* __restrict__ expo)
+{
+    float unit = 1.f;
     if (reduction == REDUCE_NONE) {
         float top = 0.f;
-        for (int64_t t = threadIdx.x; t < p.T; t += 1024)
-            if (p.target[t] != p.ignore) top = fmaxf(top, fabsf(dloss[t]));
+        for (int i = threadIdx.x & 63; i < n_tops; i += 64) top = fmaxf(top, tops[i]);
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-        __syncthreads();
-        for (int w = 0; w < 16; ++w) top = fmaxf(top, sh[w]);
-        float unit = 1.f;
         if (top > 0.f && top < INFINITY) {
             int e;
             (void)frexpf(top, &e);                       // top = f 2^e with f in [0.5, 1)
             unit = ldexpf(1.f, e < -120 ? -120 : e > 127 ? 127 : e);
         }
-        for (int64_t t = threadIdx.x; t < p.T; t += 1024) gn[t] = p.target[t] != p.ignore ? dloss[t] / unit : 0.f;
-        if (threadIdx.x == 0) *scale = unit;
-        return;
+    } else if (reduction == REDUCE_MEAN) {
+        unit = *count > 0.f ? *dloss / *count : 0.f;
+    } else {
+        unit = *dloss;
     }
-    float count = 0.f;
-    for (int64_t t = threadIdx.x; t < p.T; t += 1024) {
-        const bool in = p.target[t] != p.ignore;
-        gn[t] = in ? 1.f : 0.f;
-        count += in ? 1.f : 0.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = unit;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < p.T; t += (int64_t)gridDim.x * 256) {
+        const int64_t target = p.target[t];
+        const bool in = target != p.ignore;
+        y[t] = in ? (int)clamp_target(target, p.V) : -1;
+        if (reduction == REDUCE_NONE) gn[t] = in ? dloss[t] / unit : 0.f;
+        if (p.bias) expo[t] = in ? lse[t] : INFINITY;
+        else expo[t] = in ? fmaf(-LOG2E, lse[t], g_log2) : -INFINITY;
     }
-    count = block_sum(count, sh);
-    if (threadIdx.x == 0) *scale = reduction == REDUCE_MEAN ? (count > 0.f ? *dloss / count : 0.f) : *dloss;
+}
+
+// dx = gn * scale * dx_unit
+template <typename T>
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ unit, int64_t rows, int64_t D, const float* __restrict__ gn,
+                                                 const float* __restrict__ scale, T* __restrict__ dx)
+{
+    const float f = *scale;
+    const int64_t n = rows * D;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        dx[i] = (T)(unit[i] * (gn ? gn[i / D] * f : f));
 }
 
 // G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t w
 {
     __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
     __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
-    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr, 0}, X{(const T*)p.x, p.ldx, p.T, nullptr, 0};
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr}, X{(const T*)p.x, p.ldx, p.T, nullptr};
     const T* bias = (const T*)p.bias;
     const int64_t n0 = (int64_t)blockIdx.x * TB, m0 = v0 + (int64_t)blockIdx.y * TB;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t w
         const int64_t y0 = p.target[t];
         const bool in = y0 != p.ignore;
         const int64_t y = clamp_target(y0, p.V);
-        const float l = lse[t], q = rest[t], g = gn[t] * Traits<T>::G_SCALE;
+        const float l = lse[t], q = rest[t], g = (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -544,58 +544,109 @@ template <typename T> int pack_rows(const Args& a, Problem& p, Carve& c, bool la
     return RECO_OK;
 }
 
-template <typename T> int forward(const Args& a, int reduction, float* loss, float* state, int32_t* oob, char* ws, size_t* need, hipStream_t s)
+constexpr int REDUCE_ROWS = 16384;            // rows that one workgroup reduces by itself
+
+template <typename T>
+int forward(const Args& a, int reduction, float* loss, float* state, float* dx_unit, bool with_dx, int32_t* oob, char* ws, size_t* need, hipStream_t s)
 {
     Carve c{ws};
     Problem p;
-    const bool launch = ws != nullptr;
+    const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
     const ForwardPlan f = forward_plan(a.T, a.V);
-    Running* part = (Running*)c.take((size_t)f.splits * a.T * sizeof(Running));
+    const NarrowPlan n = narrow ? narrow_plan(a.dtype, a.T, a.V, a.D) : NarrowPlan{};
+    const int64_t splits = narrow ? n.x_splits : f.splits;
+    Running* part = (Running*)c.take((size_t)splits * a.T * sizeof(Running));
     float* z_target = (float*)c.take((size_t)a.T * 4);
     float* rows = (float*)c.take((size_t)a.T * 4);
+    float2* sums = (float2*)c.take(256 * sizeof(float2));
+    float* dx_part = narrow && with_dx ? (float*)c.take((size_t)splits * a.T * a.D * 4) : nullptr;
     const int rc = pack_rows<T>(a, p, c, launch, s);
     if (rc) return rc;
     *need = c.used;
     if (!launch) return RECO_OK;
     if (reduction == REDUCE_NONE) rows = loss;
-    hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)ceil_div64(a.T, TB), (unsigned)f.splits), dim3(256), 0, s, p, f.tiles_per_split, part, z_target);
-    hipLaunchKernelGGL(rows_kernel, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, f.splits, z_target, rows, state, state + a.T, oob);
-    if (reduction != REDUCE_NONE) hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, s, p, rows, reduction, loss);
+    if (narrow) {
+        const int rn = narrow_rows(a.dtype, p, n, a.D, part, z_target, dx_part, s);
+        if (rn) return rn;
+    } else {
+        hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)ceil_div64(a.T, TB), (unsigned)splits), dim3(256), 0, s, p, f.tiles_per_split, part, z_target);
+    }
+    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, splits, z_target, rows, state, state + a.T, oob, dx_part, a.D,
+                       dx_part ? dx_unit : nullptr);
+    if (reduction != REDUCE_NONE) {
+        int blocks = (int)clamp64(ceil_div64(a.T, REDUCE_ROWS), 1, 256);
+        hipLaunchKernelGGL(reduce_kernel, dim3(blocks), dim3(1024), 0, s, p, rows, nullptr, 0, reduction, loss, state + 2 * a.T, sums);
+        if (blocks > 1)
+            hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, s, p, rows, sums, blocks, reduction, loss, state + 2 * a.T, nullptr);
+    }
     RECO_CHECK_LAUNCH();
     return RECO_OK;
 }
 
 template <typename T>
-int backward(const Args& a, int reduction, const float* state, const float* dloss, void* dx, void* dw, void* db, char* ws, size_t* need, hipStream_t s)
+int backward(const Args& a, int reduction, const float* state, const float* dx_unit, const float* dloss, void* dx, void* dw, void* db, char* ws, size_t* need,
+             hipStream_t s)
 {
     Carve c{ws};
     Problem p;
-    const bool launch = ws != nullptr;
-    const BackwardPlan b = backward_plan(a.T, a.V, a.D, sizeof(T));
+    const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
     float* gn = (float*)c.take((size_t)a.T * 4);
     float* scale = (float*)c.take(4);
-    T* G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
-    float* x_part = (float*)c.take((size_t)b.x_slices * a.T * a.D * 4);
-    float* w_part = (float*)c.take((size_t)b.w_slices * b.width * a.D * 4);
-    float* b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
+    float* tops = (float*)c.take(256 * 4);
+    int* y = (int*)c.take((size_t)a.T * 4);
+    float* expo = (float*)c.take((size_t)a.T * 4);
+    const NarrowPlan n = narrow ? narrow_plan(a.dtype, a.T, a.V, a.D) : NarrowPlan{};
+    const BackwardPlan b = narrow ? BackwardPlan{} : backward_plan(a.T, a.V, a.D, sizeof(T));
+    T* G = nullptr;
+    float *x_part = nullptr, *w_part = nullptr, *b_part = nullptr;
+    if (narrow) {
+        if (n.w_splits > 1) {
+            w_part = (float*)c.take((size_t)n.w_splits * a.V * a.D * 4);
+            b_part = (float*)c.take((size_t)n.w_splits * a.V * 4);
+        }
+    } else {
+        G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
+        x_part = (float*)c.take((size_t)b.x_slices * a.T * a.D * 4);
+        w_part = (float*)c.take((size_t)b.w_slices * b.width * a.D * 4);
+        b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
+    }
     const int rc = pack_rows<T>(a, p, c, launch, s);
     if (rc) return rc;
     *need = c.used;
     if (!launch) return RECO_OK;
     const float *lse = state, *rest = state + a.T;
+    const int row_blocks = (int)clamp64(ceil_div64(a.T, 256), 1, 256);
+    if (reduction == REDUCE_NONE)
+        hipLaunchKernelGGL(top_kernel, dim3(row_blocks), dim3(256), 0, s, p, dloss, tops);
+    else
+        gn = nullptr;
+    hipLaunchKernelGGL(weights_kernel, dim3(row_blocks), dim3(256), 0, s, p, reduction, dloss, state + 2 * a.T, tops, row_blocks, lse,
+                       log2f(Traits<T>::G_SCALE), gn, scale, y, expo);
+    if (narrow) {
+        if (dw || db) {
+            const int rn = narrow_cols(a.dtype, p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
+            if (rn) return rn;
+            if (n.w_splits > 1 && dw)
+                hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.V * a.D)), dim3(256), 0, s, w_part, (int)n.w_splits, a.V * a.D, scale, (T*)dw);
+            if (n.w_splits > 1 && db)
+                hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.V)), dim3(256), 0, s, b_part, (int)n.w_splits, a.V, scale, (T*)db);
+        }
+        if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, dx_unit, a.T, a.D, gn, scale, (T*)dx);
+        RECO_CHECK_LAUNCH();
+        return RECO_OK;
+    }
     const unsigned tt = (unsigned)ceil_div64(a.T, TB), dt = (unsigned)ceil_div64(a.D, TB);
-    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, s, p, reduction, dloss, gn, scale);
     for (int64_t v0 = 0; v0 < a.V; v0 += b.width) {
         const int64_t width = a.V - v0 < b.width ? a.V - v0 : b.width, ldg = ceil_div64(width, TB) * TB;
         hipLaunchKernelGGL(g_kernel<T>, dim3(tt, (unsigned)(ldg / TB)), dim3(256), 0, s, p, v0, width, lse, rest, gn, G, ldg);
         if (dx) {
             // a slice without k of this (shorter) piece adds nothing; the first piece, which sets the slices, has k for all
-            const Operand<T> A{G, ldg, a.T, nullptr, 0}, B{(const T*)p.w + v0 * p.ldw, p.ldw, p.D, nullptr, 0};
+            const Operand<T> A{G, ldg, a.T, nullptr}, B{(const T*)p.w + v0 * p.ldw, p.ldw, p.D, nullptr};
             hipLaunchKernelGGL((product_kernel<T, true, false>), dim3(tt, dt, (unsigned)b.x_slices), dim3(256), 0, s, A, B, a.T, a.D, width, b.x_per, x_part,
                                v0 > 0);
         }
         if (dw) {
-            const Operand<T> A{G, ldg, ldg, nullptr, 0}, B{(const T*)p.x, p.ldx, p.D, p.target, p.ignore};
+            const Operand<T> A{G, ldg, ldg, nullptr}, B{(const T*)p.x, p.ldx, p.D, y};
             hipLaunchKernelGGL((product_kernel<T, false, false>), dim3((unsigned)(ldg / TB), dt, (unsigned)b.w_slices), dim3(256), 0, s, A, B, width, a.D, a.T,
                                b.w_per, w_part, 0);
             hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width * a.D)), dim3(256), 0, s, w_part, (int)b.w_slices, width * a.D, scale,
@@ -626,46 +677,56 @@ int check_args(const char* what, const Args& a, int reduction)
 
 }  // namespace
 
-extern "C" size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D)
+extern "C" size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D,
+                                                   int with_dx)
 {
     if (T <= 0 || V <= 0 || D <= 0) return 0;
-    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr};
     size_t need = 0;
-    (void)reco_with_type(dtype, [&](auto z) -> int { return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, &need, nullptr); });
+    (void)reco_with_type(dtype, [&](auto z) -> int {
+        return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, with_dx != 0, nullptr, nullptr, &need, nullptr);
+    });
     return need;
 }
 
+extern "C" int64_t reco_linear_xent_dx_floats(int dtype, int64_t T, int64_t D)
+{
+    return T > 0 && D > 0 && dtype >= RECO_DT_F32 && dtype <= RECO_DT_F16 && narrow_fits(dtype, D) ? T * D : 0;
+}
+
 extern "C" int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                                const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, int32_t* oob,
+                                const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, float* dx_unit, int32_t* oob,
                                 void* ws, size_t ws_bytes, void* stream)
 {
     const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
     const int rc = check_args("linear_xent", a, reduction);
     if (rc) return rc;
     RECO_REQUIRE(loss && state && ws && (uintptr_t)ws % 16 == 0, "linear_xent: null or misaligned loss, state or workspace");
-    const size_t need = reco_linear_xent_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D);
+    const size_t need = reco_linear_xent_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D, dx_unit != nullptr);
     if (ws_bytes < need) {
         reco_set_error("linear_xent: workspace of %zu bytes, %zu needed", ws_bytes, need);
         return RECO_ENOMEM;
     }
     ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
     size_t used = 0;
-    return reco_with_type(dtype, [&](auto z) -> int { return forward<decltype(z)>(a, reduction, loss, state, oob, (char*)ws, &used, (hipStream_t)stream); });
+    return reco_with_type(dtype, [&](auto z) -> int {
+        return forward<decltype(z)>(a, reduction, loss, state, dx_unit, dx_unit != nullptr, oob, (char*)ws, &used, (hipStream_t)stream);
+    });
 }
 
 extern "C" size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D)
 {
     if (T <= 0 || V <= 0 || D <= 0) return 0;
-    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr};
     size_t need = 0;
     (void)reco_with_type(dtype, [&](auto z) -> int {
-        return backward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &need, nullptr);
+        return backward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &need, nullptr);
     });
     return need;
 }
 
 extern "C" int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                                     const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dloss,
+                                     const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dx_unit, const float* dloss,
                                      void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream)
 {
     const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
@@ -677,10 +738,11 @@ extern "C" int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, 
         reco_set_error("linear_xent_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
         return RECO_ENOMEM;
     }
+    RECO_REQUIRE(!dx || dx_unit || !narrow_fits(dtype, D), "linear_xent_grad: dx needs the dx_unit that the forward call wrote");
     if (!dx && !dw && !db) return RECO_OK;
     ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
     size_t used = 0;
     return reco_with_type(dtype, [&](auto z) -> int {
-        return backward<decltype(z)>(a, reduction, state, dloss, dx, dw, db, (char*)ws, &used, (hipStream_t)stream);
+        return backward<decltype(z)>(a, reduction, state, dx_unit, dloss, dx, dw, db, (char*)ws, &used, (hipStream_t)stream);
     });
 }

@@ -502,28 +502,30 @@ def _xent_args(x, weight, target, bias, reduction, ignore_index):
     return x, weight, target, bias
 
 
-def _xent(x, weight, target, bias, reduction, ignore_index, check_ids):
-    """(loss, state) of checked operands."""
+def _xent(x, weight, target, bias, reduction, ignore_index, check_ids, with_dx):
+    """(loss, state, dx_unit) of checked operands; with_dx: a gradient of x will be asked for (see reco_linear_xent)."""
     T, D = x.shape
     dev = x.device
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    state = torch.empty(2 * T, dtype=torch.float32, device=dev)
+    state = torch.empty(2 * T + 1, dtype=torch.float32, device=dev)
     if T == 0:
-        return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), state
+        return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), state, None
     oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
     L = _lib.lib()
     what = (_p(x), _ld(x), _p(weight), _ld(weight))
-    nbytes = L.reco_linear_xent_workspace_bytes(*what, DTYPES[x.dtype], T, weight.shape[0], D)
+    floats = L.reco_linear_xent_dx_floats(DTYPES[x.dtype], T, D) if with_dx else 0
+    dx_unit = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    nbytes = L.reco_linear_xent_workspace_bytes(*what, DTYPES[x.dtype], T, weight.shape[0], D, 1 if floats else 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
         check(L.reco_linear_xent(*what, _p(bias), DTYPES[x.dtype], T, weight.shape[0], D, _p(target), ignore_index, REDUCTIONS[reduction], _p(loss),
-                                 _p(state), _p(oob), _p(ws), nbytes, _stream(dev)))
+                                 _p(state), _p(dx_unit), _p(oob), _p(ws), nbytes, _stream(dev)))
     if check_ids and int(oob.item()):
         raise IndexError("index out of range in self")
-    return loss, state
+    return loss, state, dx_unit
 
 
-def _xent_grad(x, weight, target, bias, state, dloss, reduction, ignore_index, wanted):
+def _xent_grad(x, weight, target, bias, state, dx_unit, dloss, reduction, ignore_index, wanted):
     T, D = x.shape
     V, dev = weight.shape[0], x.device
     out = [torch.empty(s, dtype=x.dtype, device=dev) if w else None for w, s in zip(wanted, ((T, D), (V, D), (V,)))]
@@ -534,8 +536,8 @@ def _xent_grad(x, weight, target, bias, state, dloss, reduction, ignore_index, w
     nbytes = L.reco_linear_xent_grad_workspace_bytes(*what, DTYPES[x.dtype], T, V, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
-        check(L.reco_linear_xent_grad(*what, _p(bias), DTYPES[x.dtype], T, V, D, _p(target), ignore_index, REDUCTIONS[reduction], _p(state), _p(dloss),
-                                      _p(out[0]), _p(out[1]), _p(out[2]), _p(ws), nbytes, _stream(dev)))
+        check(L.reco_linear_xent_grad(*what, _p(bias), DTYPES[x.dtype], T, V, D, _p(target), ignore_index, REDUCTIONS[reduction], _p(state), _p(dx_unit),
+                                      _p(dloss), _p(out[0]), _p(out[1]), _p(out[2]), _p(ws), nbytes, _stream(dev)))
     return out
 
 
@@ -543,8 +545,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, reduction, ignore_index, check_ids):
         xr, wr, target, br = _xent_args(x, weight, target, bias, reduction, ignore_index)
-        loss, state = _xent(xr, wr, target, br, reduction, ignore_index, check_ids)
-        ctx.save_for_backward(x, weight, bias, target, state)
+        loss, state, dx_unit = _xent(xr, wr, target, br, reduction, ignore_index, check_ids, ctx.needs_input_grad[0])
+        ctx.save_for_backward(x, weight, bias, target, state, dx_unit)
         ctx.reduction, ctx.ignore_index = reduction, ignore_index
         return loss
 
@@ -552,10 +554,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         _no_captured_graph("linear_cross_entropy's backward pass", "linear_cross_entropy_grad")
-        x, weight, bias, target, state = ctx.saved_tensors
+        x, weight, bias, target, state, dx_unit = ctx.saved_tensors
         bias = None if bias is None else bias.contiguous()
-        grads = _xent_grad(_rows(x, "input"), _rows(weight, "weight"), target, bias, state, dloss.contiguous(), ctx.reduction, ctx.ignore_index,
-                           ctx.needs_input_grad[:3])
+        grads = _xent_grad(_rows(x, "input"), _rows(weight, "weight"), target, bias, state, dx_unit, dloss.contiguous(), ctx.reduction,
+                           ctx.ignore_index, ctx.needs_input_grad[:3])
         return tuple(grads) + (None,) * 4
 
 
@@ -572,7 +574,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
         _no_captured_graph("linear_cross_entropy", "linear_cross_entropy_grad")
         return _LinearCrossEntropy.apply(x, weight, bias, target, reduction, ignore_index, check_ids)
-    return _xent(*_xent_args(x, weight, target, bias, reduction, ignore_index), reduction, ignore_index, check_ids)[0]
+    return _xent(*_xent_args(x, weight, target, bias, reduction, ignore_index), reduction, ignore_index, check_ids, False)[0]
 
 
 def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ignore_index=-100, grad=None):
@@ -584,8 +586,8 @@ def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ig
         grad = torch.ones(shape, dtype=torch.float32, device=x.device)
     elif not isinstance(grad, torch.Tensor) or grad.dtype != torch.float32 or grad.device != x.device or tuple(grad.shape) != shape:
         raise ValueError("grad must be a float32 tensor of shape %s on %s" % (shape, x.device))
-    loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False)
-    return (loss, *_xent_grad(x, weight, target, bias, state, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
+    loss, state, dx_unit = _xent(x, weight, target, bias, reduction, ignore_index, False, True)
+    return (loss, *_xent_grad(x, weight, target, bias, state, dx_unit, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
 
 
 # ----------------------------------------------------------------------------------------------

@@ -24,27 +24,27 @@ def test_c_refusals():
     from recommender_amd import _lib
     L = _lib.lib()
     some = ctypes.c_void_p(256)                              # never read: every call below is refused before a launch
-    ok = dict(x=some, ldx=8, w=some, ldw=8, bias=None, dtype=0, T=4, V=9, D=8, target=some, reduction=1, loss=some, state=some, dloss=some, dx=some,
+    ok = dict(x=some, ldx=8, w=some, ldw=8, bias=None, dtype=0, T=4, V=9, D=8, target=some, reduction=1, loss=some, state=some, unit=some, dloss=some, dx=some,
               dw=some, db=None, ws=some)
-    need = L.reco_linear_xent_workspace_bytes(some, 8, some, 8, 0, 4, 9, 8)
+    need = L.reco_linear_xent_workspace_bytes(some, 8, some, 8, 0, 4, 9, 8, 1)
     need_grad = L.reco_linear_xent_grad_workspace_bytes(some, 8, some, 8, 0, 4, 9, 8)
     assert need > 0 and need_grad > 0
 
     def forward(nbytes=need, **k):
         a = {**ok, **k}
         return L.reco_linear_xent(a["x"], a["ldx"], a["w"], a["ldw"], a["bias"], a["dtype"], a["T"], a["V"], a["D"], a["target"], -100, a["reduction"],
-                                  a["loss"], a["state"], None, a["ws"], nbytes, None)
+                                  a["loss"], a["state"], a["unit"], None, a["ws"], nbytes, None)
 
     def grad(nbytes=need_grad, **k):
         a = {**ok, **k}
         return L.reco_linear_xent_grad(a["x"], a["ldx"], a["w"], a["ldw"], a["bias"], a["dtype"], a["T"], a["V"], a["D"], a["target"], -100, a["reduction"],
-                                       a["state"], a["dloss"], a["dx"], a["dw"], a["db"], a["ws"], nbytes, None)
+                                       a["state"], a["unit"], a["dloss"], a["dx"], a["dw"], a["db"], a["ws"], nbytes, None)
     shared = [dict(x=None), dict(w=None), dict(target=None), dict(state=None), dict(ws=None), dict(ws=ctypes.c_void_p(8)), dict(T=0), dict(T=2 ** 31), dict(V=0),
               dict(V=2 ** 31), dict(D=0), dict(D=2 ** 20 + 1, ldx=2 ** 21, ldw=2 ** 21), dict(ldx=7), dict(ldw=7), dict(dtype=3), dict(dtype=-1),
               dict(reduction=3), dict(reduction=-1)]
     for k in shared + [dict(loss=None)]:
         assert forward(**k) == _lib.EINVAL, k
-    for k in shared + [dict(dloss=None)]:
+    for k in shared + [dict(dloss=None), dict(unit=None)]:
         assert grad(**k) == _lib.EINVAL, k
     assert forward(nbytes=need - 1) == _lib.ENOMEM and grad(nbytes=need_grad - 1) == _lib.ENOMEM
     assert grad(dx=None, dw=None, db=None) == _lib.OK         # nothing wanted, nothing launched
@@ -56,8 +56,8 @@ def test_workspace_does_not_hold_the_logits():
     some = ctypes.c_void_p(256)
     T, V, D = 8192, 100003, 128
     for dtype, size in ((0, 4), (1, 2), (2, 2)):
-        assert L.reco_linear_xent_workspace_bytes(some, D, some, D, dtype, T, V, D) < T * V * size // 10
+        assert L.reco_linear_xent_workspace_bytes(some, D, some, D, dtype, T, V, D, 1) < T * V * size // 8
         assert L.reco_linear_xent_grad_workspace_bytes(some, D, some, D, dtype, T, V, D) < T * V * size // 2
-    aligned = L.reco_linear_xent_workspace_bytes(some, D, some, D, 1, T, V, D)
-    assert L.reco_linear_xent_workspace_bytes(ctypes.c_void_p(258), D, some, D, 1, T, V, D) >= aligned + 2 * T * D       # a copy of x
-    assert L.reco_linear_xent_workspace_bytes(some, D, some, D + 1, 1, T, V, D) >= aligned + 2 * V * D                  # a copy of w
+    aligned = L.reco_linear_xent_workspace_bytes(some, D, some, D, 1, T, V, D, 0)
+    assert L.reco_linear_xent_workspace_bytes(ctypes.c_void_p(258), D, some, D, 1, T, V, D, 0) >= aligned + 2 * T * D       # a copy of x
+    assert L.reco_linear_xent_workspace_bytes(some, D, some, D + 1, 1, T, V, D, 0) >= aligned + 2 * V * D                  # a copy of w
