@@ -600,9 +600,9 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
     T* G = nullptr;
     float *x_part = nullptr, *w_part = nullptr, *b_part = nullptr;
     if (narrow) {
-        if (n.w_splits > 1) {
-            w_part = (float*)c.take((size_t)n.w_splits * a.V * a.D * 4);
-            b_part = (float*)c.take((size_t)n.w_splits * a.V * 4);
+        if (n.w_shared) {
+            w_part = (float*)c.take((size_t)n.w_shares * 2 * 128 * a.D * 4);
+            b_part = (float*)c.take((size_t)n.w_shares * 2 * 128 * 4);
         }
     } else {
         G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
@@ -626,10 +626,6 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
         if (dw || db) {
             const int rn = narrow_cols(a.dtype, p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
             if (rn) return rn;
-            if (n.w_splits > 1 && dw)
-                hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.V * a.D)), dim3(256), 0, s, w_part, (int)n.w_splits, a.V * a.D, scale, (T*)dw);
-            if (n.w_splits > 1 && db)
-                hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.V)), dim3(256), 0, s, b_part, (int)n.w_splits, a.V, scale, (T*)db);
         }
         if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, dx_unit, a.T, a.D, gn, scale, (T*)dx);
         RECO_CHECK_LAUNCH();

@@ -1,6 +1,6 @@
 // K-g, the form for narrow rows (up to 256 values in 16 bits, 128 in 32): the logits never leave the registers.
 //
-// Both kernels hold rows of one operand ("held": 32 NB per wave) as matrix fragments for the whole launch and stream the rows of the
+// Both kernels hold rows of one operand ("held": 32 per wave) as matrix fragments for the whole launch and stream the rows of the
 // other one through LDS, 32 at a time:
 //   acc[streamed, held] = C R^T       one 32 x 32 block: lane l holds column l % 32, i.e. one held row, and 16 of the 32 streamed ones
 //   e = exp(acc - ...)                in the registers the products left
@@ -26,11 +26,13 @@ template <typename T> constexpr float G_LOG2 = sizeof(T) == 2 && Traits<T>::G_SC
 template <typename T> constexpr float e_shift() { return 0.f; }
 template <> constexpr float e_shift<_Float16>() { return 10.f; }
 
-// A tile of SB streamed rows of DP values in LDS: 16-byte chunks, their order within a row changed by the row so that both ways of
-// reading (32 rows at one chunk; 4 rows at 32 bytes) touch every bank equally.  CH: chunks per row.
+// A tile of SB streamed rows of DP values in LDS.  The 64 banks take 256 bytes a cycle, i.e. 16 chunks of 16 bytes: the order of the
+// chunks of a row is changed by the row (exclusive or with twist), so that both ways of reading spread over all of them: 16 rows at
+// one chunk (logits), and 4 rows at 64 bytes each (the transposed reads).  CH: chunks per row.
 template <int CH> __device__ __forceinline__ int twist(int row)
 {
-    return CH == 4 ? (((row >> 1) & 1) << 1) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+    constexpr int C = CH < 16 ? CH : 16;                        // chunks of a row that share 256 bytes, with those of 16 / C - 1 others
+    return ((row >> 2) & 3) | ((row / (16 / C)) & (C / 4 - 1)) << 2;
 }
 
 template <typename T, int DP, int SB> struct Tile {
@@ -39,115 +41,168 @@ template <typename T, int DP, int SB> struct Tile {
     static_assert(SB * CH % 256 == 0 && (CH == 4 || CH % 8 == 0) && (CH & (CH - 1)) == 0, "tile shape");
     Pack<T, VEC> reg[PIECES];
 
-    // rows r0 .. of m [rows, ld], `width` values each; rows with drop[row] < 0 (nullable) are read as zeros
-    __device__ __forceinline__ void load(const T* m, int64_t ld, int64_t rows, int width, int64_t r0, const int* drop)
+    // rows r0 .. of m [rows, ld], `width` values each
+    __device__ __forceinline__ void load(const T* m, int64_t ld, int64_t rows, int width, int64_t r0)
     {
         const int c = threadIdx.x % CH, row = threadIdx.x / CH;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int64_t r = r0 + row + i * ROW_STEP;
-            bool ok = r < rows && c * VEC < width;
-            if (drop && ok) ok = drop[r] >= 0;
-            if (ok) {
-                reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(m + r * ld + c * VEC);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) reg[i].v[j] = (T)0.f;
-            }
+            if (r < rows && c * VEC < width) reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(m + r * ld + c * VEC);
+            else clear(i);
         }
     }
-    __device__ __forceinline__ void store(char* lds) const
+    __device__ __forceinline__ void clear(int i)
+    {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) reg[i].v[j] = (T)0.f;
+    }
+    // drops (in LDS, nullable): rows of the tile with a negative entry are stored as zeros
+    __device__ __forceinline__ void store(char* lds, const int* drops)
     {
         const int c = threadIdx.x % CH, row = threadIdx.x / CH;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int r = row + i * ROW_STEP;
+            if (drops && drops[r] < 0) clear(i);
             *reinterpret_cast<Pack<T, VEC>*>(lds + r * ROWB + ((c ^ twist<CH>(r)) << 4)) = reg[i];
         }
     }
 };
 
-// A wave's view of the streamed tile and its held rows
-template <typename T, int DP, int NB> struct Wave {
+// A wave's view of the streamed rows and its 32 held ones
+template <typename T, int DP> struct Wave {
     typedef typename Traits<T>::frag frag;
     static constexpr int STEPS = DP / Traits<T>::KSTEP, BLOCKS = DP / 32, ROWB = DP * (int)sizeof(T), CH = ROWB / 16;
     static constexpr bool WIDE = sizeof(T) == 4;
-    frag held[NB][STEPS];
-    f32x16 s[NB];
-    int by_row[4];         // byte of this lane's chunk of step j of a row: the steps repeat every 128 bytes
-    int by_col[4];         // byte of this lane's value(s) for the transposed reading
+    static constexpr int C = CH < 16 ? CH : 16, ROW_KINDS = C / 2, COL_KINDS = C / 4;
+    frag held[STEPS];
+    int by_row[ROW_KINDS];          // byte of this lane's chunk of step j of a row: the steps repeat every 256 bytes
+    int by_col[2][COL_KINDS];       // byte of this lane's value(s) for the transposed reading
 
     __device__ __forceinline__ void init(const T* m, int64_t ld, int64_t rows, int width, int64_t h0)
     {
         const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int i = 0; i < STEPS; ++i) {
+            const int64_t r = h0 + l31;
+            const int k = i * Traits<T>::KSTEP + half * Traits<T>::VEC;
+            if (r < rows && k < width) {
+                held[i] = *reinterpret_cast<const frag*>(m + r * ld + k);
+            } else {
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const int64_t r = h0 + 32 * b + l31;
-                const int k = i * Traits<T>::KSTEP + half * Traits<T>::VEC;
-                if (r < rows && k < width) {
-                    held[b][i] = *reinterpret_cast<const frag*>(m + r * ld + k);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < Traits<T>::VEC; ++j) held[b][i][j] = (T)0.f;
-                }
+                for (int j = 0; j < Traits<T>::VEC; ++j) held[i][j] = (T)0.f;
             }
+        }
         const int t = twist<CH>(l31);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) by_row[j] = l31 * ROWB + (((2 * j + half) ^ t) << 4);
-        if constexpr (WIDE) {
+        for (int j = 0; j < ROW_KINDS; ++j) by_row[j] = l31 * ROWB + (((2 * j + half) ^ t) << 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) by_col[j] = (4 * half + j) * ROWB + (((l31 >> 2) ^ ((j << 1) | half)) << 4) + (l31 & 3) * 4;
-        } else {
-            const int i16 = lane & 15, row = 4 * half + (i16 >> 2), tr = twist<CH>(row);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                by_col[j] = row * ROWB + ((((j & 1) * 4 + ((lane >> 4) & 1) * 2 + ((i16 >> 1) & 1)) ^ tr) << 4) + (i16 & 1) * 8;
-        }
+            for (int j = 0; j < COL_KINDS; ++j) {
+                if constexpr (WIDE) {       // row 8 (2 i + u) + 4 half + (0 .. 3): what twist adds above its low two bits is j
+                    by_col[u][j] = 4 * half * ROWB + (((l31 >> 2) ^ (2 * u + half) ^ ((j & 1) << 2)) << 4) + (l31 & 3) * 4;
+                } else {                    // rows 16 i + 8 u + 4 half + (0 .. 3), columns 32 j + ..
+                    const int i16 = lane & 15, row = 8 * u + 4 * half + (i16 >> 2);
+                    by_col[u][j] = row * ROWB + (((4 * j + ((lane >> 4) & 1) * 2 + ((i16 >> 1) & 1)) ^ twist<CH>(row)) << 4) + (i16 & 1) * 8;
+                }
+            }
+    }
+
+    __device__ __forceinline__ frag streamed(const char* lds, int i) const
+    {
+        return *reinterpret_cast<const frag*>(lds + by_row[i % ROW_KINDS] + i / ROW_KINDS * (C * 16));
+    }
+    // columns 32 d .. of streamed rows 16 j .., transposed
+    __device__ __forceinline__ frag turned(const char* lds, int j, int d) const
+    {
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const char* src = lds + d / COL_KINDS * (C * 16) + 16 * j * ROWB;
+        union { s16x4 h[2]; frag f; } a;
+        a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(src + by_col[0][d % COL_KINDS]));
+        a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(src + by_col[1][d % COL_KINDS]));
+        return a.f;
     }
 
     // s += the 32 streamed rows at `lds` times the held ones
-    __device__ __forceinline__ void logits(const char* lds)
+    __device__ __forceinline__ void logits(const char* lds, f32x16& s) const
     {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const frag a = *reinterpret_cast<const frag*>(lds + by_row[i & 3] + (i >> 2) * 128);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mma(s[b], a, held[b][i]);
-        }
+        for (int i = 0; i < STEPS; ++i) mma(s, streamed(lds, i), held[i]);
     }
 
-    // o += (the 32 streamed rows)^T times s, which holds weights now
-    __device__ __forceinline__ void weigh(const char* lds, f32x16 (&o)[NB][BLOCKS]) const
+    // The first streamed fragments of a block's logits are read while the block before it is worked on
+    static constexpr int AHEAD = STEPS < 3 ? STEPS : 3;
+    frag a[AHEAD];
+    __device__ __forceinline__ void read_ahead(const char* lds)
+    {
+        if constexpr (!WIDE)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) a[i] = streamed(lds, i);
+    }
+
+    // next += the logits of the block at `ahead` (its first fragments are in a), while weight(r) turns s[r] of this block (at `lds`) into
+    // its weight; then, after between(), o += (this block)^T times the weights, with beside(k, n) called as part k of n.  Leaves the
+    // first fragments of the block at `then` in a.
+    // A wave issues in order and a product waits for the one before it: the vector work stands between the products, in this order.
+    // READ_THEN: that block is in LDS already (tiles of more than one block); else the caller reads the fragments when it is.
+    template <bool SUMS, bool READ_THEN, typename Weight, typename Between, typename Beside>
+    __device__ __forceinline__ void block(const char* ahead, const char* then, const char* lds, f32x16& next, f32x16& s, f32x16 (&o)[SUMS ? BLOCKS : 1],
+                                          Weight&& weight, Between&& between, Beside&& beside)
     {
         if constexpr (WIDE) {
+            logits(ahead, next);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
+            for (int r = 0; r < 16; ++r) weight(r);
+            between();
+            beside(0, 1);
+            if constexpr (SUMS)
 #pragma unroll
-                for (int d = 0; d < BLOCKS; ++d) {
-                    const float a = *reinterpret_cast<const float*>(lds + by_col[r & 3] + 8 * (r >> 2) * ROWB + d * 128);
+                for (int r = 0; r < 16; ++r)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[b][r], o[b][d], 0, 0, 0);
-                }
+                    for (int d = 0; d < BLOCKS; ++d) {
+                        // the row's number in its 256 bytes is known here: twist's upper bits pick one of the two kinds, and the 128 bytes
+                        const int up = (r & 3) / (16 / C) & (C / 4 - 1);
+                        const float a =
+                            *reinterpret_cast<const float*>(lds + by_col[(r >> 2) & 1][up & 1] + (8 * (r >> 2) + (r & 3)) * ROWB + ((d ^ (up >> 1)) * 128));
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[r], o[d], 0, 0, 0);
+                    }
         } else {
-            frag p[NB][2];
+            constexpr int EACH_STEP = (16 + STEPS - 1) / STEPS, PARTS = 2 * BLOCKS, TURN = PARTS < 2 ? PARTS : 2;
+            frag c[TURN];
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int i = 0; i < STEPS; ++i) {
+                mma(next, a[i % AHEAD], held[i]);
+                if (i + AHEAD < STEPS) a[i % AHEAD] = streamed(ahead, i + AHEAD);
+                if constexpr (SUMS)
+                    if (i == (STEPS > 2 ? STEPS - 2 : 0))
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[b][i >> 3][i & 7] = (T)s[b][i];
-            typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+                        for (int k = 0; k < TURN; ++k) c[k] = turned(lds, k / BLOCKS, k % BLOCKS);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int r = i * EACH_STEP; r < (i + 1) * EACH_STEP && r < 16; ++r) weight(r);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            between();
+            if constexpr (SUMS) {
+                frag p[2];
 #pragma unroll
-                for (int d = 0; d < BLOCKS; ++d) {
-                    const char* src = lds + by_col[d & 1] + (d >> 1) * 128 + 16 * j * ROWB;
-                    union { s16x4 h[2]; frag f; } a;
-                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)src);
-                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(src + 8 * ROWB));
+                for (int i = 0; i < 8; ++i) p[0][i] = (T)s[i];
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) mma(o[b][d], a.f, p[b][j]);
+                for (int k = 0; k < PARTS; ++k) {
+                    mma(o[k % BLOCKS], c[k % TURN], p[k / BLOCKS]);
+                    if (k + TURN < PARTS) c[k % TURN] = turned(lds, (k + TURN) / BLOCKS, (k + TURN) % BLOCKS);
+                    if (k == 0)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) p[1][i] = (T)s[8 + i];
+                    if (READ_THEN && k == PARTS - 2) read_ahead(then);
+                    beside(k, PARTS);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+            } else {
+                if (READ_THEN) read_ahead(then);
+                beside(0, 1);
+            }
         }
     }
 };
@@ -156,271 +211,163 @@ template <typename T, int DP> constexpr int stream_rows() { return DP * (int)siz
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }        // below 2^-126: 0
 
+// Waves per SIMD that the registers are cut for
+template <typename T, int DP> constexpr int waves_per_simd() { return DP * (int)sizeof(T) >= 512 ? 1 : 2; }
+
 // ---------------------------------------------------------------------------------------------
 // rows: loss statistics, and with DX the softmax-weighted sums of W
 // ---------------------------------------------------------------------------------------------
-template <typename T, int DP, int NB, bool BIAS, bool DX>
-__global__ __launch_bounds__(256) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out, Running* __restrict__ part,
-                                                          float* __restrict__ z_target, float* __restrict__ dx_part)
+template <typename T, int DP, bool BIAS, bool DX>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out,
+                                                                                   Running* __restrict__ part, float* __restrict__ z_target,
+                                                                                   float* __restrict__ dx_part)
 {
-    constexpr int SB = stream_rows<T, DP>();
+    constexpr int SB = stream_rows<T, DP>(), NS = SB / 32;
     typedef Tile<T, DP, SB> Streamed;
-    typedef Wave<T, DP, NB> W;
-    __shared__ __attribute__((aligned(16))) char tiles[2][Streamed::BYTES];
-    __shared__ __attribute__((aligned(16))) float biases[2][SB];
+    typedef Wave<T, DP> W;
+    __shared__ __attribute__((aligned(16))) char tiles[3][Streamed::BYTES];
+    __shared__ __attribute__((aligned(16))) float biases[3][SB];
     const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t split = blockIdx.x % splits, h0 = (blockIdx.x / splits * 4 + wave) * (32 * NB);
+    const int64_t split = blockIdx.x % splits, h0 = (blockIdx.x / splits * 4 + wave) * 32, t = h0 + l31;
     const bool active = h0 < p.T;
     const T* w = (const T*)p.w;
     const T* bias = (const T*)p.bias;
     const int64_t first = split * rows_per_split, end = first + rows_per_split < p.V ? first + rows_per_split : p.V;
+    const int n_tiles = (int)((end - first + SB - 1) / SB);
 
     W me;
     me.init((const T*)p.x, p.ldx, p.T, (int)p.D, h0);
-    int y[NB];
-    float m[NB], sum[NB];
-    f32x16 o[NB][DX ? W::BLOCKS : 1];
+    int y = -1;
+    if (t < p.T && p.target[t] != p.ignore) y = (int)clamp_target(p.target[t], p.V);
+    float m = -INFINITY, sum = 0.f;
+    f32x16 o[DX ? W::BLOCKS : 1];
+    if constexpr (DX)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int64_t t = h0 + 32 * b + l31;
-        y[b] = -1;
-        if (t < p.T && p.target[t] != p.ignore) y[b] = (int)clamp_target(p.target[t], p.V);
-        m[b] = -INFINITY;
-        sum[b] = 0.f;
-        if constexpr (DX)
-#pragma unroll
-            for (int d = 0; d < W::BLOCKS; ++d) o[b][d] = f32x16{};
-    }
+        for (int d = 0; d < W::BLOCKS; ++d) o[d] = f32x16{};
 
     Streamed st;
     float bias_reg = 0.f;
-    auto fetch = [&](int64_t v0) {
-        st.load(w, p.ldw, end, (int)p.D, v0, nullptr);
+    auto fetch = [&](int tile) {
+        const int64_t v0 = first + (int64_t)tile * SB;
+        st.load(w, p.ldw, end, (int)p.D, v0);
         if (threadIdx.x < SB) {
             const int64_t v = v0 + threadIdx.x;
             bias_reg = v >= end ? -INFINITY : BIAS ? (float)bias[v] : 0.f;        // rows behind the split have no weight
         }
     };
     auto put = [&](int at) {
-        st.store(tiles[at]);
+        st.store(tiles[at], nullptr);
         if (threadIdx.x < SB) biases[at][threadIdx.x] = bias_reg;
     };
-    fetch(first);
-    put(0);
-    __syncthreads();
-    int at = 0;
-    for (int64_t v0 = first; v0 < end; v0 += SB, at ^= 1) {
-        const bool more = v0 + SB < end;
-        if (more) fetch(v0 + SB);
-        if (active) {
-            const bool tail = v0 + SB > end;
-#pragma unroll 1
-            for (int sub = 0; sub < SB / 32; ++sub) {
-                const char* rows = tiles[at] + sub * 32 * W::ROWB;
-                if (BIAS || tail) {
+    auto init = [&](const float* biases32, f32x16& z) {
+        if (BIAS) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const f32x4 c = *reinterpret_cast<const f32x4*>(&biases[at][sub * 32 + 8 * q + 4 * half]);
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 c = *reinterpret_cast<const f32x4*>(biases32 + 8 * q + 4 * half);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) me.s[b][4 * q + i] = c[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) me.s[b] = f32x16{};
-                }
-                me.logits(rows);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int here = y[b] - (int)(v0 + 32 * sub);               // the target's place in this block, if it is in it
-                    if (__any((unsigned)here < 32u)) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (here == acc_row(r, half)) {
-                                z_target[h0 + 32 * b + l31] = me.s[b][r];
-                                me.s[b][r] = -INFINITY;
-                            }
-                    }
-                    float top = me.s[b][0];
-#pragma unroll
-                    for (int r = 1; r < 16; ++r) top = fmaxf(top, me.s[b][r]);
-                    if (__any(top > m[b] + lag<T>())) {
-                        top = fmaxf(top, __shfl_xor(top, 32, 64));              // both halves of a column keep one reference
-                        if (top > m[b] + lag<T>()) {
-                            const float f = m[b] == -INFINITY ? 0.f : exp2_fast((m[b] - top) * LOG2E);
-                            m[b] = top;
-                            sum[b] *= f;
-                            if constexpr (DX)
-#pragma unroll
-                                for (int d = 0; d < W::BLOCKS; ++d) o[b][d] *= f;
-                        }
-                    }
-                    // nothing above -inf yet: any finite reference leaves the sum at 0
-                    const float base = m[b] == -INFINITY ? 0.f : m[b];
-                    if (BIAS) {                                                 // logits up to the type's lowest: their difference first
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) me.s[b][r] = exp2_fast(fmaf(me.s[b][r] - base, LOG2E, e_shift<T>()));
-                    } else {
-                        const float shift = e_shift<T>() - base * LOG2E;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) me.s[b][r] = exp2_fast(fmaf(me.s[b][r], LOG2E, shift));
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[b] += me.s[b][r];
-                }
-                if constexpr (DX) me.weigh(rows, o);
+                for (int i = 0; i < 4; ++i) z[4 * q + i] = c[i];
             }
-        }
-        if (more) put(at ^ 1);
-        __syncthreads();
-    }
-    if (!active) return;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int64_t t = h0 + 32 * b + l31;
-        const float total = sum[b] + __shfl_xor(sum[b], 32, 64);
-        if (t >= p.T) continue;
-        if (half == 0) part[split * p.T + t] = Running{m[b], total * exp2f(-e_shift<T>())};
-        if constexpr (DX) {
-            float* dst = dx_part + (split * p.T + t) * width_out;
-#pragma unroll
-            for (int d = 0; d < W::BLOCKS; ++d)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 32 * d + 8 * q + 4 * half + i;
-                        if (c < width_out) dst[c] = o[b][d][4 * q + i] * exp2f(-e_shift<T>());
-                    }
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------
-// cols: dW and dbias
-// ---------------------------------------------------------------------------------------------
-// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count; with a bias, whose logits may be the type's lowest, lse_t
-// itself and +inf.  y[t]: the target, -1 for rows that do not count.  EACH: rows have weights gn[t]
-template <typename T, int DP, int NB, bool BIAS, bool EACH>
-__global__ __launch_bounds__(256) void narrow_cols_kernel(Problem p, int splits, int64_t rows_per_split, int width_out, const float* __restrict__ expo,
-                                                          const int* __restrict__ y, const float* __restrict__ rest, const float* __restrict__ gn,
-                                                          const float* __restrict__ scale, T* __restrict__ dw, T* __restrict__ db,
-                                                          float* __restrict__ dw_part, float* __restrict__ db_part)
-{
-    constexpr int SB = stream_rows<T, DP>();
-    typedef Tile<T, DP, SB> Streamed;
-    typedef Wave<T, DP, NB> W;
-    __shared__ __attribute__((aligned(16))) char tiles[2][Streamed::BYTES];
-    __shared__ __attribute__((aligned(16))) float expos[2][SB];
-    __shared__ __attribute__((aligned(16))) float gns[2][SB];
-    __shared__ __attribute__((aligned(16))) int ys[2][SB];
-    const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t split = blockIdx.x % splits, h0 = (blockIdx.x / splits * 4 + wave) * (32 * NB);
-    const bool active = h0 < p.V;
-    const int64_t first = split * rows_per_split, end = first + rows_per_split < p.T ? first + rows_per_split : p.T;
-
-    W me;
-    me.init((const T*)p.w, p.ldw, p.V, (int)p.D, h0);
-    float bias[NB], sum[NB];
-    f32x16 o[NB][W::BLOCKS];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int64_t v = h0 + 32 * b + l31;
-        bias[b] = BIAS && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
-        sum[b] = 0.f;
-#pragma unroll
-        for (int d = 0; d < W::BLOCKS; ++d) o[b][d] = f32x16{};
-    }
-
-    Streamed st;
-    float expo_reg = 0.f, gn_reg = 0.f;
-    int y_reg = -1;
-    auto fetch = [&](int64_t t0) {
-        st.load((const T*)p.x, p.ldx, end, (int)p.D, t0, y);
-        if (threadIdx.x < SB) {
-            const int64_t t = t0 + threadIdx.x;
-            expo_reg = t < end ? expo[t] : BIAS ? INFINITY : -INFINITY;
-            y_reg = t < end ? y[t] : -1;
-            if (EACH) gn_reg = t < end ? gn[t] : 0.f;
+        } else {
+            z = f32x16{};
         }
     };
-    auto put = [&](int at) {
-        st.store(tiles[at]);
-        if (threadIdx.x < SB) {
-            expos[at][threadIdx.x] = expo_reg;
-            ys[at][threadIdx.x] = y_reg;
-            if (EACH) gns[at][threadIdx.x] = gn_reg;
+    // a finished block's rows v0 ..: those behind the split and the target's logit out, and the reference value of the exponentials;
+    // top: this lane's largest
+    auto settle = [&](int64_t v0, f32x16& z, float top) {
+        const int here = y - (int)v0;                                           // the target's place in this block, if it is in it
+        const bool tail = !BIAS && v0 + 32 > end, mine = __any((unsigned)here < 32u);
+        if (tail || mine) {
+            const int left = (int)(end - v0);
+            top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = acc_row(r, half);
+                if (row == here && row < left) z_target[t] = z[r];
+                if (row == here || row >= left) z[r] = -INFINITY;
+                top = fmaxf(top, z[r]);
+            }
+        }
+        if (__any(top > m + lag<T>())) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));                          // both halves of a column keep one reference
+            if (top > m + lag<T>()) {
+                const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * LOG2E);
+                m = top;
+                sum *= f;
+                if constexpr (DX)
+#pragma unroll
+                    for (int d = 0; d < W::BLOCKS; ++d) o[d] *= f;
+            }
         }
     };
-    fetch(first);
+    auto largest = [](const f32x16& z) {
+        float top = z[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, z[r]);
+        return top;
+    };
+
+    // Three tiles in LDS: tile i is weighed and the logits of tile i + 1's first block are taken while tile i + 2 arrives; one barrier
+    // per tile
+    fetch(0);
     put(0);
+    if (n_tiles > 1) {
+        fetch(1);
+        put(1);
+    }
     __syncthreads();
+    constexpr int BLOCK_BYTES = 32 * W::ROWB, RING = 3 * NS;
+    char* const ring = &tiles[0][0];
+    const int n_blocks = (int)((end - first + 31) / 32);
+    f32x16 s0, s1;
+    if (active) {
+        init(&biases[0][0], s0);
+        me.logits(ring, s0);
+        settle(first, s0, largest(s0));
+        if (NS > 1) me.read_ahead(ring + BLOCK_BYTES);
+    }
     int at = 0;
-    for (int64_t t0 = first; t0 < end; t0 += SB, at ^= 1) {
-        const bool more = t0 + SB < end;
-        if (more) fetch(t0 + SB);
+    // block i: s holds its logits, next gets those of block i + 1
+    auto work = [&](int i, f32x16& s, f32x16& next) {
+        const int after = at + 1 == RING ? 0 : at + 1, then = after + 1 == RING ? 0 : after + 1;
+        const int tile = i / NS;
+        if (i % NS == 0 && tile + 2 < n_tiles) fetch(tile + 2);
         if (active) {
-#pragma unroll 1
-            for (int sub = 0; sub < SB / 32; ++sub) {
-                const char* rows = tiles[at] + sub * 32 * W::ROWB;
+            // nothing above -inf yet: any finite reference leaves the sum at 0
+            const float base = m == -INFINITY ? 0.f : m, shift = e_shift<T>() - base * LOG2E;
+            float top = -INFINITY;
+            init(&biases[0][0] + after * 32, next);
+            if (NS == 1) me.read_ahead(ring + after * BLOCK_BYTES);
+            me.template block<DX, (NS > 1)>(
+                ring + after * BLOCK_BYTES, ring + then * BLOCK_BYTES, ring + at * BLOCK_BYTES, next, s, o,
+                [&](int r) {
+                    // with a bias the logits may be the type's lowest: their difference first
+                    s[r] = BIAS ? exp2_fast(fmaf(s[r] - base, LOG2E, e_shift<T>())) : exp2_fast(fmaf(s[r], LOG2E, shift));
+                },
+                [] {},
+                [&](int k, int n) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) me.s[b] = f32x16{};
-                me.logits(rows);
-                // targets of these 32 rows that lie in this wave's part of the vocabulary
-                const int64_t away = (int64_t)ys[at][sub * 32 + l31] - h0;
-                const bool hit = __any(away >= 0 && away < 32 * NB);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 x4 = *reinterpret_cast<const f32x4*>(&expos[at][sub * 32 + 8 * q + 4 * half]);
-                    f32x4 g4;
-                    if (EACH) g4 = *reinterpret_cast<const f32x4*>(&gns[at][sub * 32 + 8 * q + 4 * half]);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float z = me.s[b][4 * q + i];
-                            float e = BIAS ? exp2_fast(fmaf(z + bias[b] - x4[i], LOG2E, G_LOG2<T>)) : exp2_fast(fmaf(z, LOG2E, x4[i]));
-                            if (EACH) e *= g4[i];
-                            me.s[b][4 * q + i] = e;
-                        }
-                }
-                if (hit) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int row = sub * 32 + acc_row(r, half);
-                            if ((int64_t)ys[at][row] == h0 + 32 * b + l31) {
-                                const float q = rest[t0 + row] * Traits<T>::G_SCALE;
-                                me.s[b][r] = EACH ? -q * gns[at][row] : -q;
-                            }
-                        }
-                }
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[b] += me.s[b][r];
-                me.weigh(rows, o);
-            }
+                    for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) sum += s[r];
+                    if (k == n / 2) top = largest(next);
+                });
+            if (i + 1 < n_blocks) settle(first + 32 * (int64_t)(i + 1), next, top);
         }
-        if (more) put(at ^ 1);
-        __syncthreads();
+        if (i % NS == NS - 1) {
+            if (tile + 2 < n_tiles) put((tile + 2) % 3);
+            __syncthreads();
+        }
+        at = after;
+    };
+#pragma unroll 1
+    for (int i = 0; i < n_blocks; i += 2) {
+        work(i, s0, s1);
+        if (i + 1 < n_blocks) work(i + 1, s1, s0);
     }
     if (!active) return;
-    const float f = splits == 1 ? *scale / Traits<T>::G_SCALE : 1.f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int64_t v = h0 + 32 * b + l31;
-        const float total = (sum[b] + __shfl_xor(sum[b], 32, 64)) * f;
-        if (v >= p.V) continue;
-        if (half == 0) {
-            if (splits == 1) {
-                if (db) db[v] = (T)total;
-            } else {
-                db_part[split * p.V + v] = total;
-            }
-        }
+    const float total = sum + __shfl_xor(sum, 32, 64);
+    if (t >= p.T) return;
+    if (half == 0) part[split * p.T + t] = Running{m, total * exp2f(-e_shift<T>())};
+    if constexpr (DX) {
+        float* dst = dx_part + (split * p.T + t) * width_out;
 #pragma unroll
         for (int d = 0; d < W::BLOCKS; ++d)
 #pragma unroll
@@ -428,26 +375,207 @@ __global__ __launch_bounds__(256) void narrow_cols_kernel(Problem p, int splits,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int c = 32 * d + 8 * q + 4 * half + i;
-                    if (c < width_out) {
-                        if (splits == 1) {
-                            if (dw) dw[v * width_out + c] = (T)(o[b][d][4 * q + i] * f);
-                        } else {
-                            dw_part[(split * p.V + v) * width_out + c] = o[b][d][4 * q + i];
-                        }
-                    }
+                    if (c < width_out) dst[c] = o[d][4 * q + i] * exp2f(-e_shift<T>());
                 }
     }
 }
 
-// held rows per wave, in blocks of 32
-template <typename T, int DP> constexpr int held_blocks() { return sizeof(T) == 2 && DP <= 128 ? 2 : 1; }
+// ---------------------------------------------------------------------------------------------
+// cols: dW and dbias
+// ---------------------------------------------------------------------------------------------
+// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count; with a bias, whose logits may be the type's lowest, lse_t
+// itself and +inf.  y[t]: the target, -1 for rows that do not count.  EACH: rows have weights gn[t].
+// The work is groups of 128 held rows times tiles of streamed ones, in that order; every workgroup takes an equal share of consecutive
+// (group, tile) units, so that the groups need not be a multiple of what the chip holds at once (782 groups over 512 places: 0.72 ms
+// with a group to a workgroup).  A group inside one share is finished there; else its parts are written in 32 bits (place 1 of a
+// workgroup: a part that begins its group, place 0: one that does not) and added by narrow_join_kernel in order.
+template <typename T, int DP, bool BIAS, bool EACH>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_kernel(Problem p, int64_t units, int64_t share, int tiles_in_all, int width_out,
+                                                                                   const float* __restrict__ expo, const int* __restrict__ y,
+                                                                                   const float* __restrict__ rest, const float* __restrict__ gn,
+                                                                                   const float* __restrict__ scale, T* __restrict__ dw, T* __restrict__ db,
+                                                                                   float* __restrict__ dw_part, float* __restrict__ db_part)
+{
+    constexpr int SB = stream_rows<T, DP>(), NS = SB / 32;
+    typedef Tile<T, DP, SB> Streamed;
+    typedef Wave<T, DP> W;
+    __shared__ __attribute__((aligned(16))) char tiles[3][Streamed::BYTES];
+    __shared__ __attribute__((aligned(16))) float expos[3][SB];
+    __shared__ __attribute__((aligned(16))) float gns[EACH ? 3 : 1][SB];
+    __shared__ __attribute__((aligned(16))) int ys[4][SB];
+    const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
+    char* const ring = &tiles[0][0];
+    constexpr int BLOCK_BYTES = 32 * W::ROWB, RING = 3 * NS;
+    const int64_t u1 = (blockIdx.x + 1) * share < units ? (blockIdx.x + 1) * share : units;
+#pragma unroll 1
+    for (int64_t u = blockIdx.x * share; u < u1;) {
+    const int64_t group = u / tiles_in_all;
+    const int tile0 = (int)(u - group * tiles_in_all), n_tiles = u1 - u < tiles_in_all - tile0 ? (int)(u1 - u) : tiles_in_all - tile0;
+    const int64_t h0 = (group * 4 + wave) * 32, v = h0 + l31;
+    const bool active = h0 < p.V;
+    const int64_t first = (int64_t)tile0 * SB, end = first + (int64_t)n_tiles * SB < p.T ? first + (int64_t)n_tiles * SB : p.T;
+    const bool whole = n_tiles == tiles_in_all;
+    u += n_tiles;
 
-template <typename F> int with_width(int64_t D, int size, F&& fn)
+    W me;
+    me.init((const T*)p.w, p.ldw, p.V, (int)p.D, h0);
+    const float bias = BIAS && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
+    float sum = 0.f;
+    f32x16 o[W::BLOCKS];
+#pragma unroll
+    for (int d = 0; d < W::BLOCKS; ++d) o[d] = f32x16{};
+
+    Streamed st;
+    float expo_reg = 0.f, gn_reg = 0.f;
+    int y_reg = -1;
+    auto fetch = [&](int tile) {
+        const int64_t t0 = first + (int64_t)tile * SB;
+        st.load((const T*)p.x, p.ldx, end, (int)p.D, t0);
+        if (threadIdx.x < SB) {
+            const int64_t t = t0 + threadIdx.x;
+            expo_reg = t < end ? expo[t] : BIAS ? INFINITY : -INFINITY;
+            y_reg = t + SB < end ? y[t + SB] : -1;
+            if (EACH) gn_reg = t < end ? gn[t] : 0.f;
+        }
+    };
+    // the targets run one tile ahead of the rows: storing a tile looks at those of its rows that do not count
+    auto put = [&](int tile) {
+        const int at = tile % 3;
+        st.store(tiles[at], ys[tile & 3]);
+        if (threadIdx.x < SB) {
+            expos[at][threadIdx.x] = expo_reg;
+            ys[(tile + 1) & 3][threadIdx.x] = y_reg;
+            if (EACH) gns[at][threadIdx.x] = gn_reg;
+        }
+    };
+    if (threadIdx.x < 2 * SB) ys[threadIdx.x / SB][threadIdx.x % SB] = first + threadIdx.x < end ? y[first + threadIdx.x] : -1;
+    __syncthreads();
+    fetch(0);
+    put(0);
+    if (n_tiles > 1) {
+        fetch(1);
+        put(1);
+    }
+    __syncthreads();
+    const int n_blocks = (int)((end - first + 31) / 32);
+    f32x16 s0 = {}, s1;
+    f32x4 x4, g4, x_next = {}, g_next = {};
+    if (active) {
+        x_next = *reinterpret_cast<const f32x4*>(&expos[0][4 * half]);
+        if (EACH) g_next = *reinterpret_cast<const f32x4*>(&gns[0][4 * half]);
+        me.logits(ring, s0);
+        if (NS > 1) me.read_ahead(ring + BLOCK_BYTES);
+    }
+    int at = 0;
+    auto work = [&](int i, f32x16& s, f32x16& next) {
+        const int after = at + 1 == RING ? 0 : at + 1, then = after + 1 == RING ? 0 : after + 1;
+        const int tile = i / NS;
+        if (i % NS == 0 && tile + 2 < n_tiles) fetch(tile + 2);
+        if (active) {
+            const float *expo32 = &expos[0][0] + 4 * half, *gn32 = &gns[0][0] + 4 * half;
+            const int* y32 = &ys[tile & 3][i % NS * 32];
+            const int mine = y32[l31];
+            next = f32x16{};
+            if (NS == 1) me.read_ahead(ring + after * BLOCK_BYTES);
+            me.template block<true, (NS > 1)>(
+                ring + after * BLOCK_BYTES, ring + then * BLOCK_BYTES, ring + at * BLOCK_BYTES, next, s, o,
+                [&](int r) {
+                    if (r % 4 == 0) {                               // the rows' constants are read four ahead
+                        const int ahead = r < 12 ? at * 32 + 8 * (r / 4 + 1) : after * 32;
+                        x4 = x_next;
+                        x_next = *reinterpret_cast<const f32x4*>(expo32 + ahead);
+                        if (EACH) {
+                            g4 = g_next;
+                            g_next = *reinterpret_cast<const f32x4*>(gn32 + ahead);
+                        }
+                    }
+                    const float e = BIAS ? exp2_fast(fmaf(s[r] + bias - x4[r % 4], LOG2E, G_LOG2<T>)) : exp2_fast(fmaf(s[r], LOG2E, x4[r % 4]));
+                    s[r] = EACH ? e * g4[r % 4] : e;
+                },
+                [&] {
+                    // a target of these 32 rows that lies in this wave's part of the vocabulary
+                    if (__any((unsigned)(mine - (int)h0) < 32u))
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int row = acc_row(r, half);
+                            if (y32[row] == (int)v) {
+                                const float q = rest[first + 32 * (int64_t)i + row] * Traits<T>::G_SCALE;
+                                s[r] = EACH ? -q * gns[0][at * 32 + row] : -q;
+                            }
+                        }
+                },
+                [&](int k, int n) {
+#pragma unroll
+                    for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) sum += s[r];
+                });
+        }
+        if (i % NS == NS - 1) {
+            if (tile + 2 < n_tiles) put(tile + 2);
+            __syncthreads();
+        }
+        at = after;
+    };
+#pragma unroll 1
+    for (int i = 0; i < n_blocks; i += 2) {
+        work(i, s0, s1);
+        if (i + 1 < n_blocks) work(i + 1, s1, s0);
+    }
+    __syncthreads();                                            // the next group's tiles overwrite these
+    if (!active) continue;
+    const float f = whole ? *scale / Traits<T>::G_SCALE : 1.f;
+    const float total = (sum + __shfl_xor(sum, 32, 64)) * f;
+    if (v >= p.V) continue;
+    const int64_t row = ((int64_t)blockIdx.x * 2 + (tile0 ? 0 : 1)) * 128 + wave * 32 + l31;
+    if (half == 0) {
+        if (!whole) db_part[row] = total;
+        else if (db) db[v] = (T)total;
+    }
+#pragma unroll
+    for (int d = 0; d < W::BLOCKS; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = 32 * d + 8 * q + 4 * half + i;
+                if (c < width_out) {
+                    if (!whole) dw_part[row * width_out + c] = o[d][4 * q + i];
+                    else if (dw) dw[v * width_out + c] = (T)(o[d][4 * q + i] * f);
+                }
+            }
+    }
+}
+
+// The groups that several workgroups shared: blockIdx.x is the group, the threads take its 128 x (width, then 1) sums
+template <typename T>
+__global__ __launch_bounds__(256) void narrow_join_kernel(int64_t V, int64_t share, int tiles_in_all, int width, const float* __restrict__ scale,
+                                                          const float* __restrict__ dw_part, const float* __restrict__ db_part, T* __restrict__ dw, T* __restrict__ db)
+{
+    const int64_t group = blockIdx.x, a = group * tiles_in_all / share, b = ((group + 1) * tiles_in_all - 1) / share;
+    if (a == b) return;
+    const float f = *scale / Traits<T>::G_SCALE;
+    const int n = 128 * width;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < n + 128; i += gridDim.y * 256) {
+        const bool bias = i >= n;
+        const int64_t v = group * 128 + (bias ? i - n : i / width);
+        if (v >= V || !(bias ? db : dw)) continue;
+        float s = 0.f;
+#pragma unroll 4
+        for (int64_t g = a; g <= b; ++g) {
+            const int64_t place = g * 2 + (g == a ? 1 : 0);
+            s += bias ? db_part[place * 128 + (i - n)] : dw_part[place * n + i];
+        }
+        if (bias) db[v] = (T)(s * f);
+        else dw[group * n + i] = (T)(s * f);
+    }
+}
+
+template <typename T, typename F> int with_width(int64_t D, F&& fn)
 {
     if (D <= 32) return fn(std::integral_constant<int, 32>());
     if (D <= 64) return fn(std::integral_constant<int, 64>());
-    if (D <= 128 || size == 4) return fn(std::integral_constant<int, 128>());
-    return fn(std::integral_constant<int, 256>());
+    if constexpr (sizeof(T) == 2)
+        if (D > 128) return fn(std::integral_constant<int, 256>());
+    return fn(std::integral_constant<int, 128>());
 }
 
 template <typename F> int with_flag(bool v, F&& fn) { return v ? fn(std::true_type()) : fn(std::false_type()); }
@@ -455,6 +583,8 @@ template <typename F> int with_flag(bool v, F&& fn) { return v ? fn(std::true_ty
 }  // namespace
 
 namespace xent {
+
+static constexpr int64_t HELD = 128;           // held rows per workgroup: 4 waves of 32
 
 bool narrow_fits(int dtype, int64_t D) { return D <= (dtype == RECO_DT_F32 ? 128 : 256); }
 
@@ -470,9 +600,9 @@ static void split_plan(int64_t held_groups, int64_t streamed, int64_t tile, int6
 
 template <typename T, typename F> static int shape_of(int64_t D, F&& fn)
 {
-    return with_width(D, sizeof(T), [&](auto dp) -> int {
+    return with_width<T>(D, [&](auto dp) -> int {
         constexpr int DP = decltype(dp)::value;
-        return fn(dp, std::integral_constant<int, held_blocks<T, DP>()>(), (int64_t)stream_rows<T, DP>());
+        return fn(dp, (int64_t)stream_rows<T, DP>());
     });
 }
 
@@ -480,12 +610,17 @@ NarrowPlan narrow_plan(int dtype, int64_t T, int64_t V, int64_t D)
 {
     NarrowPlan n{};
     (void)reco_with_type(dtype, [&](auto z) -> int {
-        return shape_of<decltype(z)>(D, [&](auto, auto nb, int64_t tile) -> int {
-            const int64_t per = 128 * decltype(nb)::value;
-            n.x_groups = ceil_div64(T, per);
-            n.w_groups = ceil_div64(V, per);
+        return shape_of<decltype(z)>(D, [&](auto dp, int64_t tile) -> int {
+            n.x_groups = ceil_div64(T, HELD);
             split_plan(n.x_groups, V, tile, &n.x_splits, &n.x_per);
-            split_plan(n.w_groups, T, tile, &n.w_splits, &n.w_per);
+            n.w_groups = ceil_div64(V, HELD);
+            n.w_tiles = ceil_div64(T, tile);
+            const int64_t units = n.w_groups * n.w_tiles, places = 256 * waves_per_simd<decltype(z), decltype(dp)::value>();
+            // a share of less than four tiles is mostly beginning and end
+            n.w_share = ceil_div64(units, places);
+            if (n.w_share < 4) n.w_share = n.w_tiles < 4 ? n.w_tiles : 4;
+            n.w_shares = ceil_div64(units, n.w_share);
+            n.w_shared = n.w_share % n.w_tiles != 0;
             return RECO_OK;
         });
     });
@@ -496,10 +631,10 @@ int narrow_rows(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_
 {
     return reco_with_type(dtype, [&](auto z) -> int {
         typedef decltype(z) T;
-        return shape_of<T>(p.D, [&](auto dp, auto nb, int64_t) -> int {
+        return shape_of<T>(p.D, [&](auto dp, int64_t) -> int {
             return with_flag(p.bias != nullptr, [&](auto bias) -> int {
                 return with_flag(dx_part != nullptr, [&](auto dx) -> int {
-                    hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(nb)::value, decltype(bias)::value, decltype(dx)::value>),
+                    hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(dx)::value>),
                                        dim3((unsigned)(n.x_groups * n.x_splits)), dim3(256), 0, s, p, (int)n.x_splits, n.x_per, (int)width_out, part, z_target,
                                        dx_part);
                     RECO_CHECK_LAUNCH();
@@ -515,12 +650,15 @@ int narrow_cols(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_
 {
     return reco_with_type(dtype, [&](auto z) -> int {
         typedef decltype(z) T;
-        return shape_of<T>(p.D, [&](auto dp, auto nb, int64_t) -> int {
+        return shape_of<T>(p.D, [&](auto dp, int64_t) -> int {
             return with_flag(p.bias != nullptr, [&](auto bias) -> int {
                 return with_flag(gn != nullptr, [&](auto each) -> int {
-                    hipLaunchKernelGGL((narrow_cols_kernel<T, decltype(dp)::value, decltype(nb)::value, decltype(bias)::value, decltype(each)::value>),
-                                       dim3((unsigned)(n.w_groups * n.w_splits)), dim3(256), 0, s, p, (int)n.w_splits, n.w_per, (int)width_out, expo, y, rest, gn,
-                                       scale, (T*)dw, (T*)db, dw_part, db_part);
+                    hipLaunchKernelGGL((narrow_cols_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(each)::value>), dim3((unsigned)n.w_shares),
+                                       dim3(256), 0, s, p, n.w_groups * n.w_tiles, n.w_share, (int)n.w_tiles, (int)width_out, expo, y, rest, gn, scale, (T*)dw,
+                                       (T*)db, dw_part, db_part);
+                    if (n.w_shared)
+                        hipLaunchKernelGGL(narrow_join_kernel<T>, dim3((unsigned)n.w_groups, (unsigned)ceil_div64(HELD * (width_out + 1), 1024)), dim3(256), 0, s, p.V,
+                                           n.w_share, (int)n.w_tiles, (int)width_out, scale, dw_part, db_part, (T*)dw, (T*)db);
                     RECO_CHECK_LAUNCH();
                     return RECO_OK;
                 });

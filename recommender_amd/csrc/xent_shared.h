@@ -63,9 +63,11 @@ __device__ __forceinline__ Running joined(Running a, Running b)
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
-// The form for narrow rows (xent_narrow.hip): held rows are split into groups, streamed ones into splits of `per` rows
+// The form for narrow rows (xent_narrow.hip).  x: groups of held rows, times splits of `per` vocabulary rows.  w: groups of held
+// vocabulary rows, times tiles of x rows, in shares of consecutive (group, tile) units; shared: some group has parts in several.
 struct NarrowPlan {
-    int64_t x_groups, x_splits, x_per, w_groups, w_splits, w_per;
+    int64_t x_groups, x_splits, x_per, w_groups, w_tiles, w_share, w_shares;
+    bool w_shared;
 };
 bool narrow_fits(int dtype, int64_t D);
 NarrowPlan narrow_plan(int dtype, int64_t T, int64_t V, int64_t D);

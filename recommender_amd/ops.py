@@ -3,6 +3,7 @@
 Everything here runs on the GPU through libreco_hip.so; there is no eager-PyTorch arithmetic on the
 product path.  torch is used for allocation (torch.empty), streams and device guards only.
 """
+import contextlib
 import ctypes
 import os
 
@@ -127,6 +128,23 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+# The training-side calls are short beside what Python adds to them: pointers go as plain integers, the device guard is entered only
+# where another device is current.
+_no_guard = contextlib.nullcontext()
+
+
+def _on(device):
+    return _no_guard if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _number(v, name):
     if isinstance(v, torch.Tensor) or isinstance(v, bool):
         raise TypeError("%s must be a number, got %s" % (name, type(v).__name__))
@@ -151,31 +169,52 @@ def _no_captured_graph(what, instead):
 
 
 def _embedding(ids, table, scale, check_ids):
-    out = torch.empty((ids.numel(), table.shape[1]), dtype=table.dtype, device=table.device)
+    dev, (rows, dim), n = table.device, table.shape, ids.numel()
+    out = torch.empty((n, dim), dtype=table.dtype, device=dev)
     if out.numel() == 0:
         return out
-    oob = torch.zeros(1, dtype=torch.int32, device=table.device) if check_ids else None
-    with torch.cuda.device(table.device):
-        check(_lib.lib().reco_embedding(_p(table), table.shape[0], _ld(table), table.shape[1], DTYPES[table.dtype], _p(ids), ids.numel(),
-                                        scale, _p(out), _p(oob), _stream(table.device)))
+    oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
+    with _on(dev):
+        check(_lib.lib().reco_embedding(table.data_ptr(), rows, _ld(table), dim, DTYPES[table.dtype], ids.data_ptr(), n, scale, out.data_ptr(), _at(oob),
+                                        _raw_stream(dev)))
     if check_ids and int(oob.item()):
         raise IndexError("index out of range in self")
     return out
 
 
+def _embedding_grad(ids, grad, rows, scale, padding):
+    n, dim = grad.shape
+    dev = grad.device
+    out = torch.empty((rows, dim), dtype=grad.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    L = _lib.lib()
+    nbytes = L.reco_embedding_grad_workspace_bytes(n, rows, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev):
+        check(L.reco_embedding_grad(ids.data_ptr(), n, grad.data_ptr(), _ld(grad), dim, DTYPES[grad.dtype], rows, scale, padding, out.data_ptr(), _at(ws),
+                                    nbytes, _raw_stream(dev)))
+    return out
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, ids, scale, padding, check_ids):
+    def forward(ctx, table, rows, ids, scale, padding, check_ids):
         ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.padding = table.shape[0], scale, padding
-        return _embedding(ids, _rows(table, "table"), scale, check_ids)
+        ctx.args = rows.shape[0], scale, padding
+        return _embedding(ids, rows, scale, check_ids)
+
+    @staticmethod
+    def backward(ctx, grad):
+        _no_captured_graph("embedding's backward pass", "embedding_grad")
+        if torch.is_grad_enabled():                     # create_graph: the result refuses to be differentiated again
+            return _Embedding.once(ctx, grad)
+        return _embedding_grad(ctx.saved_tensors[0], _rows(grad, "grad"), *ctx.args), None, None, None, None, None
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        _no_captured_graph("embedding's backward pass", "embedding_grad")
-        (ids,) = ctx.saved_tensors
-        return embedding_grad(ids, grad, ctx.rows, ctx.scale, ctx.padding if ctx.padding >= 0 else None), None, None, None, None
+    def once(ctx, grad):
+        return _Embedding.backward(ctx, grad)
 
 
 def embedding(ids, table, scale=1.0, padding_idx=None, check_ids=True):
@@ -194,7 +233,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None, check_ids=True):
     ids = _i64(ids, "ids", t.device)
     if torch.is_grad_enabled() and table.requires_grad:
         _no_captured_graph("embedding", "embedding_grad")
-        out = _Embedding.apply(table, ids, scale, padding, check_ids)
+        out = _Embedding.apply(table, t, ids, scale, padding, check_ids)
     else:
         out = _embedding(ids, t, scale, check_ids)
     return out if shape is None or len(shape) == 1 else out.view(shape + (t.shape[1],))
@@ -213,20 +252,9 @@ def embedding_grad(ids, grad, rows, scale=1.0, padding_idx=None):
     if isinstance(ids, torch.Tensor) and ids.dim() != 1:
         ids = ids.reshape(-1)
     ids = _i64(ids, "ids", grad.device)
-    n, dim = grad.shape
-    if ids.numel() != n:
-        raise ValueError("grad has %d rows for %d ids" % (n, ids.numel()))
-    padding = _padding(padding_idx, rows)
-    out = torch.empty((rows, dim), dtype=grad.dtype, device=grad.device)
-    if out.numel() == 0:
-        return out
-    L = _lib.lib()
-    nbytes = L.reco_embedding_grad_workspace_bytes(n, rows, dim)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
-    with torch.cuda.device(grad.device):
-        check(L.reco_embedding_grad(_p(ids), n, _p(grad), _ld(grad), dim, DTYPES[grad.dtype], rows, scale, padding, _p(out), _p(ws), nbytes,
-                                    _stream(grad.device)))
-    return out
+    if ids.numel() != grad.shape[0]:
+        raise ValueError("grad has %d rows for %d ids" % (grad.shape[0], ids.numel()))
+    return _embedding_grad(ids, grad, rows, scale, _padding(padding_idx, rows))
 
 
 # ----------------------------------------------------------------------------------------------
@@ -503,62 +531,69 @@ def _xent_args(x, weight, target, bias, reduction, ignore_index):
 
 
 def _xent(x, weight, target, bias, reduction, ignore_index, check_ids, with_dx):
-    """(loss, state, dx_unit) of checked operands; with_dx: a gradient of x will be asked for (see reco_linear_xent)."""
+    """(loss, state) of checked operands; with_dx: a gradient of x will be asked for (state begins with dx_unit, see
+    reco_linear_xent)."""
     T, D = x.shape
-    dev = x.device
+    dev, dtype, V = x.device, DTYPES[x.dtype], weight.shape[0]
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    state = torch.empty(2 * T + 1, dtype=torch.float32, device=dev)
     if T == 0:
-        return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), state, None
-    oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
+        return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), None
     L = _lib.lib()
-    what = (_p(x), _ld(x), _p(weight), _ld(weight))
-    floats = L.reco_linear_xent_dx_floats(DTYPES[x.dtype], T, D) if with_dx else 0
-    dx_unit = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-    nbytes = L.reco_linear_xent_workspace_bytes(*what, DTYPES[x.dtype], T, weight.shape[0], D, 1 if floats else 0)
+    floats = L.reco_linear_xent_dx_floats(dtype, T, D) if with_dx else 0
+    state = torch.empty(floats + 2 * T + 1, dtype=torch.float32, device=dev)
+    at = state.data_ptr()
+    oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
+    what = (x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight))
+    nbytes = L.reco_linear_xent_workspace_bytes(*what, dtype, T, V, D, 1 if floats else 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        check(L.reco_linear_xent(*what, _p(bias), DTYPES[x.dtype], T, weight.shape[0], D, _p(target), ignore_index, REDUCTIONS[reduction], _p(loss),
-                                 _p(state), _p(dx_unit), _p(oob), _p(ws), nbytes, _stream(dev)))
+    with _on(dev):
+        check(L.reco_linear_xent(*what, _at(bias), dtype, T, V, D, target.data_ptr(), ignore_index, REDUCTIONS[reduction], loss.data_ptr(), at + 4 * floats,
+                                 at if floats else None, _at(oob), ws.data_ptr(), nbytes, _raw_stream(dev)))
     if check_ids and int(oob.item()):
         raise IndexError("index out of range in self")
-    return loss, state, dx_unit
+    return loss, state
 
 
-def _xent_grad(x, weight, target, bias, state, dx_unit, dloss, reduction, ignore_index, wanted):
+def _xent_grad(x, weight, target, bias, state, dloss, reduction, ignore_index, wanted):
     T, D = x.shape
-    V, dev = weight.shape[0], x.device
-    out = [torch.empty(s, dtype=x.dtype, device=dev) if w else None for w, s in zip(wanted, ((T, D), (V, D), (V,)))]
+    V, dev, dtype = weight.shape[0], x.device, DTYPES[x.dtype]
+    dx = torch.empty((T, D), dtype=x.dtype, device=dev) if wanted[0] else None
+    dw = torch.empty((V, D), dtype=x.dtype, device=dev) if wanted[1] else None
+    db = torch.empty(V, dtype=x.dtype, device=dev) if wanted[2] else None
     if T == 0:
-        return [o if o is None else o.zero_() for o in out]
+        return [o if o is None else o.zero_() for o in (dx, dw, db)]
     L = _lib.lib()
-    what = (_p(x), _ld(x), _p(weight), _ld(weight))
-    nbytes = L.reco_linear_xent_grad_workspace_bytes(*what, DTYPES[x.dtype], T, V, D)
+    floats = state.numel() - 2 * T - 1
+    at = state.data_ptr()
+    what = (x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight))
+    nbytes = L.reco_linear_xent_grad_workspace_bytes(*what, dtype, T, V, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        check(L.reco_linear_xent_grad(*what, _p(bias), DTYPES[x.dtype], T, V, D, _p(target), ignore_index, REDUCTIONS[reduction], _p(state), _p(dx_unit),
-                                      _p(dloss), _p(out[0]), _p(out[1]), _p(out[2]), _p(ws), nbytes, _stream(dev)))
-    return out
+    with _on(dev):
+        check(L.reco_linear_xent_grad(*what, _at(bias), dtype, T, V, D, target.data_ptr(), ignore_index, REDUCTIONS[reduction], at + 4 * floats,
+                                      at if floats else None, dloss.data_ptr(), _at(dx), _at(dw), _at(db), ws.data_ptr(), nbytes, _raw_stream(dev)))
+    return dx, dw, db
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, target, reduction, ignore_index, check_ids):
-        xr, wr, target, br = _xent_args(x, weight, target, bias, reduction, ignore_index)
-        loss, state, dx_unit = _xent(xr, wr, target, br, reduction, ignore_index, check_ids, ctx.needs_input_grad[0])
-        ctx.save_for_backward(x, weight, bias, target, state, dx_unit)
-        ctx.reduction, ctx.ignore_index = reduction, ignore_index
+    def forward(ctx, x, weight, bias, rows, target, reduction, ignore_index, check_ids):
+        xr, wr, br = rows
+        loss, state = _xent(xr, wr, target, br, reduction, ignore_index, check_ids, ctx.needs_input_grad[0])
+        ctx.save_for_backward(xr, wr, target, br, state)
+        ctx.args = reduction, ignore_index
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         _no_captured_graph("linear_cross_entropy's backward pass", "linear_cross_entropy_grad")
-        x, weight, bias, target, state, dx_unit = ctx.saved_tensors
-        bias = None if bias is None else bias.contiguous()
-        grads = _xent_grad(_rows(x, "input"), _rows(weight, "weight"), target, bias, state, dx_unit, dloss.contiguous(), ctx.reduction,
-                           ctx.ignore_index, ctx.needs_input_grad[:3])
-        return tuple(grads) + (None,) * 4
+        if torch.is_grad_enabled():                     # create_graph: the result refuses to be differentiated again
+            return _LinearCrossEntropy.once(ctx, dloss)
+        return (*_xent_grad(*ctx.saved_tensors, dloss.contiguous(), *ctx.args, ctx.needs_input_grad[:3]), None, None, None, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def once(ctx, dloss):
+        return _LinearCrossEntropy.backward(ctx, dloss)
 
 
 def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, check_ids=True):
@@ -571,10 +606,11 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     IndexError; check_ids=False skips that report (one device-to-host sync) and clamps them.  Inside a HIP graph: under no_grad with
     check_ids=False, and linear_cross_entropy_grad for the gradients.
     """
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
+    xr, wr, target, br = _xent_args(x, weight, target, bias, reduction, ignore_index)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         _no_captured_graph("linear_cross_entropy", "linear_cross_entropy_grad")
-        return _LinearCrossEntropy.apply(x, weight, bias, target, reduction, ignore_index, check_ids)
-    return _xent(*_xent_args(x, weight, target, bias, reduction, ignore_index), reduction, ignore_index, check_ids, False)[0]
+        return _LinearCrossEntropy.apply(x, weight, bias, (xr, wr, br), target, reduction, ignore_index, check_ids)
+    return _xent(xr, wr, target, br, reduction, ignore_index, check_ids, False)[0]
 
 
 def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ignore_index=-100, grad=None):
@@ -586,8 +622,8 @@ def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ig
         grad = torch.ones(shape, dtype=torch.float32, device=x.device)
     elif not isinstance(grad, torch.Tensor) or grad.dtype != torch.float32 or grad.device != x.device or tuple(grad.shape) != shape:
         raise ValueError("grad must be a float32 tensor of shape %s on %s" % (shape, x.device))
-    loss, state, dx_unit = _xent(x, weight, target, bias, reduction, ignore_index, False, True)
-    return (loss, *_xent_grad(x, weight, target, bias, state, dx_unit, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
+    loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False, True)
+    return (loss, *_xent_grad(x, weight, target, bias, state, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
 
 
 # ----------------------------------------------------------------------------------------------

@@ -137,8 +137,9 @@ def test_loss_and_gradients(dtype, T, V, D):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,V,D", [(4200, 9000, 24), (5000, 4000, 300), (17000, 300, 40)])
-def test_larger_than_one_piece(dtype, T, V, D):
+@pytest.mark.parametrize("T,V,D", [(4200, 9000, 24), (5000, 4000, 300), (17000, 300, 40), (2100, 5000, 60), (2100, 5000, 100), (2100, 5003, 128), (2100, 5000, 250),
+                                   (4500, 3001, 192), (300, 40000, 16)])
+def test_many_tiles_and_pieces(dtype, T, V, D):
     x, w, target, b = _problem(T, V, D, dtype, True)
     _check(x, w, target, b, "mean")
 
