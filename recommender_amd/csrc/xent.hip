@@ -21,36 +21,43 @@ namespace {
 using namespace xent;
 
 // ---------------------------------------------------------------------------------------------
-// a 128 x 128 tile of a matrix product: 4 waves, 64 x 64 each; operands staged through LDS, the next step's in registers meanwhile
+// a B x B tile of a matrix product, B = 256 (8 waves, 128 x 64 each) or 128 (4 waves, 64 x 64 each): operands staged through LDS, two
+// steps of k in it; the next one arrives in registers while this one is multiplied; one barrier per step
 // ---------------------------------------------------------------------------------------------
-constexpr int TB = 128;
+constexpr int TB = 128;          // sizes of slices and paddings are multiples of this
 
-// A matrix of which 128 rows r take part: KC: element (r, k) at p[r * ld + k], else at p[k * ld + r].  Row starts are 16-byte
-// aligned; `rows` and `k_end` count whole VEC groups along the contiguous side.
+// A matrix of which B rows r take part: KC: element (r, k) at p[r * ld + k], else at p[k * ld + r].  Row starts are 16-byte aligned;
+// `rows` (the limit of r) and k_end count whole VEC groups along the contiguous side.
 template <typename T> struct Operand {
     const T* p;
     int64_t ld;
     int64_t rows;
-    const int* keep;          // !KC: k rows whose keep[k] is negative are read as zeros (nullable)
 };
 
-template <typename T, bool KC> struct Stage {
+template <int B> struct Shape {
+    static constexpr int THREADS = B * 2, WAVES_N = B / 64, WM = B == 256 ? 128 : 64, WN = 64, MB = WM / 32, NB = 2;
+    static __device__ __forceinline__ int wm() { return (threadIdx.x >> 6) / WAVES_N * WM; }
+    static __device__ __forceinline__ int wn() { return (threadIdx.x >> 6) % WAVES_N * WN; }
+};
+
+// 64 (32-bit: 32) of k for B rows in LDS, without padding: the 16-byte chunks of a stored row change places with the row, so that 16 rows
+// at one chunk, or 4 rows at 64 bytes (the transposed reads), spread over the 64 banks
+template <typename T, bool KC, int B> struct Stage {
     static constexpr int VEC = Traits<T>::VEC, BK = Traits<T>::BK;
-    static constexpr int PITCH = KC ? BK + VEC : TB + VEC;             // 16 bytes of padding: rows start on different banks
-    static constexpr int SIZE = (KC ? TB : BK) * PITCH;
-    static constexpr int PER_ROW = (KC ? BK : TB) / VEC;               // 16-byte pieces per stored row
-    static constexpr int PIECES = 4;                                   // per thread: 1,024 in all
+    static constexpr int ROW = KC ? BK : B, CH = ROW / VEC, ROWS = KC ? B : BK;
+    static constexpr int SIZE = ROWS * ROW, PIECES = ROWS * CH / Shape<B>::THREADS, ROW_STEP = Shape<B>::THREADS / CH;
     Pack<T, VEC> reg[PIECES];
+
+    static __device__ __forceinline__ int twist(int row) { return KC ? (row >> 1) & 7 : ((row >> 2) & 3) | (row & 3) << 2; }
 
     __device__ __forceinline__ void load(const Operand<T>& o, int64_t r0, int64_t k0, int64_t k_end)
     {
+        const int col = threadIdx.x % CH * VEC, row = threadIdx.x / CH;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int c = threadIdx.x + 256 * i, row = c / PER_ROW, col = (c % PER_ROW) * VEC;
-            const int64_t r = r0 + (KC ? row : col), k = k0 + (KC ? col : row);
-            bool ok = r < o.rows && k < k_end;
-            if (!KC && ok && o.keep) ok = o.keep[k] >= 0;
-            if (ok) {
+            const int at = row + i * ROW_STEP;
+            const int64_t r = r0 + (KC ? at : col), k = k0 + (KC ? col : at);
+            if (r < o.rows && k < k_end) {
                 reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(o.p + (KC ? r * o.ld + k : k * o.ld + r));
             } else {
 #pragma unroll
@@ -60,133 +67,193 @@ template <typename T, bool KC> struct Stage {
     }
     __device__ __forceinline__ void store(T* lds) const
     {
+        const int c = threadIdx.x % CH, row = threadIdx.x / CH;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int c = threadIdx.x + 256 * i;
-            *reinterpret_cast<Pack<T, VEC>*>(lds + (c / PER_ROW) * PITCH + (c % PER_ROW) * VEC) = reg[i];
+            const int at = row + i * ROW_STEP;
+            *reinterpret_cast<Pack<T, VEC>*>(lds + at * ROW + ((c ^ twist(at)) * VEC)) = reg[i];
         }
     }
-    // rows r .. r + 31 and one KSTEP of k from LDS
+    // rows r .. r + 31 (r a multiple of 32) and one KSTEP of k (a multiple of KSTEP) from LDS
     static __device__ __forceinline__ typename Traits<T>::frag frag(const T* lds, int r, int k)
     {
-        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
         typename Traits<T>::frag f;
         if constexpr (KC) {
-            f = *reinterpret_cast<const typename Traits<T>::frag*>(lds + (r + (lane & 31)) * PITCH + k + half * VEC);
+            f = *reinterpret_cast<const typename Traits<T>::frag*>(lds + (r + l31) * ROW + (((k / VEC + half) ^ twist(l31)) * VEC));
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = lds[(k + 4 * half + i) * PITCH + r + (lane & 31)];
+            for (int i = 0; i < 4; ++i) {
+                const int row = k + 4 * half + i;
+                f[i] = lds[row * ROW + (((r + l31) / 4) ^ twist(row)) * 4 + (l31 & 3)];
+            }
         } else {
             // 16 lanes read 4 k rows of 16 values and get them transposed: lane i value i of each row
-            const T* src = lds + (k + 8 * half + ((lane & 15) >> 2)) * PITCH + r + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            const int row = k + 8 * half + ((lane & 15) >> 2), c = r / 8 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), in = (lane & 1) * 4;
             typedef __attribute__((address_space(3))) s16x4* lds_ptr;
             union { s16x4 h[2]; typename Traits<T>::frag f; } u;
-            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)src);
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(src + 4 * PITCH));
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + row * ROW + (c ^ twist(row)) * 8 + in));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (row + 4) * ROW + (c ^ twist(row + 4)) * 8 + in));
             f = u.f;
         }
         return f;
     }
 };
 
-// acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end)
-template <typename T, bool AKC, bool BKC>
-__device__ __forceinline__ void tile_product(f32x16 (&acc)[2][2], const Operand<T>& A, const Operand<T>& B, int64_t m0, int64_t n0, int64_t k0,
-                                             int64_t k_end, T* la, T* lb)
+// Workgroups with the same number modulo 8 run on the same XCD, which has a cache of its own: the n-th of `total` takes the place that
+// gives every XCD a contiguous run of places.  Neighbouring places share panels.
+__device__ __forceinline__ int64_t place_of(int64_t n, int64_t total)
 {
+    const int64_t q = total / 8, r = total % 8, xcd = n % 8;
+    return xcd * q + (xcd < r ? xcd : r) + n / 8;
+}
+
+// Places as (a, b), a < na: runs of 4 a beside each other, so that 32 consecutive places hold 4 a times 8 b
+__device__ __forceinline__ void pair_of(int64_t place, int64_t na, int64_t nb, int64_t& a, int64_t& b)
+{
+    const int64_t group = place / (4 * nb), in = place - group * 4 * nb, wide = na - group * 4 < 4 ? na - group * 4 : 4;
+    a = group * 4 + in % wide;
+    b = in / wide;
+}
+
+template <typename T, bool AKC, bool BKC, int B> struct TileLds {
+    T a[2][Stage<T, AKC, B>::SIZE];
+    T b[2][Stage<T, BKC, B>::SIZE];
+};
+
+template <int B> using Acc = f32x16[Shape<B>::MB][Shape<B>::NB];
+
+// acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end)
+template <typename T, bool AKC, bool BKC, int B>
+__device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, const Operand<T>& Bm, int64_t m0, int64_t n0, int64_t k0, int64_t k_end,
+                                             TileLds<T, AKC, BKC, B>& lds)
+{
+    typedef Shape<B> S;
     constexpr int BK = Traits<T>::BK, KSTEP = Traits<T>::KSTEP;
-    const int wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    Stage<T, AKC> sa;
-    Stage<T, BKC> sb;
+    const int wm = S::wm(), wn = S::wn();
+    Stage<T, AKC, B> sa;
+    Stage<T, BKC, B> sb;
     sa.load(A, m0, k0, k_end);
-    sb.load(B, n0, k0, k_end);
-    for (int64_t k = k0; k < k_end; k += BK) {
-        __syncthreads();
-        sa.store(la);
-        sb.store(lb);
-        __syncthreads();
-        if (k + BK < k_end) {
+    sb.load(Bm, n0, k0, k_end);
+    __syncthreads();                                     // the last product's LDS is free
+    sa.store(lds.a[0]);
+    sb.store(lds.b[0]);
+    __syncthreads();
+    int at = 0;
+#pragma unroll 1
+    for (int64_t k = k0; k < k_end; k += BK, at ^= 1) {
+        const bool more = k + BK < k_end;
+        if (more) {
             sa.load(A, m0, k + BK, k_end);
-            sb.load(B, n0, k + BK, k_end);
+            sb.load(Bm, n0, k + BK, k_end);
         }
+        const T *la = lds.a[at], *lb = lds.b[at];
 #pragma unroll
         for (int s = 0; s < BK; s += KSTEP) {
-            typename Traits<T>::frag a[2], b[2];
+            typename Traits<T>::frag a[S::MB], b[S::NB];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = Stage<T, AKC>::frag(la, wm + 32 * i, s);
-                b[i] = Stage<T, BKC>::frag(lb, wn + 32 * i, s);
+            for (int j = 0; j < S::NB; ++j) b[j] = Stage<T, BKC, B>::frag(lb, wn + 32 * j, s);
+#pragma unroll
+            for (int i = 0; i < S::MB; ++i) a[i] = Stage<T, AKC, B>::frag(la, wm + 32 * i, s);
+            if constexpr (sizeof(T) == 4) {
+                // the four products of a fragment pair add to one accumulator: those of the other pairs stand between them
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                        for (int j = 0; j < S::NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][u], b[j][u], acc[i][j], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::NB; ++j) mma(acc[i][j], a[i], b[j]);
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) mma(acc[i][j], a[i], b[j]);
         }
+        if (more) {
+            sa.store(lds.a[at ^ 1]);
+            sb.store(lds.b[at ^ 1]);
+        }
+        __syncthreads();
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void stats_kernel(Problem p, int64_t tiles_per_split, Running* __restrict__ part, float* __restrict__ z_target)
+template <typename T, int B>
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, int64_t splits, int64_t tiles_per_split, Running* __restrict__ part, float* __restrict__ z_target)
 {
-    __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
-    __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
-    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr}, X{(const T*)p.x, p.ldx, p.T, nullptr};
+    typedef Shape<B> S;
+    int64_t token_tile, split;
+    pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, splits, token_tile, split);
+    __shared__ __attribute__((aligned(16))) TileLds<T, true, true, B> lds;
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
     const T* bias = (const T*)p.bias;
-    const int64_t n0 = (int64_t)blockIdx.x * TB;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    int64_t y[2];
-    Running run[2];
+    const int64_t n0 = token_tile * B;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
+    int64_t y[S::NB];
+    Running run[S::NB];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < S::NB; ++j) {
         const int64_t t = n0 + wn + 32 * j + (lane & 31);
         y[j] = -1;
         if (t < p.T && p.target[t] != p.ignore) y[j] = clamp_target(p.target[t], p.V);
         run[j] = Running{-INFINITY, 0.f};
     }
-    const int64_t first = blockIdx.y * tiles_per_split * TB;
-    const int64_t end = first + tiles_per_split * TB < p.V ? first + tiles_per_split * TB : p.V;
-    for (int64_t m0 = first; m0 < end; m0 += TB) {
-        f32x16 acc[2][2] = {};
-        tile_product<T, true, true>(acc, W, X, m0, n0, 0, p.D, la, lb);
+    const int64_t first = split * tiles_per_split * B;
+    const int64_t end = first + tiles_per_split * B < p.V ? first + tiles_per_split * B : p.V;
+#pragma unroll 1
+    for (int64_t m0 = first; m0 < end; m0 += B) {
+        Acc<B> acc = {};
+        tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, lds);
+        if (bias)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int64_t t = n0 + wn + 32 * j + (lane & 31);
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S::MB; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
-                    float z = acc[i][j][r];
-                    if (bias && v < p.V) z += (float)bias[v];
-                    if (v >= p.V) z = -INFINITY;
-                    if (v == y[j]) {
-                        z_target[t] = z;
-                        z = -INFINITY;
-                    }
-                    acc[i][j][r] = z;
-                    top = fmaxf(top, z);
+                    const float z = v < p.V ? (float)bias[v] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
                 }
+        const bool tail = m0 + B > p.V;
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) {
+            const int64_t t = n0 + wn + 32 * j + (lane & 31);
+            const int64_t here = y[j] - m0;
+            if (tail || __any(here >= 0 && here < B)) {
+#pragma unroll
+                for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
+                        if (v == y[j]) z_target[t] = acc[i][j][r];
+                        if (v == y[j] || v >= p.V) acc[i][j][r] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
             const float m = fmaxf(run[j].m, top), base = m == -INFINITY ? 0.f : m;
             float s = run[j].s * exp2f((run[j].m - base) * LOG2E);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += exp2f((acc[i][j][r] - base) * LOG2E);
+                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
             run[j] = Running{m, s};
         }
     }
     __syncthreads();
-    Running* sh = reinterpret_cast<Running*>(la);                // [2 waves along the vocabulary][128 tokens]
+    Running* sh = reinterpret_cast<Running*>(&lds);              // [2 waves along the vocabulary][B tokens]
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < S::NB; ++j) {
         const Running o{__shfl_xor(run[j].m, 32, 64), __shfl_xor(run[j].s, 32, 64)};
         const Running both = half ? joined(o, run[j]) : joined(run[j], o);
-        if (half == 0) sh[(wave >> 1) * TB + wn + 32 * j + lane] = both;
+        if (half == 0) sh[(wm ? B : 0) + wn + 32 * j + lane] = both;
     }
     __syncthreads();
     const int64_t t = n0 + threadIdx.x;
-    if (threadIdx.x < TB && t < p.T) part[(int64_t)blockIdx.y * p.T + t] = joined(sh[threadIdx.x], sh[TB + threadIdx.x]);
+    if (threadIdx.x < B && t < p.T) part[split * p.T + t] = joined(sh[threadIdx.x], sh[B + threadIdx.x]);
 }
 
 // One wave per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
@@ -342,20 +409,32 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ unit,
 }
 
 // G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero
-template <typename T>
-__global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t width, const float* __restrict__ lse, const float* __restrict__ rest,
-                                                const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
+template <typename T, int B>
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int64_t v0, const float* __restrict__ lse, const float* __restrict__ rest,
+                                                                 const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
 {
-    __shared__ __attribute__((aligned(16))) T la[Stage<T, true>::SIZE];
-    __shared__ __attribute__((aligned(16))) T lb[Stage<T, true>::SIZE];
-    const Operand<T> W{(const T*)p.w, p.ldw, p.V, nullptr}, X{(const T*)p.x, p.ldx, p.T, nullptr};
+    typedef Shape<B> S;
+    int64_t token_tile, panel;
+    pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, ldg / B, token_tile, panel);
+    __shared__ __attribute__((aligned(16))) TileLds<T, true, true, B> lds;
+    const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
     const T* bias = (const T*)p.bias;
-    const int64_t n0 = (int64_t)blockIdx.x * TB, m0 = v0 + (int64_t)blockIdx.y * TB;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x16 acc[2][2] = {};
-    tile_product<T, true, true>(acc, W, X, m0, n0, 0, p.D, la, lb);
+    const int64_t n0 = token_tile * B, m0 = v0 + panel * B;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
+    Acc<B> acc = {};
+    tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, lds);
+    if (bias)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+        for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
+                const float z = v < p.V ? (float)bias[v] : 0.f;
+#pragma unroll
+                for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
+            }
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j) {
         const int64_t t = n0 + wn + 32 * j + (lane & 31);
         if (t >= p.T) continue;
         const int64_t y0 = p.target[t];
@@ -363,7 +442,7 @@ __global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t w
         const int64_t y = clamp_target(y0, p.V);
         const float l = lse[t], q = rest[t], g = (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::MB; ++i)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
                 const int64_t v = m0 + wm + 32 * i + 8 * r4 + 4 * half;
@@ -371,9 +450,7 @@ __global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t w
                 Pack<T, 4> o;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    float z = acc[i][j][4 * r4 + u];
-                    if (bias && v + u < p.V) z += (float)bias[v + u];
-                    const float e = v + u == y ? -q : exp2f((z - l) * LOG2E);
+                    const float e = v + u == y ? -q : __builtin_amdgcn_exp2f((acc[i][j][4 * r4 + u] - l) * LOG2E);
                     o.v[u] = (T)(in && v + u < p.V ? e * g : 0.f);
                 }
                 *reinterpret_cast<Pack<T, 4>*>(G + t * ldg + (v - v0)) = o;
@@ -381,30 +458,58 @@ __global__ __launch_bounds__(256) void g_kernel(Problem p, int64_t v0, int64_t w
     }
 }
 
-// Slice blockIdx.z of out [slices][M][N] (+)= A B over its share of k, in 32 bits
-template <typename T, bool AKC, bool BKC>
-__global__ __launch_bounds__(256) void product_kernel(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t K, int64_t k_per_slice, float* out, int add)
+// A B in equal shares: the units are (tile, step of TB in k), the steps of a tile together, tiles of one row of tiles beside each other;
+// every workgroup takes `share` consecutive units and writes the sums of each tile it touches, in 32 bits, to a place of its own: place
+// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.
+template <typename T, bool AKC, bool BKC, int B>
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T> A, Operand<T> Bm, int64_t tiles_n, int64_t K, int64_t steps, int64_t units, int64_t share,
+                                                                       float* __restrict__ part)
 {
-    __shared__ __attribute__((aligned(16))) T la[Stage<T, AKC>::SIZE];
-    __shared__ __attribute__((aligned(16))) T lb[Stage<T, BKC>::SIZE];
-    const int64_t m0 = (int64_t)blockIdx.x * TB, n0 = (int64_t)blockIdx.y * TB;
-    const int64_t k0 = blockIdx.z * k_per_slice, k1 = k0 + k_per_slice < K ? k0 + k_per_slice : K;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x16 acc[2][2] = {};
-    tile_product<T, AKC, BKC>(acc, A, B, m0, n0, k0, k1, la, lb);
-    out += blockIdx.z * M * N;
+    typedef Shape<B> S;
+    __shared__ __attribute__((aligned(16))) TileLds<T, AKC, BKC, B> lds;
+    const int64_t worker = place_of(blockIdx.x, gridDim.x);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
+    const int64_t end = (worker + 1) * share < units ? (worker + 1) * share : units;
+#pragma unroll 1
+    for (int64_t u = worker * share; u < end;) {
+        const int64_t tile = u / steps, step = u - tile * steps, n = end - u < steps - step ? end - u : steps - step;
+        const int64_t k0 = step * TB, k1 = (step + n) * TB < K ? (step + n) * TB : K;
+        u += n;
+        Acc<B> acc = {};
+        tile_product<T, AKC, BKC, B>(acc, A, Bm, tile / tiles_n * B, tile % tiles_n * B, k0, k1, lds);
+        float* out = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < S::NB; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = m0 + wm + 32 * i + acc_row(r, half), n = n0 + wn + 32 * j + (lane & 31);
-                if (m < M && n < N) {
-                    float* o = out + m * N + n;
-                    *o = add ? *o + acc[i][j][r] : acc[i][j][r];
-                }
-            }
+                for (int r = 0; r < 16; ++r) out[(wm + 32 * i + acc_row(r, half)) * B + wn + 32 * j + (lane & 31)] = acc[i][j][r];
+    }
+}
+
+// The places of every tile added; with `sum` [M, N] added to (first: written to) it, or with `out` its total (and sum's, if !first)
+// times scale / G_SCALE rounded to T
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int B, int64_t tiles_n, int64_t steps, int64_t share, int64_t M, int64_t N,
+                                                   const float* __restrict__ scale, int first, float* __restrict__ sum, T* __restrict__ out)
+{
+    const int64_t tile = blockIdx.x, a = tile * steps / share, b = ((tile + 1) * steps - 1) / share;
+    const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
+    const float f = out ? *scale / Traits<T>::G_SCALE : 1.f;
+    for (int i = (blockIdx.y * 256 + threadIdx.x) * 4; i < B * B; i += gridDim.y * 1024) {
+        const int64_t m = m0 + i / B, n = n0 + i % B;
+        if (m >= M || n >= N) continue;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t w = a; w <= b; ++w) s += *reinterpret_cast<const f32x4*>(part + (w * 2 + (w == a ? 1 : 0)) * (B * B) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (n + j >= N) break;
+            float v = s[j];
+            if (sum && !first) v += sum[m * N + n + j];
+            if (out) out[m * N + n + j] = (T)(v * f);
+            else sum[m * N + n + j] = v;
+        }
+    }
 }
 
 // out[i] = scale / G_SCALE * sum over slices, rounded to T
@@ -431,14 +536,15 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ G
     out[blockIdx.y * width + v] = s;
 }
 
-// rows with their width filled up to `ldo` with zeros
+// rows with their width filled up to `ldo` with zeros; rows whose target (nullable) is `ignore` as zeros
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ in, int64_t rows, int64_t ld, int64_t D, T* __restrict__ out, int64_t ldo)
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ in, int64_t rows, int64_t ld, int64_t D, T* __restrict__ out, int64_t ldo,
+                                                   const int64_t* __restrict__ target, int64_t ignore)
 {
     const int64_t n = rows * ldo;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / ldo, c = i - r * ldo;
-        out[i] = c < D ? in[r * ld + c] : (T)0.f;
+        out[i] = c < D && !(target && target[r] == ignore) ? in[r * ld + c] : (T)0.f;
     }
 }
 
@@ -488,60 +594,111 @@ struct ForwardPlan {
     int64_t splits, tiles_per_split;
 };
 
-ForwardPlan forward_plan(int64_t T, int64_t V)
+// 256-wide tiles in 16 bits (a 128-wide one asks LDS for 1.5 times as much per product), 128-wide ones where one side has no more rows,
+// and in 32 bits, whose matrix instructions are 16 times slower and whose smaller tiles fill the chip more evenly
+int tile_of(int size, int64_t rows_a, int64_t rows_b) { return size == 2 && rows_a > 128 && rows_b > 128 ? 256 : 128; }
+
+// workgroups of these kernels that the chip holds at once: one of 8 waves per compute unit, or two of 4
+int64_t places_of(int tile) { return tile == 256 ? 256 : 512; }
+
+// The split of the vocabulary with the fewest rounds of tiles; the longest runs of tiles among equals
+ForwardPlan forward_plan(int64_t T, int64_t V, int tile)
 {
-    const int64_t tiles = ceil_div64(V, TB), rows = ceil_div64(T, TB);
-    ForwardPlan f;
-    f.splits = clamp64(1024 / rows, 1, tiles);
-    f.tiles_per_split = ceil_div64(tiles, f.splits);
-    f.splits = ceil_div64(tiles, f.tiles_per_split);
-    return f;
+    const int64_t tiles = ceil_div64(V, tile), rows = ceil_div64(T, tile);
+    int64_t best = 1, cost = INT64_MAX;
+    for (int64_t per = 1; per <= tiles && per <= 256; ++per) {
+        const int64_t c = ceil_div64(rows * ceil_div64(tiles, per), places_of(tile)) * per;
+        if (c <= cost) {
+            cost = c;
+            best = per;
+        }
+    }
+    // more splits than the sums of a row are worth: at most 2048
+    if (ceil_div64(tiles, best) > 2048) best = ceil_div64(tiles, 2048);
+    return ForwardPlan{ceil_div64(tiles, best), best};
+}
+
+// A product in shares (product_kernel)
+struct ProductPlan {
+    int tile;
+    int64_t tiles_m, tiles_n, steps, units, share, workers;
+    size_t floats;                    // of the places
+};
+
+ProductPlan product_plan(int size, int64_t M, int64_t N, int64_t K)
+{
+    ProductPlan q;
+    q.tile = tile_of(size, M, N);
+    q.tiles_m = ceil_div64(M, q.tile);
+    q.tiles_n = ceil_div64(N, q.tile);
+    q.steps = ceil_div64(K, TB);
+    q.units = q.tiles_m * q.tiles_n * q.steps;
+    q.share = ceil_div64(q.units, places_of(q.tile));
+    q.workers = ceil_div64(q.units, q.share);
+    q.floats = (size_t)q.workers * 2 * q.tile * q.tile;
+    return q;
 }
 
 struct BackwardPlan {
-    int64_t width;                    // vocabulary rows per piece, a multiple of TB
-    int64_t x_slices, w_slices, b_slices;
-    int64_t x_per, w_per, b_per;      // k per slice
+    int64_t width;                    // vocabulary rows per piece, a multiple of 256
+    int64_t b_slices, b_per;          // row slices of G's column sums
 };
 
-constexpr size_t PIECE_BYTES = (size_t)64 << 20;
+constexpr size_t PIECE_BYTES = (size_t)128 << 20;
 
 BackwardPlan backward_plan(int64_t T, int64_t V, int64_t D, int size)
 {
     BackwardPlan b;
-    const int64_t tiles = ceil_div64(V, TB);
-    // the piece of G, and the 32-bit rows of dW that belong to it
-    const int64_t by_g = (int64_t)(PIECE_BYTES / ((size_t)T * size)) / TB, by_w = (int64_t)(4 * PIECE_BYTES / ((size_t)D * 4)) / TB;
-    b.width = clamp64(by_g < by_w ? by_g : by_w, 1, tiles < 32768 ? tiles : 32768) * TB;
-    const int64_t dt = ceil_div64(D, TB), tt = ceil_div64(T, TB);
-    b.x_slices = clamp64(512 / (tt * dt), 1, b.width / TB);
-    b.x_per = ceil_div64(b.width / TB, b.x_slices) * TB;
-    b.x_slices = ceil_div64(b.width, b.x_per);
-    b.w_slices = clamp64(512 / (b.width / TB * dt), 1, tt);
-    b.w_per = ceil_div64(tt, b.w_slices) * TB;
-    b.w_slices = ceil_div64(T, b.w_per);
-    b.b_slices = clamp64(512 / ceil_div64(b.width, 256), 1, tt);
+    const int64_t tiles = ceil_div64(V, 256), by_g = (int64_t)(PIECE_BYTES / ((size_t)T * size)) / 256;
+    b.width = clamp64(by_g, 1, tiles < 16384 ? tiles : 16384) * 256;
+    b.b_slices = clamp64(512 / ceil_div64(b.width, 256), 1, ceil_div64(T, TB));
     b.b_per = ceil_div64(T, b.b_slices);
     b.b_slices = ceil_div64(T, b.b_per);
     return b;
 }
 
-template <typename T> int pack_rows(const Args& a, Problem& p, Carve& c, bool launch, hipStream_t s)
+// `clean`: x copied in any case, rows that do not count as zeros (they are multiplied by zeros, and may hold anything)
+template <typename T> int pack_rows(const Args& a, Problem& p, bool clean, Carve& c, bool launch, hipStream_t s)
 {
     const int64_t padded = ceil_div64(a.D, Traits<T>::VEC) * Traits<T>::VEC;
     p = Problem{a.T, a.V, padded, a.ldx, a.ldw, a.x, a.w, a.bias, a.target, a.ignore};
     struct { const void** p; int64_t* ld; int64_t rows; } in[2] = {{&p.x, &p.ldx, a.T}, {&p.w, &p.ldw, a.V}};
     for (auto& m : in) {
-        if (!must_pack(*m.p, *m.ld, a.D, sizeof(T))) continue;
+        const bool is_x = m.p == &p.x;
+        if (!(clean && is_x) && !must_pack(*m.p, *m.ld, a.D, sizeof(T))) continue;
         T* to = (T*)c.take((size_t)m.rows * padded * sizeof(T));
         if (launch) {
-            hipLaunchKernelGGL(pack_kernel<T>, dim3(stream_blocks(m.rows * padded)), dim3(256), 0, s, (const T*)*m.p, m.rows, *m.ld, a.D, to, padded);
+            hipLaunchKernelGGL(pack_kernel<T>, dim3(stream_blocks(m.rows * padded)), dim3(256), 0, s, (const T*)*m.p, m.rows, *m.ld, a.D, to, padded,
+                               clean && is_x ? a.target : nullptr, a.ignore);
             RECO_CHECK_LAUNCH();
             *m.p = to;
             *m.ld = padded;
         }
     }
     return RECO_OK;
+}
+
+template <typename T, typename F> int with_tile(int tile, F&& fn)
+{
+    if constexpr (sizeof(T) == 2)
+        if (tile == 256) return fn(std::integral_constant<int, 256>());
+    return fn(std::integral_constant<int, 128>());
+}
+
+// sum (+)= A B, or with `out` its (and sum's) total times *scale, rounded to T
+template <typename T, bool AKC, bool BKC>
+int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t N, int64_t K, const float* scale, bool first, float* part, float* sum, T* out,
+                   hipStream_t s)
+{
+    const ProductPlan q = product_plan(sizeof(T), M, N, K);
+    return with_tile<T>(q.tile, [&](auto t) -> int {
+        constexpr int W = decltype(t)::value;
+        hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W>), dim3((unsigned)q.workers), dim3(Shape<W>::THREADS), 0, s, A, B, q.tiles_n, K, q.steps, q.units, q.share, part);
+        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / 4096)), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
+                           scale, first, sum, out);
+        RECO_CHECK_LAUNCH();
+        return RECO_OK;
+    });
 }
 
 constexpr int REDUCE_ROWS = 16384;            // rows that one workgroup reduces by itself
@@ -552,7 +709,8 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     Carve c{ws};
     Problem p;
     const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
-    const ForwardPlan f = forward_plan(a.T, a.V);
+    const int tile = tile_of(sizeof(T), a.T, a.V);
+    const ForwardPlan f = forward_plan(a.T, a.V, tile);
     const NarrowPlan n = narrow ? narrow_plan(a.dtype, a.T, a.V, a.D) : NarrowPlan{};
     const int64_t splits = narrow ? n.x_splits : f.splits;
     Running* part = (Running*)c.take((size_t)splits * a.T * sizeof(Running));
@@ -560,7 +718,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     float* rows = (float*)c.take((size_t)a.T * 4);
     float2* sums = (float2*)c.take(256 * sizeof(float2));
     float* dx_part = narrow && with_dx ? (float*)c.take((size_t)splits * a.T * a.D * 4) : nullptr;
-    const int rc = pack_rows<T>(a, p, c, launch, s);
+    const int rc = pack_rows<T>(a, p, false, c, launch, s);
     if (rc) return rc;
     *need = c.used;
     if (!launch) return RECO_OK;
@@ -569,7 +727,13 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
         const int rn = narrow_rows(a.dtype, p, n, a.D, part, z_target, dx_part, s);
         if (rn) return rn;
     } else {
-        hipLaunchKernelGGL(stats_kernel<T>, dim3((unsigned)ceil_div64(a.T, TB), (unsigned)splits), dim3(256), 0, s, p, f.tiles_per_split, part, z_target);
+        const int rs = with_tile<T>(tile, [&](auto t) -> int {
+            constexpr int B = decltype(t)::value;
+            hipLaunchKernelGGL((stats_kernel<T, B>), dim3((unsigned)(ceil_div64(a.T, B) * splits)), dim3(Shape<B>::THREADS), 0, s, p, splits, f.tiles_per_split,
+                               part, z_target);
+            return RECO_OK;
+        });
+        if (rs) return rs;
     }
     hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, splits, z_target, rows, state, state + a.T, oob, dx_part, a.D,
                        dx_part ? dx_unit : nullptr);
@@ -606,11 +770,12 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
         }
     } else {
         G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
-        x_part = (float*)c.take((size_t)b.x_slices * a.T * a.D * 4);
-        w_part = (float*)c.take((size_t)b.w_slices * b.width * a.D * 4);
+        const size_t xf = product_plan(sizeof(T), a.T, a.D, b.width).floats, wf = product_plan(sizeof(T), b.width, a.D, a.T).floats;
+        w_part = (float*)c.take((xf > wf ? xf : wf) * 4);
+        if (b.width < a.V) x_part = (float*)c.take((size_t)a.T * a.D * 4);
         b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
     }
-    const int rc = pack_rows<T>(a, p, c, launch, s);
+    const int rc = pack_rows<T>(a, p, !narrow, c, launch, s);
     if (rc) return rc;
     *need = c.used;
     if (!launch) return RECO_OK;
@@ -631,23 +796,19 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
         RECO_CHECK_LAUNCH();
         return RECO_OK;
     }
-    const unsigned tt = (unsigned)ceil_div64(a.T, TB), dt = (unsigned)ceil_div64(a.D, TB);
     for (int64_t v0 = 0; v0 < a.V; v0 += b.width) {
-        const int64_t width = a.V - v0 < b.width ? a.V - v0 : b.width, ldg = ceil_div64(width, TB) * TB;
-        hipLaunchKernelGGL(g_kernel<T>, dim3(tt, (unsigned)(ldg / TB)), dim3(256), 0, s, p, v0, width, lse, rest, gn, G, ldg);
-        if (dx) {
-            // a slice without k of this (shorter) piece adds nothing; the first piece, which sets the slices, has k for all
-            const Operand<T> A{G, ldg, a.T, nullptr}, B{(const T*)p.w + v0 * p.ldw, p.ldw, p.D, nullptr};
-            hipLaunchKernelGGL((product_kernel<T, true, false>), dim3(tt, dt, (unsigned)b.x_slices), dim3(256), 0, s, A, B, a.T, a.D, width, b.x_per, x_part,
-                               v0 > 0);
-        }
-        if (dw) {
-            const Operand<T> A{G, ldg, ldg, nullptr}, B{(const T*)p.x, p.ldx, p.D, y};
-            hipLaunchKernelGGL((product_kernel<T, false, false>), dim3((unsigned)(ldg / TB), dt, (unsigned)b.w_slices), dim3(256), 0, s, A, B, width, a.D, a.T,
-                               b.w_per, w_part, 0);
-            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width * a.D)), dim3(256), 0, s, w_part, (int)b.w_slices, width * a.D, scale,
-                               (T*)dw + v0 * a.D);
-        }
+        const int64_t width = a.V - v0 < b.width ? a.V - v0 : b.width, ldg = ceil_div64(width, 256) * 256;
+        int rl = with_tile<T>(tile_of(sizeof(T), a.T, b.width), [&](auto t) -> int {
+            constexpr int B = decltype(t)::value;
+            hipLaunchKernelGGL((g_kernel<T, B>), dim3((unsigned)(ceil_div64(a.T, B) * (ldg / B))), dim3(Shape<B>::THREADS), 0, s, p, v0, lse, rest, gn, G, ldg);
+            RECO_CHECK_LAUNCH();
+            return RECO_OK;
+        });
+        if (!rl && dx)
+            rl = launch_product<T, true, false>({G, ldg, a.T}, {(const T*)p.w + v0 * p.ldw, p.ldw, p.D}, a.T, a.D, width, scale, v0 == 0, w_part, x_part,
+                                                v0 + width == a.V ? (T*)dx : nullptr, s);
+        if (!rl && dw) rl = launch_product<T, false, false>({G, ldg, ldg}, {(const T*)p.x, p.ldx, p.D}, width, a.D, a.T, scale, true, w_part, nullptr, (T*)dw + v0 * a.D, s);
+        if (rl) return rl;
         if (db) {
             hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(width, 256), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per, width,
                                b_part);
@@ -655,8 +816,6 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
         }
         RECO_CHECK_LAUNCH();
     }
-    if (dx) hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, x_part, (int)b.x_slices, a.T * a.D, scale, (T*)dx);
-    RECO_CHECK_LAUNCH();
     return RECO_OK;
 }
 
