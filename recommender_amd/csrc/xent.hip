@@ -40,47 +40,55 @@ template <int B> struct Shape {
     static __device__ __forceinline__ int wn() { return (threadIdx.x >> 6) % WAVES_N * WN; }
 };
 
-// 64 (32-bit: 32) of k for B rows in LDS, without padding: the 16-byte chunks of a stored row change places with the row, so that 16 rows
-// at one chunk, or 4 rows at 64 bytes (the transposed reads), spread over the 64 banks
+// 64 (32-bit: 32) of k for B rows, on their way from memory to LDS and from there to fragments.  In LDS without padding: the 16-byte
+// chunks of a stored row change places with the row, so that 16 rows at one chunk, or 4 rows at 64 bytes (the transposed reads), spread
+// over the 64 banks.  Memory to LDS without registers: a wave's load fills 1 KB in lane order, so the lanes choose what they fetch.
 template <typename T, bool KC, int B> struct Stage {
+    typedef typename Traits<T>::frag frag;
     static constexpr int VEC = Traits<T>::VEC, BK = Traits<T>::BK;
-    static constexpr int ROW = KC ? BK : B, CH = ROW / VEC, ROWS = KC ? B : BK;
-    static constexpr int SIZE = ROWS * ROW, PIECES = ROWS * CH / Shape<B>::THREADS, ROW_STEP = Shape<B>::THREADS / CH;
-    Pack<T, VEC> reg[PIECES];
+    static constexpr int ROW = KC ? BK : B, CH = ROW / VEC, ROWS = KC ? B : BK, WAVES = Shape<B>::THREADS / 64;
+    static constexpr int SIZE = ROWS * ROW, PIECES = SIZE / VEC / Shape<B>::THREADS, ROW_STEP = ROWS / PIECES;
+    static constexpr uint32_t NOWHERE = 0x80000000u;       // an offset behind every buffer: reads as zeros
+    const T* base;
+    int64_t step;
+    uint32_t offset[PIECES];
+    int k_of;               // KC: this lane's k inside the step; else the k of its first piece
 
     static __device__ __forceinline__ int twist(int row) { return KC ? (row >> 1) & 7 : ((row >> 2) & 3) | (row & 3) << 2; }
 
-    __device__ __forceinline__ void load(const Operand<T>& o, int64_t r0, int64_t k0, int64_t k_end)
+    __device__ __forceinline__ void init(const Operand<T>& o, int64_t r0, int64_t k0)
     {
-        const int col = threadIdx.x % CH * VEC, row = threadIdx.x / CH;
+        const int row = threadIdx.x / CH;
+        base = o.p + (KC ? r0 * o.ld + k0 : k0 * o.ld + r0);
+        step = KC ? BK : BK * o.ld;
+        static_assert(!KC || ROW_STEP % 16 == 0, "every piece of a lane has the same k");
+        k_of = KC ? ((threadIdx.x % CH) ^ twist(row)) * VEC : row;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int at = row + i * ROW_STEP;
-            const int64_t r = r0 + (KC ? at : col), k = k0 + (KC ? col : at);
-            if (r < o.rows && k < k_end) {
-                reg[i] = *reinterpret_cast<const Pack<T, VEC>*>(o.p + (KC ? r * o.ld + k : k * o.ld + r));
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) reg[i].v[j] = (T)0.f;
-            }
+            const int at = row + i * ROW_STEP, col = ((threadIdx.x % CH) ^ twist(at)) * VEC;
+            offset[i] = r0 + (KC ? at : col) < o.rows ? (uint32_t)((at * o.ld + col) * (int64_t)sizeof(T)) : NOWHERE;
         }
     }
-    __device__ __forceinline__ void store(T* lds) const
+    // the next step's values, `left` of k before its end, set out for `lds`
+    __device__ __forceinline__ void load(T* lds, int64_t left)
     {
-        const int c = threadIdx.x % CH, row = threadIdx.x / CH;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        base += step;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int at = row + i * ROW_STEP;
-            *reinterpret_cast<Pack<T, VEC>*>(lds + at * ROW + ((c ^ twist(at)) * VEC)) = reg[i];
+            const bool in = k_of + (KC ? 0 : i * ROW_STEP) < left;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (i * WAVES + wave) * (64 * VEC)), 16,
+                                                     in ? offset[i] : NOWHERE, 0, 0, 0);
         }
     }
     // rows r .. r + 31 (r a multiple of 32) and one KSTEP of k (a multiple of KSTEP) from LDS
-    static __device__ __forceinline__ typename Traits<T>::frag frag(const T* lds, int r, int k)
+    static __device__ __forceinline__ frag fragment(const T* lds, int r, int k)
     {
         const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
-        typename Traits<T>::frag f;
+        frag f;
         if constexpr (KC) {
-            f = *reinterpret_cast<const typename Traits<T>::frag*>(lds + (r + l31) * ROW + (((k / VEC + half) ^ twist(l31)) * VEC));
+            f = *reinterpret_cast<const frag*>(lds + (r + l31) * ROW + (((k / VEC + half) ^ twist(l31)) * VEC));
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -91,7 +99,7 @@ template <typename T, bool KC, int B> struct Stage {
             // 16 lanes read 4 k rows of 16 values and get them transposed: lane i value i of each row
             const int row = k + 8 * half + ((lane & 15) >> 2), c = r / 8 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), in = (lane & 1) * 4;
             typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-            union { s16x4 h[2]; typename Traits<T>::frag f; } u;
+            union { s16x4 h[2]; frag f; } u;
             u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + row * ROW + (c ^ twist(row)) * 8 + in));
             u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (row + 4) * ROW + (c ^ twist(row + 4)) * 8 + in));
             f = u.f;
@@ -116,66 +124,91 @@ __device__ __forceinline__ void pair_of(int64_t place, int64_t na, int64_t nb, i
     b = in / wide;
 }
 
-template <typename T, bool AKC, bool BKC, int B> struct TileLds {
-    T a[2][Stage<T, AKC, B>::SIZE];
-    T b[2][Stage<T, BKC, B>::SIZE];
-};
+// Two steps of both operands: four arrays, so that the compiler sees that what is read is not what is on its way
+#define TILE_LDS(T, AKC, BKC, B)                                                                              \
+    __shared__ __attribute__((aligned(1024))) T lds_a0[Stage<T, AKC, B>::SIZE], lds_a1[Stage<T, AKC, B>::SIZE]; \
+    __shared__ __attribute__((aligned(1024))) T lds_b0[Stage<T, BKC, B>::SIZE], lds_b1[Stage<T, BKC, B>::SIZE]
+#define TILE_LDS_ARGS lds_a0, lds_a1, lds_b0, lds_b1
 
 template <int B> using Acc = f32x16[Shape<B>::MB][Shape<B>::NB];
 
-// acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end)
+// All of this wave's loads and LDS accesses are done, then the workgroup's
+__device__ __forceinline__ void drain_and_meet()
+{
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+}
+
+// acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end).  Fragments are read one KSTEP before they are multiplied.  The barrier
+// stands before the last quarter of a step, whose fragments are in registers already: behind it nobody reads this half of LDS any
+// more, the step after next sets out for it, and the other half has arrived.
 template <typename T, bool AKC, bool BKC, int B>
-__device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, const Operand<T>& Bm, int64_t m0, int64_t n0, int64_t k0, int64_t k_end,
-                                             TileLds<T, AKC, BKC, B>& lds)
+__device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, const Operand<T>& Bm, int64_t m0, int64_t n0, int64_t k0, int64_t k_end, T* a0, T* a1,
+                                             T* b0, T* b1)
 {
     typedef Shape<B> S;
+    typedef Stage<T, AKC, B> SA;
+    typedef Stage<T, BKC, B> SB;
     constexpr int BK = Traits<T>::BK, KSTEP = Traits<T>::KSTEP;
+    static_assert(BK == 4 * KSTEP, "a step is four products deep");
     const int wm = S::wm(), wn = S::wn();
-    Stage<T, AKC, B> sa;
-    Stage<T, BKC, B> sb;
-    sa.load(A, m0, k0, k_end);
-    sb.load(Bm, n0, k0, k_end);
-    __syncthreads();                                     // the last product's LDS is free
-    sa.store(lds.a[0]);
-    sb.store(lds.b[0]);
-    __syncthreads();
-    int at = 0;
-#pragma unroll 1
-    for (int64_t k = k0; k < k_end; k += BK, at ^= 1) {
-        const bool more = k + BK < k_end;
-        if (more) {
-            sa.load(A, m0, k + BK, k_end);
-            sb.load(Bm, n0, k + BK, k_end);
-        }
-        const T *la = lds.a[at], *lb = lds.b[at];
+    SA sa;
+    SB sb;
+    typename Traits<T>::frag a[2][S::MB], b[2][S::NB];
+    auto read = [&](const T* la, const T* lb, int s) {
 #pragma unroll
-        for (int s = 0; s < BK; s += KSTEP) {
-            typename Traits<T>::frag a[S::MB], b[S::NB];
+        for (int j = 0; j < S::NB; ++j) b[s & 1][j] = SB::fragment(lb, wn + 32 * j, s * KSTEP);
 #pragma unroll
-            for (int j = 0; j < S::NB; ++j) b[j] = Stage<T, BKC, B>::frag(lb, wn + 32 * j, s);
+        for (int i = 0; i < S::MB; ++i) a[s & 1][i] = SA::fragment(la, wm + 32 * i, s * KSTEP);
+    };
+    auto multiply = [&](int s) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (sizeof(T) == 4) {
+            // the four products of a fragment pair add to one accumulator: those of the other pairs stand between them
 #pragma unroll
-            for (int i = 0; i < S::MB; ++i) a[i] = Stage<T, AKC, B>::frag(la, wm + 32 * i, s);
-            if constexpr (sizeof(T) == 4) {
-                // the four products of a fragment pair add to one accumulator: those of the other pairs stand between them
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                        for (int j = 0; j < S::NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][u], b[j][u], acc[i][j], 0, 0, 0);
-            } else {
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::NB; ++j) mma(acc[i][j], a[i], b[j]);
-            }
+                    for (int j = 0; j < S::NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s & 1][i][u], b[s & 1][j][u], acc[i][j], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                for (int j = 0; j < S::NB; ++j) mma(acc[i][j], a[s & 1][i], b[s & 1][j]);
         }
-        if (more) {
-            sa.store(lds.a[at ^ 1]);
-            sb.store(lds.b[at ^ 1]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Without a branch, which would part the accumulators' registers: behind the end of k the loads are told to fetch nothing (zeros), an
+    // odd number of steps is rounded up by one of zeros.  left: k from the present step's beginning to the end.
+    int64_t left = k_end - k0;
+    auto step = [&](T* la, T* lb, T* next_a, T* next_b) {
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            read(la, lb, s + 1);
+            multiply(s);
         }
-        __syncthreads();
-    }
+        drain_and_meet();
+        sa.load(la, left - 2 * BK);
+        sb.load(lb, left - 2 * BK);
+        read(next_a, next_b, 0);
+        multiply(3);
+        left -= BK;
+    };
+    sa.init(A, m0, k0);
+    sb.init(Bm, n0, k0);
+    drain_and_meet();                                    // the last product's LDS is free
+    sa.load(a0, left);
+    sb.load(b0, left);
+    drain_and_meet();
+    sa.load(a1, left - BK);
+    sb.load(b1, left - BK);
+    read(a0, b0, 0);
+#pragma unroll 1
+    do {
+        step(a0, b0, a1, b1);
+        step(a1, b1, a0, b0);
+    } while (left > 0);
 }
 
 template <typename T, int B>
@@ -184,7 +217,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
     typedef Shape<B> S;
     int64_t token_tile, split;
     pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, splits, token_tile, split);
-    __shared__ __attribute__((aligned(16))) TileLds<T, true, true, B> lds;
+    TILE_LDS(T, true, true, B);
     const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
     const T* bias = (const T*)p.bias;
     const int64_t n0 = token_tile * B;
@@ -203,7 +236,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
 #pragma unroll 1
     for (int64_t m0 = first; m0 < end; m0 += B) {
         Acc<B> acc = {};
-        tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, lds);
+        tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
         if (bias)
 #pragma unroll
             for (int i = 0; i < S::MB; ++i)
@@ -244,7 +277,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
         }
     }
     __syncthreads();
-    Running* sh = reinterpret_cast<Running*>(&lds);              // [2 waves along the vocabulary][B tokens]
+    Running* sh = reinterpret_cast<Running*>(lds_a0);              // [2 waves along the vocabulary][B tokens]
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
         const Running o{__shfl_xor(run[j].m, 32, 64), __shfl_xor(run[j].s, 32, 64)};
@@ -416,13 +449,13 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
     typedef Shape<B> S;
     int64_t token_tile, panel;
     pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, ldg / B, token_tile, panel);
-    __shared__ __attribute__((aligned(16))) TileLds<T, true, true, B> lds;
+    TILE_LDS(T, true, true, B);
     const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
     const T* bias = (const T*)p.bias;
     const int64_t n0 = token_tile * B, m0 = v0 + panel * B;
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     Acc<B> acc = {};
-    tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, lds);
+    tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
     if (bias)
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
@@ -466,7 +499,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
                                                                        float* __restrict__ part)
 {
     typedef Shape<B> S;
-    __shared__ __attribute__((aligned(16))) TileLds<T, AKC, BKC, B> lds;
+    TILE_LDS(T, AKC, BKC, B);
     const int64_t worker = place_of(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     const int64_t end = (worker + 1) * share < units ? (worker + 1) * share : units;
@@ -476,7 +509,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
         const int64_t k0 = step * TB, k1 = (step + n) * TB < K ? (step + n) * TB : K;
         u += n;
         Acc<B> acc = {};
-        tile_product<T, AKC, BKC, B>(acc, A, Bm, tile / tiles_n * B, tile % tiles_n * B, k0, k1, lds);
+        tile_product<T, AKC, BKC, B>(acc, A, Bm, tile / tiles_n * B, tile % tiles_n * B, k0, k1, TILE_LDS_ARGS);
         float* out = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
@@ -587,8 +620,11 @@ struct Args {
 };
 
 // Rows as the kernels read them: as they are, or copied with their width filled up, where a row does not start on 16 bytes or its
-// width is no whole number of 16-byte groups.
-bool must_pack(const void* p, int64_t ld, int64_t D, int size) { return (uintptr_t)p % 16 || ld * size % 16 || D * size % 16; }
+// width is no whole number of 16-byte groups (or a row lies 4 MB from the next: 256 rows are reached with 32-bit offsets).
+bool must_pack(const void* p, int64_t ld, int64_t D, int size)
+{
+    return (uintptr_t)p % 16 || ld * size % 16 || D * size % 16 || ld * size >= (int64_t)1 << 22;
+}
 
 struct ForwardPlan {
     int64_t splits, tiles_per_split;
