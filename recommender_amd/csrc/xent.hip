@@ -466,37 +466,53 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
 #pragma unroll
                 for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
             }
+    // through LDS, so that a row's values leave 16 bytes a lane: a wave's 64 rows (tokens) of WM values, chunks changing places by the row
+    drain_and_meet();
+    constexpr int ROW = S::WM, CH = ROW * (int)sizeof(T) / 16, VEC = Traits<T>::VEC, PER_ARRAY = Stage<T, true, B>::SIZE / (S::WN * ROW);
+    const int wave = threadIdx.x >> 6;
+    const int array = wave / PER_ARRAY;
+    T* const mine = (array == 0 ? lds_a0 : array == 1 ? lds_a1 : array == 2 ? lds_b0 : lds_b1) + wave % PER_ARRAY * (S::WN * ROW);
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
-        const int64_t t = n0 + wn + 32 * j + (lane & 31);
-        if (t >= p.T) continue;
-        const int64_t y0 = p.target[t];
+        const int row = 32 * j + (lane & 31);
+        const int64_t t = n0 + wn + row;
+        const int64_t y0 = t < p.T ? p.target[t] : p.ignore;
         const bool in = y0 != p.ignore;
-        const int64_t y = clamp_target(y0, p.V);
-        const float l = lse[t], q = rest[t], g = (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE;
+        const int64_t y = in ? clamp_target(y0, p.V) : -1;
+        const float l = in ? lse[t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE : 0.f;
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
-                const int64_t v = m0 + wm + 32 * i + 8 * r4 + 4 * half;
-                if (v - v0 >= ldg) continue;
+                const int c = 32 * i + 8 * r4 + 4 * half;
                 Pack<T, 4> o;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const float e = v + u == y ? -q : __builtin_amdgcn_exp2f((acc[i][j][4 * r4 + u] - l) * LOG2E);
-                    o.v[u] = (T)(in && v + u < p.V ? e * g : 0.f);
+                    const int64_t v = m0 + wm + c + u;
+                    const float e = v == y ? -q : __builtin_amdgcn_exp2f((acc[i][j][4 * r4 + u] - l) * LOG2E);
+                    o.v[u] = (T)(in && v < p.V ? e * g : 0.f);
                 }
-                *reinterpret_cast<Pack<T, 4>*>(G + t * ldg + (v - v0)) = o;
+                *reinterpret_cast<Pack<T, 4>*>(mine + row * ROW + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC) = o;
             }
+    }
+    drain_and_meet();
+    for (int at = lane; at < S::WN * CH; at += 64) {
+        const int row = at / CH, c = at % CH;
+        const int64_t t = n0 + wn + row;
+        if (t < p.T)
+            *reinterpret_cast<Pack<T, VEC>*>(G + t * ldg + (m0 - v0 + wm) + c * VEC) =
+                *reinterpret_cast<const Pack<T, VEC>*>(mine + row * ROW + (c ^ (row & (CH - 1))) * VEC);
     }
 }
 
 // A B in equal shares: the units are (tile, step of TB in k), the steps of a tile together, tiles of one row of tiles beside each other;
 // every workgroup takes `share` consecutive units and writes the sums of each tile it touches, in 32 bits, to a place of its own: place
-// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.
+// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.  With `out` [M, N] a tile that lies in one share is finished
+// here: times scale / G_SCALE, rounded to T.
 template <typename T, bool AKC, bool BKC, int B>
-__global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T> A, Operand<T> Bm, int64_t tiles_n, int64_t K, int64_t steps, int64_t units, int64_t share,
-                                                                       float* __restrict__ part)
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T> A, Operand<T> Bm, int64_t tiles_n, int64_t M, int64_t N, int64_t K, int64_t steps,
+                                                                       int64_t units, int64_t share, const float* __restrict__ scale, float* __restrict__ part,
+                                                                       T* __restrict__ out)
 {
     typedef Shape<B> S;
     TILE_LDS(T, AKC, BKC, B);
@@ -509,24 +525,41 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
         const int64_t k0 = step * TB, k1 = (step + n) * TB < K ? (step + n) * TB : K;
         u += n;
         Acc<B> acc = {};
-        tile_product<T, AKC, BKC, B>(acc, A, Bm, tile / tiles_n * B, tile % tiles_n * B, k0, k1, TILE_LDS_ARGS);
-        float* out = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
+        const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
+        tile_product<T, AKC, BKC, B>(acc, A, Bm, m0, n0, k0, k1, TILE_LDS_ARGS);
+        if (out && n == steps) {
+            const float f = *scale / Traits<T>::G_SCALE;
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j) {
+                const int64_t c = n0 + wn + 32 * j + (lane & 31);
+#pragma unroll
+                for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t m = m0 + wm + 32 * i + acc_row(r, half);
+                        if (m < M && c < N) out[m * N + c] = (T)(acc[i][j][r] * f);
+                    }
+            }
+            continue;
+        }
+        float* to = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
 #pragma unroll
             for (int j = 0; j < S::NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) out[(wm + 32 * i + acc_row(r, half)) * B + wn + 32 * j + (lane & 31)] = acc[i][j][r];
+                for (int r = 0; r < 16; ++r) to[(wm + 32 * i + acc_row(r, half)) * B + wn + 32 * j + (lane & 31)] = acc[i][j][r];
     }
 }
 
-// The places of every tile added; with `sum` [M, N] added to (first: written to) it, or with `out` its total (and sum's, if !first)
+// The places of every tile added (direct: of those in several shares); with `sum` [M, N] added to (first: written to) it, or with `out` its total (and sum's, if !first)
 // times scale / G_SCALE rounded to T
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int B, int64_t tiles_n, int64_t steps, int64_t share, int64_t M, int64_t N,
-                                                   const float* __restrict__ scale, int first, float* __restrict__ sum, T* __restrict__ out)
+                                                   const float* __restrict__ scale, int first, int direct, float* __restrict__ sum, T* __restrict__ out)
 {
     const int64_t tile = blockIdx.x, a = tile * steps / share, b = ((tile + 1) * steps - 1) / share;
+    if (direct && a == b) return;
     const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
     const float f = out ? *scale / Traits<T>::G_SCALE : 1.f;
     for (int i = (blockIdx.y * 256 + threadIdx.x) * 4; i < B * B; i += gridDim.y * 1024) {
@@ -545,28 +578,36 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     }
 }
 
-// out[i] = scale / G_SCALE * sum over slices, rounded to T
+// out[i] = scale / G_SCALE * sum over slices, `ld` values apart, rounded to T
 template <typename T>
-__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int slices, int64_t n, const float* __restrict__ scale, T* __restrict__ out)
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ part, int slices, int64_t ld, int64_t n, const float* __restrict__ scale, T* __restrict__ out)
 {
     const float f = *scale / Traits<T>::G_SCALE;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float s = 0.f;
-        for (int k = 0; k < slices; ++k) s += part[k * n + i];
+#pragma unroll 8
+        for (int k = 0; k < slices; ++k) s += part[k * ld + i];
         out[i] = (T)(s * f);
     }
 }
 
-// column sums of G, [slices][width] in 32 bits: slice blockIdx.y takes rows [y * rows_per, ...)
+// column sums of G, [slices][ldg] in 32 bits: slice blockIdx.y takes rows [y * rows_per, ...); 16 bytes of a row per thread
 template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ G, int64_t ldg, int64_t T_rows, int64_t rows_per, int64_t width, float* __restrict__ out)
+__global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ G, int64_t ldg, int64_t T_rows, int64_t rows_per, float* __restrict__ out)
 {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    constexpr int VEC = Traits<T>::VEC;
+    const int64_t v = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
     const int64_t t0 = blockIdx.y * rows_per, t1 = t0 + rows_per < T_rows ? t0 + rows_per : T_rows;
-    if (v >= width) return;
-    float s = 0.f;
-    for (int64_t t = t0; t < t1; ++t) s += (float)G[t * ldg + v];
-    out[blockIdx.y * width + v] = s;
+    if (v >= ldg) return;
+    float s[VEC] = {};
+#pragma unroll 8
+    for (int64_t t = t0; t < t1; ++t) {
+        const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC>*>(G + t * ldg + v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += (float)g.v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[blockIdx.y * ldg + v + i] = s[i];
 }
 
 // rows with their width filled up to `ldo` with zeros; rows whose target (nullable) is `ignore` as zeros
@@ -687,7 +728,7 @@ BackwardPlan backward_plan(int64_t T, int64_t V, int64_t D, int size)
     BackwardPlan b;
     const int64_t tiles = ceil_div64(V, 256), by_g = (int64_t)(PIECE_BYTES / ((size_t)T * size)) / 256;
     b.width = clamp64(by_g, 1, tiles < 16384 ? tiles : 16384) * 256;
-    b.b_slices = clamp64(512 / ceil_div64(b.width, 256), 1, ceil_div64(T, TB));
+    b.b_slices = clamp64(512 / ceil_div64(b.width, 256 * (16 / size)), 1, ceil_div64(T, 32) < 64 ? ceil_div64(T, 32) : 64);
     b.b_per = ceil_div64(T, b.b_slices);
     b.b_slices = ceil_div64(T, b.b_per);
     return b;
@@ -729,9 +770,12 @@ int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t 
     const ProductPlan q = product_plan(sizeof(T), M, N, K);
     return with_tile<T>(q.tile, [&](auto t) -> int {
         constexpr int W = decltype(t)::value;
-        hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W>), dim3((unsigned)q.workers), dim3(Shape<W>::THREADS), 0, s, A, B, q.tiles_n, K, q.steps, q.units, q.share, part);
-        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / 4096)), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
-                           scale, first, sum, out);
+        const bool direct = out && !sum;
+        hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W>), dim3((unsigned)q.workers), dim3(Shape<W>::THREADS), 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share,
+                           scale, part, direct ? out : nullptr);
+        if (!direct || q.share % q.steps)
+            hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / 4096)), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
+                           scale, first, direct, sum, out);
         RECO_CHECK_LAUNCH();
         return RECO_OK;
     });
@@ -846,9 +890,9 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
         if (!rl && dw) rl = launch_product<T, false, false>({G, ldg, ldg}, {(const T*)p.x, p.ldx, p.D}, width, a.D, a.T, scale, true, w_part, nullptr, (T*)dw + v0 * a.D, s);
         if (rl) return rl;
         if (db) {
-            hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(width, 256), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per, width,
+            hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(ldg, 256 * Traits<T>::VEC), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per,
                                b_part);
-            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, width, scale, (T*)db + v0);
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, ldg, width, scale, (T*)db + v0);
         }
         RECO_CHECK_LAUNCH();
     }
