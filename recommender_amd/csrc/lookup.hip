@@ -9,8 +9,7 @@
 // 32 bits in an order that depends on the sizes alone: no atomic adds, the same bits on every run.  Ids of `padding` sort behind
 // all others and are never read.
 //   sort     least-significant-digit radix sort, stable; up to SMALL_SORT ids in the LDS of one workgroup, else tile by tile
-//            (count, scan, scatter per digit).  The first launch also writes the zeros of the whole gradient from the workgroups
-//            that have nothing to sort.
+//            (count, scan, scatter per digit).  Workgroups beside the sorting ones write the zeros of the whole gradient meanwhile.
 //   sum      the sorted list is cut into chunks of equal length, whatever the ids are, so that a very frequent id is shared out
 //            as evenly as the rest: a run that lies in one chunk is finished there, one that crosses chunks leaves 32-bit partial
 //            rows, and join_kernel adds those in chunk order.
@@ -22,8 +21,7 @@ namespace {
 
 constexpr int RADIX_BITS = 11;
 constexpr int BINS = 1 << RADIX_BITS;
-constexpr int TILE = 4096;              // ids per workgroup and pass
-constexpr int SORT_THREADS = 256;       // 4 waves, 16 ids per lane
+constexpr int SORT_THREADS = 256;
 constexpr int SMALL_SORT = 4096;        // ids that one workgroup sorts by itself
 constexpr int SMALL_THREADS = 1024;
 
@@ -70,6 +68,7 @@ struct SortPass {
     int64_t n;
     int64_t rows, padding;
     int shift, bits, tiles;
+    int per_tile;            // ids per workgroup and pass: a multiple of SORT_THREADS, at most 16 of them per thread
 };
 
 __device__ __forceinline__ uint32_t id_key(int64_t id, int64_t rows, int64_t padding)
@@ -96,21 +95,27 @@ __device__ __forceinline__ void zero_fill(const Fill& f, int64_t first, int64_t 
     if (first < f.words) reinterpret_cast<uint16_t*>(f.p + f.packs)[first] = 0;
 }
 
-// tile's digit counts; workgroups behind the tiles write zeros (the gradient, 16 bytes at a time) meanwhile
+// The sort leaves most of the memory's time unused: each of its launches has workgroups behind its own `work` ones that write a part of
+// the gradient's zeros (16 bytes at a time).  All three kernels have 256 threads.
+__device__ __forceinline__ bool fills(const Fill& fill, int work)
+{
+    if ((int)blockIdx.x < work) return false;
+    zero_fill(fill, (int64_t)(blockIdx.x - work) * 256 + threadIdx.x, (int64_t)(gridDim.x - work) * 256);
+    return true;
+}
+
+// a tile's digit counts
 __global__ __launch_bounds__(SORT_THREADS) void count_kernel(SortPass a, Fill fill)
 {
     __shared__ uint32_t bin[BINS];
-    if ((int)blockIdx.x >= a.tiles) {
-        zero_fill(fill, (int64_t)(blockIdx.x - a.tiles) * SORT_THREADS + threadIdx.x, (int64_t)(gridDim.x - a.tiles) * SORT_THREADS);
-        return;
-    }
+    if (fills(fill, a.tiles)) return;
     const int bins = 1 << a.bits;
     for (int b = threadIdx.x; b < bins; b += SORT_THREADS) bin[b] = 0;
     __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * TILE;
+    const int64_t t0 = (int64_t)blockIdx.x * a.per_tile;
 #pragma unroll 4
-    for (int i = 0; i < TILE / SORT_THREADS; ++i) {
-        const int64_t t = t0 + i * SORT_THREADS + threadIdx.x;
+    for (int i = 0; i < a.per_tile; i += SORT_THREADS) {
+        const int64_t t = t0 + i + threadIdx.x;
         if (t < a.n) atomicAdd(&bin[(load_key(a, t) >> a.shift) & (bins - 1)], 1u);
     }
     __syncthreads();
@@ -128,8 +133,9 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v, int lane)
 }
 
 // one wave per digit: how many of its ids lie in earlier tiles
-__global__ __launch_bounds__(256) void scan_kernel(SortPass a)
+__global__ __launch_bounds__(256) void scan_kernel(SortPass a, Fill fill)
 {
+    if (fills(fill, ((1 << a.bits) + 3) / 4)) return;
     const int b = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (b >= (1 << a.bits)) return;
     uint32_t* row = a.counts + (int64_t)b * a.tiles;
@@ -202,12 +208,14 @@ __device__ __forceinline__ uint32_t place_of(uint32_t* at, uint32_t digit, int b
     return base + rank;
 }
 
-__global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(SortPass a)
+template <int STEPS>
+__global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(SortPass a, Fill fill)
 {
-    constexpr int WAVES = SORT_THREADS / 64, STEPS = TILE / SORT_THREADS;
+    constexpr int WAVES = SORT_THREADS / 64;
     __shared__ uint32_t first[BINS];
     __shared__ uint32_t at[WAVES][BINS];
     __shared__ uint32_t scratch[WAVES];
+    if (fills(fill, a.tiles)) return;
     const int bins = 1 << a.bits, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int b = tid; b < bins; b += SORT_THREADS) {
         first[b] = a.totals[b];
@@ -216,7 +224,7 @@ __global__ __launch_bounds__(SORT_THREADS) void scatter_kernel(SortPass a)
     }
     __syncthreads();
     block_exclusive<SORT_THREADS>(first, bins, scratch);
-    const int64_t t0 = (int64_t)blockIdx.x * TILE + wave * (STEPS * 64);
+    const int64_t t0 = (int64_t)blockIdx.x * a.per_tile + wave * (STEPS * 64);
     uint32_t key[STEPS], pos[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
@@ -374,17 +382,27 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a, const T* __restrict
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     float* part = a.part + c * 2 * (int64_t)a.dim + col * N;
-    for (int64_t i = i0; i < i1; i += AHEAD) {
-        uint32_t key[AHEAD];
-        P v[AHEAD];
+    // places are read one batch before their rows
+    uint32_t key[AHEAD], next_key[AHEAD], next_pos[AHEAD];
+    auto places = [&](int64_t i) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int64_t at = i + u < i1 ? i + u : i1 - 1;
-            key[u] = i + u < i1 ? a.key[at] : last;
+            next_key[u] = i + u < i1 ? a.key[at] : last;
+            next_pos[u] = a.pos[at];
+        }
+    };
+    places(i0);
+    for (int64_t i = i0; i < i1; i += AHEAD) {
+        P v[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            key[u] = next_key[u];
             // behind the chunk and for padding: row 0 of the gradient is read and not used
-            const int64_t p = key[u] < last ? a.pos[at] : 0;
+            const int64_t p = key[u] < last ? next_pos[u] : 0;
             v[u] = *reinterpret_cast<const P*>(grad + p * a.ldg + col * N);
         }
+        if (i + AHEAD < i1) places(i + AHEAD);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (i + u < i1 && cur < last) {
@@ -419,39 +437,47 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a, const T* __restrict
 }
 
 // A run that starts in chunk c and goes on: its partial rows are [c][1], then [c + 1][0] .. [e][0] with e the chunk it ends in.
-// One workgroup looks at JOIN consecutive chunks; the groups of lanes take the partial rows in turn and their sums are added in
+// One workgroup looks at `per` consecutive chunks (at most 8); the groups of lanes take the partial rows in turn and their sums are added in
 // group order.
-constexpr int JOIN = 8;
 template <typename T, int N>
-__global__ __launch_bounds__(256) void join_kernel(SumArgs a, T* __restrict__ out, int lanes_sh)
+__global__ __launch_bounds__(256) void join_kernel(SumArgs a, int per, T* __restrict__ out, int lanes_sh)
 {
-    __shared__ int64_t ends[JOIN];
+    __shared__ int goes_on[8];
+    __shared__ int window_end;
     __shared__ float sums[256 * N];
     const int lanes = 1 << lanes_sh, groups = 256 >> lanes_sh;
     const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_sh;
     const int col = blockIdx.y * lanes + lane;
-    if (threadIdx.x < JOIN) {
-        const int64_t c = (int64_t)blockIdx.x * JOIN + threadIdx.x;
-        int64_t end = -1;
+    if ((int)threadIdx.x < per) {
+        const int64_t c = (int64_t)blockIdx.x * per + threadIdx.x;
+        bool run = false;
         if (c + 1 < a.chunks) {
             const int64_t i0 = c * a.chunk, i1 = i0 + a.chunk;
             const uint32_t k = a.key[i1 - 1];
-            const bool starts_here = i0 == 0 || a.key[i0 - 1] != k;
-            if (k < (uint32_t)a.rows && a.key[i1] == k && starts_here) {
-                int64_t lo = i1, hi = a.n;                       // the first place behind the run
-                while (lo < hi) {
-                    const int64_t mid = (lo + hi) >> 1;
-                    if (a.key[mid] > k) hi = mid; else lo = mid + 1;
-                }
-                end = (lo - 1) / a.chunk;
-            }
+            run = k < (uint32_t)a.rows && a.key[i1] == k && (i0 == 0 || a.key[i0 - 1] != k);
         }
-        ends[threadIdx.x] = end;
+        goes_on[threadIdx.x] = run;
     }
     __syncthreads();
-    for (int j = 0; j < JOIN; ++j) {
-        const int64_t c = (int64_t)blockIdx.x * JOIN + j, e = ends[j];
-        if (e < 0) continue;                                     // the same for the whole workgroup
+    for (int j = 0; j < per; ++j) {
+        if (!goes_on[j]) continue;                               // the same for the whole workgroup
+        const int64_t c = (int64_t)blockIdx.x * per + j;
+        // the last chunk that begins with the run's key, looked for 256 chunks at a time
+        const uint32_t k = a.key[(c + 1) * a.chunk];
+        int64_t e = c + 1;
+        for (;;) {
+            const int64_t at = e + 1 + threadIdx.x;
+            const bool out = at >= a.chunks || a.key[at * a.chunk] != k;
+            const unsigned long long outs = __ballot(out);
+            if (threadIdx.x == 0) window_end = 256;
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0 && outs) atomicMin(&window_end, (int)(threadIdx.x + __ffsll(outs) - 1));
+            __syncthreads();
+            const int more = window_end;
+            __syncthreads();
+            e += more;
+            if (more < 256) break;
+        }
         float acc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
@@ -470,7 +496,7 @@ __global__ __launch_bounds__(256) void join_kernel(SumArgs a, T* __restrict__ ou
             for (int g = 1; g < groups; ++g)
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i] += sums[(g * lanes + lane) * N + i];
-            store_row<T, N>(out + a.key[(c + 1) * a.chunk] * (int64_t)a.dim + col * N, acc, a.scale);
+            store_row<T, N>(out + k * (int64_t)a.dim + col * N, acc, a.scale);
         }
         __syncthreads();
     }
@@ -512,7 +538,7 @@ int bit_length(int64_t v)
 }
 
 struct GradPlan {
-    int tiles, passes, bits, chunk;
+    int per_tile, tiles, passes, bits, chunk, join;
     int64_t chunks;
     size_t keys, poss, counts, totals, part, total;
 };
@@ -523,9 +549,11 @@ GradPlan grad_plan(int64_t n, int64_t rows, int dim)
     const int need = bit_length(rows);                 // keys 0 .. rows, the last one being padding
     p.passes = (need + RADIX_BITS - 1) / RADIX_BITS;
     p.bits = (need + p.passes - 1) / p.passes;
-    p.tiles = (int)ceil_div64(n, TILE);
-    p.chunk = n <= 16384 ? 8 : n <= (1 << 18) ? 32 : n <= (1 << 20) ? 64 : 128;
+    p.per_tile = n <= (1 << 20) ? 1024 : 4096;
+    p.tiles = (int)ceil_div64(n, p.per_tile);
+    p.chunk = n <= 16384 ? 8 : n <= (1 << 17) ? 16 : n <= (1 << 20) ? 32 : 64;
     p.chunks = ceil_div64(n, p.chunk);
+    p.join = p.chunks <= 4096 ? 1 : 4;
     const bool small = n <= SMALL_SORT;
     const size_t copies = small ? 1 : 2;
     const size_t list = align_up((size_t)n * 4, 256);
@@ -589,7 +617,7 @@ extern "C" int reco_embedding_grad(const int64_t* ids, int64_t n, const void* gr
         return RECO_ENOMEM;
     }
     SortPass a{};
-    a.ids = ids; a.n = n; a.rows = rows; a.padding = padding; a.bits = p.bits; a.tiles = p.tiles;
+    a.ids = ids; a.n = n; a.rows = rows; a.padding = padding; a.bits = p.bits; a.tiles = p.tiles; a.per_tile = p.per_tile;
     char* w = (char*)ws;
     const uint32_t *key = nullptr, *pos = nullptr;
     if (n <= SMALL_SORT) {
@@ -604,17 +632,34 @@ extern "C" int reco_embedding_grad(const int64_t* ids, int64_t n, const void* gr
         pos = a.pos_out;
     } else {
         const size_t list = align_up((size_t)n * 4, 256);
-        const int64_t blocks = fill_want < 2048 ? fill_want : 2048;
         a.counts = (uint32_t*)(w + p.counts);
         a.totals = (uint32_t*)(w + p.totals);
+        // the zeros in proportion to the time that the launches take (10 : 6 : 14 measured at 524,289 ids, 10-bit digits); the last one
+        // takes the rest
+        int64_t filled = 0;
+        int share = 0;
+        auto part = [&](int weight, int64_t* blocks) {
+            share += weight;
+            const int64_t to = share == 30 * p.passes ? fill.packs : fill.packs * share / (30 * p.passes);
+            const Fill f{fill.p + filled, to - filled, share == 30 * p.passes ? fill.words : 0};
+            filled = to;
+            const int64_t want = ceil_div64(f.packs, 4 * 256);
+            *blocks = want < 1 ? (f.words ? 1 : 0) : want < 1024 ? want : 1024;
+            return f;
+        };
         for (int pass = 0; pass < p.passes; ++pass) {
             a.shift = pass * p.bits;
             a.key_out = (uint32_t*)(w + p.keys + (pass & 1) * list);
             a.pos_out = (uint32_t*)(w + p.poss + (pass & 1) * list);
             ProfScope prof(s, RECO_PROF_EMBEDDING);
-            hipLaunchKernelGGL(count_kernel, dim3((unsigned)(p.tiles + (pass ? 0 : blocks))), dim3(SORT_THREADS), 0, s, a, pass ? Fill{} : fill);
-            hipLaunchKernelGGL(scan_kernel, dim3((unsigned)ceil_div64(1 << p.bits, 4)), dim3(256), 0, s, a);
-            hipLaunchKernelGGL(scatter_kernel, dim3((unsigned)p.tiles), dim3(SORT_THREADS), 0, s, a);
+            int64_t extra;
+            Fill f = part(10, &extra);
+            hipLaunchKernelGGL(count_kernel, dim3((unsigned)(p.tiles + extra)), dim3(SORT_THREADS), 0, s, a, f);
+            f = part(6, &extra);
+            hipLaunchKernelGGL(scan_kernel, dim3((unsigned)(ceil_div64(1 << p.bits, 4) + extra)), dim3(256), 0, s, a, f);
+            f = part(14, &extra);
+            if (p.per_tile == 1024) hipLaunchKernelGGL(scatter_kernel<4>, dim3((unsigned)(p.tiles + extra)), dim3(SORT_THREADS), 0, s, a, f);
+            else hipLaunchKernelGGL(scatter_kernel<16>, dim3((unsigned)(p.tiles + extra)), dim3(SORT_THREADS), 0, s, a, f);
             RECO_CHECK_LAUNCH();
             a.ids = nullptr;
             a.key_in = a.key_out;
@@ -633,7 +678,7 @@ extern "C" int reco_embedding_grad(const int64_t* ids, int64_t n, const void* gr
             const unsigned cols = (unsigned)ceil_div64(b.packs, 1 << sh);
             ProfScope prof(s, RECO_PROF_EMBEDDING);
             hipLaunchKernelGGL((sum_kernel<T, N>), dim3((unsigned)ceil_div64(p.chunks, 256 >> sh), cols), dim3(256), 0, s, b, (const T*)grad, (T*)out, sh);
-            hipLaunchKernelGGL((join_kernel<T, N>), dim3((unsigned)ceil_div64(p.chunks, JOIN), cols), dim3(256), 0, s, b, (T*)out, sh);
+            hipLaunchKernelGGL((join_kernel<T, N>), dim3((unsigned)ceil_div64(p.chunks, p.join), cols), dim3(256), 0, s, b, p.join, (T*)out, sh);
             RECO_CHECK_LAUNCH();
             return RECO_OK;
         });
