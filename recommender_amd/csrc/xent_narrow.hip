@@ -402,6 +402,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     __shared__ __attribute__((aligned(16))) char tiles[3][Streamed::BYTES];
     __shared__ __attribute__((aligned(16))) float expos[3][SB];
     __shared__ __attribute__((aligned(16))) float gns[EACH ? 3 : 1][SB];
+    __shared__ __attribute__((aligned(16))) float minus_q[3][SB];
     __shared__ __attribute__((aligned(16))) int ys[4][SB];
     const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     char* const ring = &tiles[0][0];
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     for (int d = 0; d < W::BLOCKS; ++d) o[d] = f32x16{};
 
     Streamed st;
-    float expo_reg = 0.f, gn_reg = 0.f;
+    float expo_reg = 0.f, gn_reg = 0.f, q_reg = 0.f;
     int y_reg = -1;
     auto fetch = [&](int tile) {
         const int64_t t0 = first + (int64_t)tile * SB;
@@ -435,6 +436,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
             const int64_t t = t0 + threadIdx.x;
             expo_reg = t < end ? expo[t] : BIAS ? INFINITY : -INFINITY;
             y_reg = t + SB < end ? y[t + SB] : -1;
+            q_reg = t < end ? rest[t] : 0.f;
             if (EACH) gn_reg = t < end ? gn[t] : 0.f;
         }
     };
@@ -444,6 +446,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
         st.store(tiles[at], ys[tile & 3]);
         if (threadIdx.x < SB) {
             expos[at][threadIdx.x] = expo_reg;
+            minus_q[at][threadIdx.x] = -Traits<T>::G_SCALE * (EACH ? q_reg * gn_reg : q_reg);
             ys[(tile + 1) & 3][threadIdx.x] = y_reg;
             if (EACH) gns[at][threadIdx.x] = gn_reg;
         }
@@ -493,15 +496,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
                     s[r] = EACH ? e * g4[r % 4] : e;
                 },
                 [&] {
-                    // a target of these 32 rows that lies in this wave's part of the vocabulary
+                    // A target of these 32 rows that lies in this wave's part of the vocabulary.  Without memory loads or branches per
+                    // value: with a popular item among its 32, a wave comes here for most blocks.
                     if (__any((unsigned)(mine - (int)h0) < 32u))
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int row = acc_row(r, half);
-                            if (y32[row] == (int)v) {
-                                const float q = rest[first + 32 * (int64_t)i + row] * Traits<T>::G_SCALE;
-                                s[r] = EACH ? -q * gns[0][at * 32 + row] : -q;
-                            }
+                        for (int q = 0; q < 4; ++q) {
+                            const i32x4 y4 = *reinterpret_cast<const i32x4*>(y32 + 8 * q + 4 * half);
+                            const f32x4 q4 = *reinterpret_cast<const f32x4*>(&minus_q[0][0] + at * 32 + 8 * q + 4 * half);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[4 * q + j] = y4[j] == (int)v ? q4[j] : s[4 * q + j];
                         }
                 },
                 [&](int k, int n) {
