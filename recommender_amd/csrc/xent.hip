@@ -791,7 +791,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
     const int tile = tile_of(sizeof(T), a.T, a.V);
     const ForwardPlan f = forward_plan(a.T, a.V, tile);
-    const NarrowPlan n = narrow ? narrow_plan(a.dtype, a.T, a.V, a.D) : NarrowPlan{};
+    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
     const int64_t splits = narrow ? n.x_splits : f.splits;
     Running* part = (Running*)c.take((size_t)splits * a.T * sizeof(Running));
     float* z_target = (float*)c.take((size_t)a.T * 4);
@@ -804,7 +804,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     if (!launch) return RECO_OK;
     if (reduction == REDUCE_NONE) rows = loss;
     if (narrow) {
-        const int rn = narrow_rows(a.dtype, p, n, a.D, part, z_target, dx_part, s);
+        const int rn = narrow_rows_of<T>(p, n, a.D, part, z_target, dx_part, s);
         if (rn) return rn;
     } else {
         const int rs = with_tile<T>(tile, [&](auto t) -> int {
@@ -839,7 +839,7 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
     float* tops = (float*)c.take(256 * 4);
     int* y = (int*)c.take((size_t)a.T * 4);
     float* expo = (float*)c.take((size_t)a.T * 4);
-    const NarrowPlan n = narrow ? narrow_plan(a.dtype, a.T, a.V, a.D) : NarrowPlan{};
+    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
     const BackwardPlan b = narrow ? BackwardPlan{} : backward_plan(a.T, a.V, a.D, sizeof(T));
     T* G = nullptr;
     float *x_part = nullptr, *w_part = nullptr, *b_part = nullptr;
@@ -869,7 +869,7 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
                        log2f(Traits<T>::G_SCALE), gn, scale, y, expo);
     if (narrow) {
         if (dw || db) {
-            const int rn = narrow_cols(a.dtype, p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
+            const int rn = narrow_cols_of<T>(p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
             if (rn) return rn;
         }
         if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, dx_unit, a.T, a.D, gn, scale, (T*)dx);

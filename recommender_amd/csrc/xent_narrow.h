@@ -12,6 +12,7 @@
 //       grows by more than LAG (a power of e): then O and the sum are rescaled, which is rare after the first blocks.
 // cols: held W, streamed x with the finished lse: O is dW, the sum of e over the streamed rows is dbias.
 // A launch splits the streamed rows where there are few held ones; the parts are joined in order of the splits.
+#pragma once
 #include "xent_shared.h"
 
 namespace {
@@ -583,91 +584,98 @@ template <typename T, typename F> int with_width(int64_t D, F&& fn)
 
 template <typename F> int with_flag(bool v, F&& fn) { return v ? fn(std::true_type()) : fn(std::false_type()); }
 
+constexpr int64_t HELD = 128;                  // held rows per workgroup: 4 waves of 32
+
+template <typename T, typename F> int shape_of(int64_t D, F&& fn)
+{
+    return with_width<T>(D, [&](auto dp) -> int {
+        constexpr int DP = decltype(dp)::value;
+        return fn(dp, (int64_t)stream_rows<T, DP>(), 256 * waves_per_simd<T, DP>());
+    });
+}
+
+// Splits of the streamed rows, whole tiles each: the fewest microseconds out of rounds of workgroups (at the rate that the kernels reach,
+// 0.8 PFLOP/s in 16 bits and 0.12 in 32, and 4 us to begin and end one) and of the parts of dx, written and read at 4 TB/s
+inline void split_plan(int64_t T, int64_t D, int64_t groups, int64_t streamed, int64_t tile, int64_t places, double rate, int64_t* splits, int64_t* per)
+{
+    const int64_t tiles = ceil_div64(streamed, tile);
+    const double tile_us = 4.0 * tile * HELD * D * places / rate * 1e6;
+    double best = 1e30;
+    int64_t most = 4 * places / groups + 1;
+    if (most > tiles) most = tiles;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t run = ceil_div64(tiles, s), n = ceil_div64(tiles, run);
+        const double us = ceil_div64(groups * n, places) * (run * tile_us + 4.0) + n * T * D * 8.0 / 4e12 * 1e6;
+        if (us < best) {
+            best = us;
+            *splits = n;
+            *per = run * tile;
+        }
+    }
+}
+
 }  // namespace
 
 namespace xent {
 
-static constexpr int64_t HELD = 128;           // held rows per workgroup: 4 waves of 32
-
-bool narrow_fits(int dtype, int64_t D) { return D <= (dtype == RECO_DT_F32 ? 128 : 256); }
-
-// Splits of the streamed rows: about two workgroups per compute unit, whole tiles each
-static void split_plan(int64_t held_groups, int64_t streamed, int64_t tile, int64_t* splits, int64_t* per)
-{
-    const int64_t tiles = ceil_div64(streamed, tile);
-    int64_t s = 512 / held_groups;
-    s = s < 1 ? 1 : s > tiles ? tiles : s;
-    *per = ceil_div64(tiles, s) * tile;
-    *splits = ceil_div64(streamed, *per);
-}
-
-template <typename T, typename F> static int shape_of(int64_t D, F&& fn)
-{
-    return with_width<T>(D, [&](auto dp) -> int {
-        constexpr int DP = decltype(dp)::value;
-        return fn(dp, (int64_t)stream_rows<T, DP>());
-    });
-}
-
-NarrowPlan narrow_plan(int dtype, int64_t T, int64_t V, int64_t D)
+template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D)
 {
     NarrowPlan n{};
-    (void)reco_with_type(dtype, [&](auto z) -> int {
-        return shape_of<decltype(z)>(D, [&](auto dp, int64_t tile) -> int {
-            n.x_groups = ceil_div64(T, HELD);
-            split_plan(n.x_groups, V, tile, &n.x_splits, &n.x_per);
-            n.w_groups = ceil_div64(V, HELD);
-            n.w_tiles = ceil_div64(T, tile);
-            const int64_t units = n.w_groups * n.w_tiles, places = 256 * waves_per_simd<decltype(z), decltype(dp)::value>();
-            // a share of less than four tiles is mostly beginning and end
-            n.w_share = ceil_div64(units, places);
-            if (n.w_share < 4) n.w_share = n.w_tiles < 4 ? n.w_tiles : 4;
-            n.w_shares = ceil_div64(units, n.w_share);
-            n.w_shared = n.w_share % n.w_tiles != 0;
-            return RECO_OK;
-        });
+    (void)shape_of<T>(D, [&](auto dp, int64_t tile, int64_t places) -> int {
+        n.x_groups = ceil_div64(T_rows, HELD);
+        split_plan(T_rows, decltype(dp)::value, n.x_groups, V, tile, places, sizeof(T) == 2 ? 0.8e15 : 0.12e15, &n.x_splits, &n.x_per);
+        n.w_groups = ceil_div64(V, HELD);
+        n.w_tiles = ceil_div64(T_rows, tile);
+        const int64_t units = n.w_groups * n.w_tiles;
+        // a share of less than four tiles is mostly beginning and end
+        n.w_share = ceil_div64(units, places);
+        if (n.w_share < 4) n.w_share = n.w_tiles < 4 ? n.w_tiles : 4;
+        n.w_shares = ceil_div64(units, n.w_share);
+        n.w_shared = n.w_share % n.w_tiles != 0;
+        return RECO_OK;
     });
     return n;
 }
 
-int narrow_rows(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_out, Running* part, float* z_target, float* dx_part, hipStream_t s)
+template <typename T> int narrow_rows_of(const Problem& p, const NarrowPlan& n, int64_t width_out, Running* part, float* z_target, float* dx_part, hipStream_t s)
 {
-    return reco_with_type(dtype, [&](auto z) -> int {
-        typedef decltype(z) T;
-        return shape_of<T>(p.D, [&](auto dp, int64_t) -> int {
-            return with_flag(p.bias != nullptr, [&](auto bias) -> int {
-                return with_flag(dx_part != nullptr, [&](auto dx) -> int {
-                    hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(dx)::value>),
-                                       dim3((unsigned)(n.x_groups * n.x_splits)), dim3(256), 0, s, p, (int)n.x_splits, n.x_per, (int)width_out, part, z_target,
-                                       dx_part);
-                    RECO_CHECK_LAUNCH();
-                    return RECO_OK;
-                });
+    return shape_of<T>(p.D, [&](auto dp, int64_t, int64_t) -> int {
+        return with_flag(p.bias != nullptr, [&](auto bias) -> int {
+            return with_flag(dx_part != nullptr, [&](auto dx) -> int {
+                hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(dx)::value>),
+                                   dim3((unsigned)(n.x_groups * n.x_splits)), dim3(256), 0, s, p, (int)n.x_splits, n.x_per, (int)width_out, part, z_target, dx_part);
+                RECO_CHECK_LAUNCH();
+                return RECO_OK;
             });
         });
     });
 }
 
-int narrow_cols(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_out, const float* expo, const int* y, const float* rest, const float* gn,
-                const float* scale, void* dw, void* db, float* dw_part, float* db_part, hipStream_t s)
+template <typename T>
+int narrow_cols_of(const Problem& p, const NarrowPlan& n, int64_t width_out, const float* expo, const int* y, const float* rest, const float* gn,
+                   const float* scale, void* dw, void* db, float* dw_part, float* db_part, hipStream_t s)
 {
-    return reco_with_type(dtype, [&](auto z) -> int {
-        typedef decltype(z) T;
-        return shape_of<T>(p.D, [&](auto dp, int64_t) -> int {
-            return with_flag(p.bias != nullptr, [&](auto bias) -> int {
-                return with_flag(gn != nullptr, [&](auto each) -> int {
-                    hipLaunchKernelGGL((narrow_cols_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(each)::value>), dim3((unsigned)n.w_shares),
-                                       dim3(256), 0, s, p, n.w_groups * n.w_tiles, n.w_share, (int)n.w_tiles, (int)width_out, expo, y, rest, gn, scale, (T*)dw,
-                                       (T*)db, dw_part, db_part);
-                    if (n.w_shared)
-                        hipLaunchKernelGGL(narrow_join_kernel<T>, dim3((unsigned)n.w_groups, (unsigned)ceil_div64(HELD * (width_out + 1), 1024)), dim3(256), 0, s, p.V,
-                                           n.w_share, (int)n.w_tiles, (int)width_out, scale, dw_part, db_part, (T*)dw, (T*)db);
-                    RECO_CHECK_LAUNCH();
-                    return RECO_OK;
-                });
+    return shape_of<T>(p.D, [&](auto dp, int64_t, int64_t) -> int {
+        return with_flag(p.bias != nullptr, [&](auto bias) -> int {
+            return with_flag(gn != nullptr, [&](auto each) -> int {
+                hipLaunchKernelGGL((narrow_cols_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(each)::value>), dim3((unsigned)n.w_shares), dim3(256),
+                                   0, s, p, n.w_groups * n.w_tiles, n.w_share, (int)n.w_tiles, (int)width_out, expo, y, rest, gn, scale, (T*)dw, (T*)db, dw_part,
+                                   db_part);
+                if (n.w_shared)
+                    hipLaunchKernelGGL(narrow_join_kernel<T>, dim3((unsigned)n.w_groups, (unsigned)ceil_div64(HELD * (width_out + 1), 1024)), dim3(256), 0, s, p.V,
+                                       n.w_share, (int)n.w_tiles, (int)width_out, scale, dw_part, db_part, (T*)dw, (T*)db);
+                RECO_CHECK_LAUNCH();
+                return RECO_OK;
             });
         });
     });
 }
 
 }  // namespace xent
+
+// One source file per element type instantiates these
+#define XENT_NARROW(T)                                                                                                                             \
+    template xent::NarrowPlan xent::narrow_plan_of<T>(int64_t, int64_t, int64_t);                                                                  \
+    template int xent::narrow_rows_of<T>(const xent::Problem&, const xent::NarrowPlan&, int64_t, xent::Running*, float*, float*, hipStream_t);      \
+    template int xent::narrow_cols_of<T>(const xent::Problem&, const xent::NarrowPlan&, int64_t, const float*, const int*, const float*,            \
+                                         const float*, const float*, void*, void*, float*, float*, hipStream_t)

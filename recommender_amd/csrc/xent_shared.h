@@ -63,16 +63,19 @@ __device__ __forceinline__ Running joined(Running a, Running b)
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
-// The form for narrow rows (xent_narrow.hip).  x: groups of held rows, times splits of `per` vocabulary rows.  w: groups of held
+// The form for narrow rows (xent_narrow.h).  x: groups of held rows, times splits of `per` vocabulary rows.  w: groups of held
 // vocabulary rows, times tiles of x rows, in shares of consecutive (group, tile) units; shared: some group has parts in several.
 struct NarrowPlan {
     int64_t x_groups, x_splits, x_per, w_groups, w_tiles, w_share, w_shares;
     bool w_shared;
 };
-bool narrow_fits(int dtype, int64_t D);
-NarrowPlan narrow_plan(int dtype, int64_t T, int64_t V, int64_t D);
-int narrow_rows(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_out, Running* part, float* z_target, float* dx_part, hipStream_t s);
-int narrow_cols(int dtype, const Problem& p, const NarrowPlan& n, int64_t width_out, const float* expo, const int* y, const float* rest, const float* gn,
-                const float* scale, void* dw, void* db, float* dw_part, float* db_part, hipStream_t s);
+template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D);
+template <typename T> int narrow_rows_of(const Problem& p, const NarrowPlan& n, int64_t width_out, Running* part, float* z_target, float* dx_part, hipStream_t s);
+template <typename T>
+int narrow_cols_of(const Problem& p, const NarrowPlan& n, int64_t width_out, const float* expo, const int* y, const float* rest, const float* gn,
+                   const float* scale, void* dw, void* db, float* dw_part, float* db_part, hipStream_t s);
+
+// widths of the narrow form: what fits the registers of a wave beside its sums
+inline bool narrow_fits(int dtype, int64_t D) { return D <= (dtype == RECO_DT_F32 ? 128 : 256); }
 
 }  // namespace xent
