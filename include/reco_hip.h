@@ -142,7 +142,7 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
  * target int64 [T]; a row whose target equals `ignore` has no loss and no gradient whatever its x holds; other targets outside
  * [0, V) are clamped and counted in *oob (nullable).  bias may hold -inf (items that are never offered) or the type's lowest value.
  * reduction: RECO_XENT_NONE (loss [T]), _MEAN over the rows that count (loss [1]; NaN when none does), _SUM.  loss and state are fp32.
- * state [2 T + 1] is written by the forward call and read by the gradient call, which takes the same operands.
+ * state [3 T + 1] is written by the forward call and read by the gradient call, which takes the same operands.
  * dx_unit: where reco_linear_xent_dx_floats() is not 0 (narrow rows), the forward call can write that many floats, dx for an incoming
  * gradient of one, in the same pass (NULL: no gradient of x will be asked for); the gradient call needs them for dx.
  * dloss fp32: [T] for RECO_XENT_NONE, else [1].  dx [T, D], dw [V, D], db [V] dense, of `dtype`; NULL = not wanted.

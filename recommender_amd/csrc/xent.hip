@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __r
     if (t >= p.T) return;
     const int64_t y = p.target[t];
     if (y == p.ignore) {
-        if (lane == 0) loss[t] = lse[t] = rest[t] = 0.f;
+        if (lane == 0) loss[t] = lse[t] = lse[p.T + t] = rest[t] = 0.f;
         if (dx_unit)
             for (int64_t d = lane; d < D_out; d += 64) dx_unit[t * D_out + d] = 0.f;
         return;
@@ -313,27 +313,32 @@ __global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __r
         const Running o{__shfl_xor(r.m, d, 64), __shfl_xor(r.s, d, 64)};
         r = (lane & d) ? joined(o, r) : joined(r, o);
     }
-    const float zt = z_target[t], others = r.m + logf(r.s), d = others - zt;
+    const float zt = z_target[t], ls = logf(r.s), d = (r.m - zt) + ls;
     // log(1 + e^d) from the smaller of e^d and e^-d; a target at -inf leaves the others' sum, a row of -inf alone is NaN
     const float e = expf(-fabsf(d)), l = log1pf(e);
-    const bool none = d != d || zt == INFINITY;
-    const float whole = none ? NAN : d > 0.f ? others + l : zt + l;
-    const float q = none ? NAN : d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
+    const bool none = d != d || zt == INFINITY, target_less = d > 0.f;
+    const float q = none ? NAN : target_less ? 1.f / (1.f + e) : e / (1.f + e);
     if (lane == 0) {
         if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
-        loss[t] = none ? NAN : d > 0.f ? d + l : l;
-        lse[t] = whole;
+        loss[t] = none ? NAN : target_less ? d + l : l;
+        // lse in two parts: as 32 bits round it, and what that leaves
+        const float base = target_less ? r.m : zt, more = target_less ? ls + l : l, whole = base + more;
+        lse[t] = none ? NAN : whole;
+        lse[p.T + t] = none ? NAN : (base - whole) + more;
         rest[t] = q;
     }
     if (!dx_unit) return;
+    // p of a part's term = exp(m - M) / sum, all of them and the target's against one M
+    const float M = fmaxf(r.m, zt), sum = r.s * exp2f((r.m - M) * LOG2E) + exp2f((zt - M) * LOG2E);
     const T* w = (const T*)p.w + clamp_target(y, p.V) * p.ldw;
     for (int64_t c = lane; c < D_out; c += 64) {
-        float sum = 0.f;
+        float total = 0.f;
+#pragma unroll 4
         for (int64_t s = 0; s < splits; ++s) {
-            const float m = part[s * p.T + t].m;
-            if (m != -INFINITY) sum = fmaf(exp2f((m - whole) * LOG2E), dx_part[(s * p.T + t) * D_out + c], sum);
+            const float m = part[s * p.T + t].m, v = dx_part[(s * p.T + t) * D_out + c];
+            total += m != -INFINITY ? exp2f((m - M) * LOG2E) * v : 0.f;
         }
-        dx_unit[t * D_out + c] = fmaf(-q, (float)w[c], sum);
+        dx_unit[t * D_out + c] = none ? NAN : fmaf(-q, (float)w[c], total / sum);
     }
 }
 
@@ -400,7 +405,7 @@ __global__ __launch_bounds__(256) void top_kernel(Problem p, const float* __rest
 // Also what the gradient kernels read per row: the target as 32 bits (-1: the row does not count), and for the narrow form the constant
 // of its exponentials (see narrow_cols_kernel).
 __global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, const float* __restrict__ dloss, const float* __restrict__ count,
-                                                      const float* __restrict__ tops, int n_tops, const float* __restrict__ lse, float g_log2,
+                                                      const float* __restrict__ tops, int n_tops, const float* __restrict__ lse, int whole_lse, float g_log2,
                                                       float* __restrict__ gn, float* __restrict__ scale, int* __restrict__ y, float* __restrict__ expo)
 {
     float unit = 1.f;
@@ -425,8 +430,10 @@ __global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, 
         const bool in = target != p.ignore;
         y[t] = in ? (int)clamp_target(target, p.V) : -1;
         if (reduction == REDUCE_NONE) gn[t] = in ? dloss[t] / unit : 0.f;
-        if (p.bias) expo[t] = in ? lse[t] : INFINITY;
-        else expo[t] = in ? fmaf(-LOG2E, lse[t], g_log2) : -INFINITY;
+        if (p.bias || whole_lse) {
+            expo[t] = in ? lse[t] : INFINITY;
+            expo[p.T + t] = in ? -LOG2E * lse[p.T + t] : 0.f;
+        } else expo[t] = in ? fmaf(-LOG2E, lse[t], g_log2) : -INFINITY;
     }
 }
 
@@ -479,7 +486,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
         const int64_t y0 = t < p.T ? p.target[t] : p.ignore;
         const bool in = y0 != p.ignore;
         const int64_t y = in ? clamp_target(y0, p.V) : -1;
-        const float l = in ? lse[t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE : 0.f;
+        const float l = in ? lse[t] : 0.f, low = in ? -LOG2E * lse[p.T + t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE : 0.f;
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
 #pragma unroll
@@ -489,7 +496,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int64_t v = m0 + wm + c + u;
-                    const float e = v == y ? -q : __builtin_amdgcn_exp2f((acc[i][j][4 * r4 + u] - l) * LOG2E);
+                    const float e = v == y ? -q : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * r4 + u] - l, LOG2E, low));
                     o.v[u] = (T)(in && v < p.V ? e * g : 0.f);
                 }
                 *reinterpret_cast<Pack<T, 4>*>(mine + row * ROW + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC) = o;
@@ -815,13 +822,13 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
         });
         if (rs) return rs;
     }
-    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, splits, z_target, rows, state, state + a.T, oob, dx_part, a.D,
+    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D,
                        dx_part ? dx_unit : nullptr);
     if (reduction != REDUCE_NONE) {
         int blocks = (int)clamp64(ceil_div64(a.T, REDUCE_ROWS), 1, 256);
-        hipLaunchKernelGGL(reduce_kernel, dim3(blocks), dim3(1024), 0, s, p, rows, nullptr, 0, reduction, loss, state + 2 * a.T, sums);
+        hipLaunchKernelGGL(reduce_kernel, dim3(blocks), dim3(1024), 0, s, p, rows, nullptr, 0, reduction, loss, state + 3 * a.T, sums);
         if (blocks > 1)
-            hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, s, p, rows, sums, blocks, reduction, loss, state + 2 * a.T, nullptr);
+            hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, s, p, rows, sums, blocks, reduction, loss, state + 3 * a.T, nullptr);
     }
     RECO_CHECK_LAUNCH();
     return RECO_OK;
@@ -838,7 +845,7 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
     float* scale = (float*)c.take(4);
     float* tops = (float*)c.take(256 * 4);
     int* y = (int*)c.take((size_t)a.T * 4);
-    float* expo = (float*)c.take((size_t)a.T * 4);
+    float* expo = (float*)c.take((size_t)a.T * 8);
     const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
     const BackwardPlan b = narrow ? BackwardPlan{} : backward_plan(a.T, a.V, a.D, sizeof(T));
     T* G = nullptr;
@@ -859,13 +866,13 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
     if (rc) return rc;
     *need = c.used;
     if (!launch) return RECO_OK;
-    const float *lse = state, *rest = state + a.T;
+    const float *lse = state, *rest = state + 2 * a.T;
     const int row_blocks = (int)clamp64(ceil_div64(a.T, 256), 1, 256);
     if (reduction == REDUCE_NONE)
         hipLaunchKernelGGL(top_kernel, dim3(row_blocks), dim3(256), 0, s, p, dloss, tops);
     else
         gn = nullptr;
-    hipLaunchKernelGGL(weights_kernel, dim3(row_blocks), dim3(256), 0, s, p, reduction, dloss, state + 2 * a.T, tops, row_blocks, lse,
+    hipLaunchKernelGGL(weights_kernel, dim3(row_blocks), dim3(256), 0, s, p, reduction, dloss, state + 3 * a.T, tops, row_blocks, lse, (int)(sizeof(T) == 4),
                        log2f(Traits<T>::G_SCALE), gn, scale, y, expo);
     if (narrow) {
         if (dw || db) {

@@ -341,8 +341,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_rows_ke
             me.template block<DX, (NS > 1)>(
                 ring + after * BLOCK_BYTES, ring + then * BLOCK_BYTES, ring + at * BLOCK_BYTES, next, s, o,
                 [&](int r) {
-                    // with a bias the logits may be the type's lowest: their difference first
-                    s[r] = BIAS ? exp2_fast(fmaf(s[r] - base, LOG2E, e_shift<T>())) : exp2_fast(fmaf(s[r], LOG2E, shift));
+                    // the difference first in 32 bits, for its digits, and with a bias, whose logits may be the type's lowest
+                    s[r] = BIAS || W::WIDE ? exp2_fast(fmaf(s[r] - base, LOG2E, e_shift<T>())) : exp2_fast(fmaf(s[r], LOG2E, shift));
                 },
                 [] {},
                 [&](int k, int n) {
@@ -384,8 +384,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_rows_ke
 // ---------------------------------------------------------------------------------------------
 // cols: dW and dbias
 // ---------------------------------------------------------------------------------------------
-// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count; with a bias, whose logits may be the type's lowest, lse_t
-// itself and +inf.  y[t]: the target, -1 for rows that do not count.  EACH: rows have weights gn[t].
+// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count.  In 32 bits, and with a bias, whose logits may be the type's
+// lowest: lse_t itself (+inf), and in 32 bits expo[T + t] minus what rounding left of lse_t, times log2(e).  y[t]: the target, -1 for
+// rows that do not count.  EACH: rows have weights gn[t].
 // The work is groups of 128 held rows times tiles of streamed ones, in that order; every workgroup takes an equal share of consecutive
 // (group, tile) units, so that the groups need not be a multiple of what the chip holds at once (782 groups over 512 places: 0.72 ms
 // with a group to a workgroup).  A group inside one share is finished there; else its parts are written in 32 bits (place 1 of a
@@ -402,6 +403,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     typedef Wave<T, DP> W;
     __shared__ __attribute__((aligned(16))) char tiles[3][Streamed::BYTES];
     __shared__ __attribute__((aligned(16))) float expos[3][SB];
+    __shared__ __attribute__((aligned(16))) float lows[W::WIDE ? 3 : 1][SB];
     __shared__ __attribute__((aligned(16))) float gns[EACH ? 3 : 1][SB];
     __shared__ __attribute__((aligned(16))) float minus_q[3][SB];
     __shared__ __attribute__((aligned(16))) int ys[4][SB];
@@ -428,14 +430,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     for (int d = 0; d < W::BLOCKS; ++d) o[d] = f32x16{};
 
     Streamed st;
-    float expo_reg = 0.f, gn_reg = 0.f, q_reg = 0.f;
+    float expo_reg = 0.f, low_reg = 0.f, gn_reg = 0.f, q_reg = 0.f;
     int y_reg = -1;
     auto fetch = [&](int tile) {
         const int64_t t0 = first + (int64_t)tile * SB;
         st.load((const T*)p.x, p.ldx, end, (int)p.D, t0);
         if (threadIdx.x < SB) {
             const int64_t t = t0 + threadIdx.x;
-            expo_reg = t < end ? expo[t] : BIAS ? INFINITY : -INFINITY;
+            expo_reg = t < end ? expo[t] : BIAS || W::WIDE ? INFINITY : -INFINITY;
+            if (W::WIDE) low_reg = t < end ? expo[p.T + t] : 0.f;
             y_reg = t + SB < end ? y[t + SB] : -1;
             q_reg = t < end ? rest[t] : 0.f;
             if (EACH) gn_reg = t < end ? gn[t] : 0.f;
@@ -447,6 +450,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
         st.store(tiles[at], ys[tile & 3]);
         if (threadIdx.x < SB) {
             expos[at][threadIdx.x] = expo_reg;
+            if (W::WIDE) lows[W::WIDE ? at : 0][threadIdx.x] = low_reg;
             minus_q[at][threadIdx.x] = -Traits<T>::G_SCALE * (EACH ? q_reg * gn_reg : q_reg);
             ys[(tile + 1) & 3][threadIdx.x] = y_reg;
             if (EACH) gns[at][threadIdx.x] = gn_reg;
@@ -463,7 +467,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     __syncthreads();
     const int n_blocks = (int)((end - first + 31) / 32);
     f32x16 s0 = {}, s1;
-    f32x4 x4, g4, x_next = {}, g_next = {};
+    f32x4 x4, g4, low4, x_next = {}, g_next = {};
     if (active) {
         x_next = *reinterpret_cast<const f32x4*>(&expos[0][4 * half]);
         if (EACH) g_next = *reinterpret_cast<const f32x4*>(&gns[0][4 * half]);
@@ -488,12 +492,14 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
                         const int ahead = r < 12 ? at * 32 + 8 * (r / 4 + 1) : after * 32;
                         x4 = x_next;
                         x_next = *reinterpret_cast<const f32x4*>(expo32 + ahead);
+                        if (W::WIDE) low4 = *reinterpret_cast<const f32x4*>(&lows[0][0] + at * 32 + 2 * r + 4 * half);
                         if (EACH) {
                             g4 = g_next;
                             g_next = *reinterpret_cast<const f32x4*>(gn32 + ahead);
                         }
                     }
-                    const float e = BIAS ? exp2_fast(fmaf(s[r] + bias - x4[r % 4], LOG2E, G_LOG2<T>)) : exp2_fast(fmaf(s[r], LOG2E, x4[r % 4]));
+                    const float e = W::WIDE ? exp2_fast(fmaf((BIAS ? s[r] + bias : s[r]) - x4[r % 4], LOG2E, low4[r % 4]))
+                                    : BIAS ? exp2_fast(fmaf(s[r] + bias - x4[r % 4], LOG2E, G_LOG2<T>)) : exp2_fast(fmaf(s[r], LOG2E, x4[r % 4]));
                     s[r] = EACH ? e * g4[r % 4] : e;
                 },
                 [&] {

@@ -540,7 +540,7 @@ def _xent(x, weight, target, bias, reduction, ignore_index, check_ids, with_dx):
         return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), None
     L = _lib.lib()
     floats = L.reco_linear_xent_dx_floats(dtype, T, D) if with_dx else 0
-    state = torch.empty(floats + 2 * T + 1, dtype=torch.float32, device=dev)
+    state = torch.empty(floats + 3 * T + 1, dtype=torch.float32, device=dev)
     at = state.data_ptr()
     oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
     what = (x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight))
@@ -563,7 +563,7 @@ def _xent_grad(x, weight, target, bias, state, dloss, reduction, ignore_index, w
     if T == 0:
         return [o if o is None else o.zero_() for o in (dx, dw, db)]
     L = _lib.lib()
-    floats = state.numel() - 2 * T - 1
+    floats = state.numel() - 3 * T - 1
     at = state.data_ptr()
     what = (x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight))
     nbytes = L.reco_linear_xent_grad_workspace_bytes(*what, dtype, T, V, D)

@@ -35,12 +35,14 @@ def _close(got, exact, tol, what):
 
 
 def _reference(ids, grad, rows, scale, padding):
-    """(gradient, sum of |terms|, terms per row) in 64 bits."""
+    """(gradient, sum of |terms|, terms per row) in 64 bits, on the host (a frequent id's adds queue up on the GPU)."""
+    dev = grad.device
+    ids, grad = ids.cpu(), grad.cpu()
     keep = torch.ones_like(ids, dtype=torch.bool) if padding is None else ids != padding
     ids, g = ids[keep], grad.double()[keep] * scale
-    total = torch.zeros((rows, grad.shape[1]), dtype=torch.float64, device=grad.device).index_add_(0, ids, g)
+    total = torch.zeros((rows, grad.shape[1]), dtype=torch.float64).index_add_(0, ids, g)
     size = torch.zeros_like(total).index_add_(0, ids, g.abs())
-    return total, size, torch.bincount(ids, minlength=rows).double()[:, None]
+    return total.to(dev), size.to(dev), torch.bincount(ids, minlength=rows).double()[:, None].to(dev)
 
 
 def _check_grad(ids, grad, rows, scale=1.0, padding=None):
@@ -95,7 +97,8 @@ def test_ids_out_of_range():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,dim,n", [
     (1, 1, 1), (1, 5, 3000), (2, 3, 9), (6038, 64, 4096), (6038, 64, 4097), (2047, 16, 20000), (2048, 24, 20000), (60401, 50, 70001),
-    (1000000, 8, 5000), (5000000, 4, 30000), (13, 300, 777), (300, 513, 1200), (5, 128, 9000)])
+    (1000000, 8, 5000), (5000000, 4, 30000), (13, 300, 777), (300, 513, 1200), (5, 128, 9000), (70000, 6, 1300003),
+    (2048, 130, 140000)])
 def test_gradient(dtype, rows, dim, n):
     g = torch.Generator(device="cuda").manual_seed(rows + 31 * dim + n)
     grad = torch.randn(n, dim, device="cuda", generator=g).to(dtype)

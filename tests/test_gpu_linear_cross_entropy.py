@@ -144,6 +144,50 @@ def test_many_tiles_and_pieces(dtype, T, V, D):
     _check(x, w, target, b, "mean")
 
 
+EDGES = [1, 2, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 512, 700]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seed", range(12))
+def test_sizes_around_every_tile(dtype, seed):
+    import random
+    rng = random.Random(1000 + seed)
+    T, V, D = rng.choice(EDGES), rng.choice(EDGES) + rng.choice([0, 0, 512, 2048]), rng.choice(EDGES)
+    x, w, target, b = _problem(T, V, D, dtype, rng.random() < 0.5, seed)
+    if rng.random() < 0.5:
+        target[torch.rand(T, device="cuda") < 0.3] = -100
+        target[0] = V - 1
+    reduction = rng.choice(["mean", "sum", "none"])
+    g = torch.randn(T, device="cuda") if reduction == "none" else None if rng.random() < 0.5 else torch.tensor(2.5, device="cuda")
+    _check(x, w, target, b, reduction, g=torch.ones(T, device="cuda") if reduction == "none" and g is None else g, what=str((T, V, D, reduction)))
+
+
+def test_ignore_index_may_be_a_column():
+    x, w, target, b = _problem(64, 40, 24, torch.float32, True)
+    target[::4] = 5
+    _check(x, w, target, b, "mean", ignore=5)
+    _check(x, w, target, b, "none", ignore=-1, g=torch.ones(64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(300, 900, 64), (300, 900, 128), (400, 700, 200), (300, 600, 320)])
+def test_one_popular_target_and_one_target_for_all(dtype, T, V, D):
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    target[torch.rand(T, device="cuda") < 0.6] = V // 2
+    _check(x, w, target, b, "mean")
+    target[:] = V - 1
+    _check(x, w, target, None, "none", g=torch.randn(T, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_repeats_bit_for_bit(dtype):
+    for T, V, D in ((2000, 3001, 100), (700, 3000, 400)):
+        p = _problem(T, V, D, dtype, True)
+        first = _ops().linear_cross_entropy_grad(*p)
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(first, _ops().linear_cross_entropy_grad(*p)))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_all_rows_ignored(dtype):
     ops = _ops()
