@@ -289,36 +289,49 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
     if (threadIdx.x < B && t < p.T) part[split * p.T + t] = joined(sh[threadIdx.x], sh[B + threadIdx.x]);
 }
 
-// One wave per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
-// sums of W [splits][T][D_out], also dx for an incoming gradient of one, in 32 bits.
-template <typename T>
-__global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits, const float* __restrict__ z_target,
-                                                   float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
-                                                   const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
+// WAVES waves per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
+// sums of W [splits][T][D_out], D_out <= 256, also dx for an incoming gradient of one, in 32 bits.  A wave takes 64 splits at a time, and
+// what it waits for is memory: with one wave to a row, 505 splits of 16 rows x 128 took 40 to 72 us, with eight 15; up to 64 splits the
+// further waves only cost (6038 rows x 32: 11 us with one, 25 with four; 8192 x 128: 15, 34).
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits,
+                                                                            const float* __restrict__ z_target, float* __restrict__ loss,
+                                                                            float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
+                                                                            const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
 {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    __shared__ Running runs[WAVES];
+    __shared__ float sums[WAVES > 1 ? WAVES : 1][WAVES > 1 ? 256 : 1];
+    const int lane = threadIdx.x & 63, wave = WAVES > 1 ? threadIdx.x >> 6 : 0;
+    const int64_t t = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= p.T) return;
     const int64_t y = p.target[t];
     if (y == p.ignore) {
+        if (wave) return;
         if (lane == 0) loss[t] = lse[t] = lse[p.T + t] = rest[t] = 0.f;
         if (dx_unit)
             for (int64_t d = lane; d < D_out; d += 64) dx_unit[t * D_out + d] = 0.f;
         return;
     }
     Running r{-INFINITY, 0.f};
-    for (int64_t s = lane; s < splits; s += 64) r = joined(r, part[s * p.T + t]);
+    for (int64_t s = wave * 64 + lane; s < splits; s += 64 * WAVES) r = joined(r, part[s * p.T + t]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const Running o{__shfl_xor(r.m, d, 64), __shfl_xor(r.s, d, 64)};
         r = (lane & d) ? joined(o, r) : joined(r, o);
+    }
+    if constexpr (WAVES > 1) {
+        if (lane == 0) runs[wave] = r;
+        __syncthreads();
+        r = runs[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) r = joined(r, runs[i]);
     }
     const float zt = z_target[t], ls = logf(r.s), d = (r.m - zt) + ls;
     // log(1 + e^d) from the smaller of e^d and e^-d; a target at -inf leaves the others' sum, a row of -inf alone is NaN
     const float e = expf(-fabsf(d)), l = log1pf(e);
     const bool none = d != d || zt == INFINITY, target_less = d > 0.f;
     const float q = none ? NAN : target_less ? 1.f / (1.f + e) : e / (1.f + e);
-    if (lane == 0) {
+    if (wave == 0 && lane == 0) {
         if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
         loss[t] = none ? NAN : target_less ? d + l : l;
         // lse in two parts: as 32 bits round it, and what that leaves
@@ -330,15 +343,42 @@ __global__ __launch_bounds__(256) void rows_kernel(Problem p, const Running* __r
     if (!dx_unit) return;
     // p of a part's term = exp(m - M) / sum, all of them and the target's against one M
     const float M = fmaxf(r.m, zt), sum = r.s * exp2f((r.m - M) * LOG2E) + exp2f((zt - M) * LOG2E);
+    float total[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t s0 = wave * 64; s0 < splits; s0 += 64 * WAVES) {
+        // each lane has one split's factor: 0 for a split of nothing but -inf, whose sums are not looked at
+        const float mine = s0 + lane < splits ? part[(s0 + lane) * p.T + t].m : -INFINITY, f = mine != -INFINITY ? exp2f((mine - M) * LOG2E) : 0.f;
+        const int n = splits - s0 < 64 ? (int)(splits - s0) : 64;
+        const float* src = dx_part + (s0 * p.T + t) * D_out;
+        for (int i = 0; i < n; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (64 * k >= D_out) break;
+                const int c = 64 * k + lane < D_out ? 64 * k + lane : (int)D_out - 1;        // eight loads on their way, none of them behind a branch
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = src[(int64_t)(i + j < n ? i + j : n - 1) * p.T * D_out + c];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float fj = __shfl(f, i + j, 64);
+                    total[k] += fj != 0.f ? fj * v[j] : 0.f;
+                }
+            }
+    }
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[wave][64 * k + lane] = total[k];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) total[k] += sums[i][64 * k + lane];
+    }
     const T* w = (const T*)p.w + clamp_target(y, p.V) * p.ldw;
-    for (int64_t c = lane; c < D_out; c += 64) {
-        float total = 0.f;
-#pragma unroll 4
-        for (int64_t s = 0; s < splits; ++s) {
-            const float m = part[s * p.T + t].m, v = dx_part[(s * p.T + t) * D_out + c];
-            total += m != -INFINITY ? exp2f((m - M) * LOG2E) * v : 0.f;
-        }
-        dx_unit[t * D_out + c] = none ? NAN : fmaf(-q, (float)w[c], total / sum);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int c = 64 * k + lane;
+        if (c < D_out) dx_unit[t * D_out + c] = none ? NAN : fmaf(-q, (float)w[c], total[k] / sum);
     }
 }
 
@@ -822,8 +862,13 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
         });
         if (rs) return rs;
     }
-    hipLaunchKernelGGL(rows_kernel<T>, dim3((unsigned)ceil_div64(a.T, 4)), dim3(256), 0, s, p, part, splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D,
-                       dx_part ? dx_unit : nullptr);
+    const auto join = [&](auto waves) {
+        constexpr int WAVES = decltype(waves)::value;
+        hipLaunchKernelGGL((rows_kernel<T, WAVES>), dim3((unsigned)(WAVES > 1 ? a.T : ceil_div64(a.T, 4))), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, s, p, part,
+                           splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D, dx_part ? dx_unit : nullptr);
+    };
+    if (splits > 64) join(std::integral_constant<int, 8>());
+    else join(std::integral_constant<int, 1>());
     if (reduction != REDUCE_NONE) {
         int blocks = (int)clamp64(ceil_div64(a.T, REDUCE_ROWS), 1, 256);
         hipLaunchKernelGGL(reduce_kernel, dim3(blocks), dim3(1024), 0, s, p, rows, nullptr, 0, reduction, loss, state + 3 * a.T, sums);

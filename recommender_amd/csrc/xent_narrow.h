@@ -212,6 +212,19 @@ template <typename T, int DP> constexpr int stream_rows() { return DP * (int)siz
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }        // below 2^-126: 0
 
+// Four values of a row from column c on; fours: rows are whole aligned groups of four
+template <typename U> __device__ __forceinline__ void store4(U* row, int c, int width, bool fours, float v0, float v1, float v2, float v3)
+{
+    if (fours) {
+        if (c < width) *reinterpret_cast<Pack<U, 4>*>(row + c) = Pack<U, 4>{{(U)v0, (U)v1, (U)v2, (U)v3}};
+        return;
+    }
+    if (c < width) row[c] = (U)v0;
+    if (c + 1 < width) row[c + 1] = (U)v1;
+    if (c + 2 < width) row[c + 2] = (U)v2;
+    if (c + 3 < width) row[c + 3] = (U)v3;
+}
+
 // Waves per SIMD that the registers are cut for
 template <typename T, int DP> constexpr int waves_per_simd() { return DP * (int)sizeof(T) >= 512 ? 1 : 2; }
 
@@ -369,15 +382,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_rows_ke
     if (half == 0) part[split * p.T + t] = Running{m, total * exp2f(-e_shift<T>())};
     if constexpr (DX) {
         float* dst = dx_part + (split * p.T + t) * width_out;
+        const float f = exp2f(-e_shift<T>());
 #pragma unroll
         for (int d = 0; d < W::BLOCKS; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = 32 * d + 8 * q + 4 * half + i;
-                    if (c < width_out) dst[c] = o[d][4 * q + i] * exp2f(-e_shift<T>());
-                }
+                store4(dst, 32 * d + 8 * q + 4 * half, width_out, width_out % 4 == 0, o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f);
     }
 }
 
@@ -410,19 +420,20 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
     char* const ring = &tiles[0][0];
     constexpr int BLOCK_BYTES = 32 * W::ROWB, RING = 3 * NS;
-    const int64_t u1 = (blockIdx.x + 1) * share < units ? (blockIdx.x + 1) * share : units;
+    const bool fours = width_out % 4 == 0 && (uintptr_t)dw % sizeof(Pack<T, 4>) == 0;
+    const int64_t u0 = blockIdx.x * share, u1 = u0 + share < units ? u0 + share : units;
+    W me;
+    me.init((const T*)p.w, p.ldw, p.V, (int)p.D, (u0 / tiles_in_all * 4 + wave) * 32);
 #pragma unroll 1
-    for (int64_t u = blockIdx.x * share; u < u1;) {
+    for (int64_t u = u0; u < u1;) {
     const int64_t group = u / tiles_in_all;
     const int tile0 = (int)(u - group * tiles_in_all), n_tiles = u1 - u < tiles_in_all - tile0 ? (int)(u1 - u) : tiles_in_all - tile0;
     const int64_t h0 = (group * 4 + wave) * 32, v = h0 + l31;
     const bool active = h0 < p.V;
     const int64_t first = (int64_t)tile0 * SB, end = first + (int64_t)n_tiles * SB < p.T ? first + (int64_t)n_tiles * SB : p.T;
-    const bool whole = n_tiles == tiles_in_all;
+    const bool whole = n_tiles == tiles_in_all, stage = u == u0 || tiles_in_all > 1;     // a single tile stays for every group
     u += n_tiles;
 
-    W me;
-    me.init((const T*)p.w, p.ldw, p.V, (int)p.D, h0);
     const float bias = BIAS && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
     float sum = 0.f;
     f32x16 o[W::BLOCKS];
@@ -456,15 +467,17 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
             if (EACH) gns[at][threadIdx.x] = gn_reg;
         }
     };
-    if (threadIdx.x < 2 * SB) ys[threadIdx.x / SB][threadIdx.x % SB] = first + threadIdx.x < end ? y[first + threadIdx.x] : -1;
-    __syncthreads();
-    fetch(0);
-    put(0);
-    if (n_tiles > 1) {
-        fetch(1);
-        put(1);
+    if (stage) {
+        if (threadIdx.x < 2 * SB) ys[threadIdx.x / SB][threadIdx.x % SB] = first + threadIdx.x < end ? y[first + threadIdx.x] : -1;
+        __syncthreads();
+        fetch(0);
+        put(0);
+        if (n_tiles > 1) {
+            fetch(1);
+            put(1);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const int n_blocks = (int)((end - first + 31) / 32);
     f32x16 s0 = {}, s1;
     f32x4 x4, g4, low4, x_next = {}, g_next = {};
@@ -519,7 +532,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
                     for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) sum += s[r];
                 });
         }
-        if (i % NS == NS - 1) {
+        if (i % NS == NS - 1 && tile + 1 < n_tiles) {
             if (tile + 2 < n_tiles) put(tile + 2);
             __syncthreads();
         }
@@ -530,7 +543,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
         work(i, s0, s1);
         if (i + 1 < n_blocks) work(i + 1, s1, s0);
     }
-    __syncthreads();                                            // the next group's tiles overwrite these
+    if (tiles_in_all > 1) __syncthreads();                      // the next group's tiles overwrite these
+    if (u < u1) me.init((const T*)p.w, p.ldw, p.V, (int)p.D, ((group + 1) * 4 + wave) * 32);      // on its way during the stores
     if (!active) continue;
     const float f = whole ? *scale / Traits<T>::G_SCALE : 1.f;
     const float total = (sum + __shfl_xor(sum, 32, 64)) * f;
@@ -540,17 +554,14 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
         if (!whole) db_part[row] = total;
         else if (db) db[v] = (T)total;
     }
+    if (!whole || dw)
 #pragma unroll
-    for (int d = 0; d < W::BLOCKS; ++d)
+        for (int d = 0; d < W::BLOCKS; ++d)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = 32 * d + 8 * q + 4 * half + i;
-                if (c < width_out) {
-                    if (!whole) dw_part[row * width_out + c] = o[d][4 * q + i];
-                    else if (dw) dw[v * width_out + c] = (T)(o[d][4 * q + i] * f);
-                }
+            for (int q = 0; q < 4; ++q) {
+                const int c = 32 * d + 8 * q + 4 * half;
+                if (!whole) store4(dw_part + row * width_out, c, width_out, width_out % 4 == 0, o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
+                else store4(dw + v * width_out, c, width_out, fours, o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f);
             }
     }
 }
