@@ -36,10 +36,10 @@ template <int CH> __device__ __forceinline__ int twist(int row)
     return ((row >> 2) & 3) | ((row / (16 / C)) & (C / 4 - 1)) << 2;
 }
 
-template <typename T, int DP, int SB> struct Tile {
+template <typename T, int DP, int SB, int THREADS = 256> struct Tile {
     static constexpr int VEC = Traits<T>::VEC, ROWB = DP * (int)sizeof(T), CH = ROWB / 16, BYTES = SB * ROWB;
-    static constexpr int PIECES = SB * CH / 256, ROW_STEP = 256 / CH;
-    static_assert(SB * CH % 256 == 0 && (CH == 4 || CH % 8 == 0) && (CH & (CH - 1)) == 0, "tile shape");
+    static constexpr int PIECES = SB * CH / THREADS, ROW_STEP = THREADS / CH;
+    static_assert(SB * CH % THREADS == 0 && THREADS % CH == 0 && (CH == 4 || CH % 8 == 0) && (CH & (CH - 1)) == 0, "tile shape");
     Pack<T, VEC> reg[PIECES];
 
     // rows r0 .. of m [rows, ld], `width` values each
@@ -231,18 +231,18 @@ template <typename T, int DP> constexpr int waves_per_simd() { return DP * (int)
 // ---------------------------------------------------------------------------------------------
 // rows: loss statistics, and with DX the softmax-weighted sums of W
 // ---------------------------------------------------------------------------------------------
-template <typename T, int DP, bool BIAS, bool DX>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out,
+template <typename T, int DP, bool BIAS, bool DX, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, (waves_per_simd<T, DP>())) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out,
                                                                                    Running* __restrict__ part, float* __restrict__ z_target,
                                                                                    float* __restrict__ dx_part)
 {
     constexpr int SB = stream_rows<T, DP>(), NS = SB / 32;
-    typedef Tile<T, DP, SB> Streamed;
+    typedef Tile<T, DP, SB, WAVES * 64> Streamed;
     typedef Wave<T, DP> W;
     __shared__ __attribute__((aligned(16))) char tiles[3][Streamed::BYTES];
     __shared__ __attribute__((aligned(16))) float biases[3][SB];
     const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t split = blockIdx.x % splits, h0 = (blockIdx.x / splits * 4 + wave) * 32, t = h0 + l31;
+    const int64_t split = blockIdx.x % splits, h0 = (blockIdx.x / splits * WAVES + wave) * 32, t = h0 + l31;
     const bool active = h0 < p.T;
     const T* w = (const T*)p.w;
     const T* bias = (const T*)p.bias;
@@ -603,6 +603,11 @@ template <typename F> int with_flag(bool v, F&& fn) { return v ? fn(std::true_ty
 
 constexpr int64_t HELD = 128;                  // held rows per workgroup: 4 waves of 32
 
+// Up to 32 rows keep one wave of a workgroup busy.  In 32 bits at 65 to 128 values a compute unit holds one workgroup of four waves but
+// three of one wave, and the matrix instructions bound the launch: 1 row x 1 M x 128 164 us instead of 326, with dx 255 instead of 551.
+// In 16 bits, and with shorter rows, memory does, which four waves ask more of at once (bf16 1 x 1 M x 128: 47 us, 59 with one wave).
+template <typename T, int DP> constexpr bool ONE_WAVE = sizeof(T) == 4 && DP == 128;
+
 template <typename T, typename F> int shape_of(int64_t D, F&& fn)
 {
     return with_width<T>(D, [&](auto dp) -> int {
@@ -639,8 +644,11 @@ template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64
 {
     NarrowPlan n{};
     (void)shape_of<T>(D, [&](auto dp, int64_t tile, int64_t places) -> int {
-        n.x_groups = ceil_div64(T_rows, HELD);
-        split_plan(T_rows, decltype(dp)::value, n.x_groups, V, tile, places, sizeof(T) == 2 ? 0.8e15 : 0.12e15, &n.x_splits, &n.x_per);
+        constexpr int DP = decltype(dp)::value;
+        n.x_waves = ONE_WAVE<T, DP> && T_rows <= 32 ? 1 : 4;
+        n.x_groups = ceil_div64(T_rows, 32 * n.x_waves);
+        const int64_t x_places = n.x_waves == 4 ? places : 256 * (160 * 1024 / (3 * tile * (DP * (int)sizeof(T) + 4)));
+        split_plan(T_rows, DP, n.x_groups, V, tile, x_places, sizeof(T) == 2 ? 0.8e15 : 0.12e15, &n.x_splits, &n.x_per);
         n.w_groups = ceil_div64(V, HELD);
         n.w_tiles = ceil_div64(T_rows, tile);
         const int64_t units = n.w_groups * n.w_tiles;
@@ -659,8 +667,19 @@ template <typename T> int narrow_rows_of(const Problem& p, const NarrowPlan& n, 
     return shape_of<T>(p.D, [&](auto dp, int64_t, int64_t) -> int {
         return with_flag(p.bias != nullptr, [&](auto bias) -> int {
             return with_flag(dx_part != nullptr, [&](auto dx) -> int {
-                hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(dx)::value>),
-                                   dim3((unsigned)(n.x_groups * n.x_splits)), dim3(256), 0, s, p, (int)n.x_splits, n.x_per, (int)width_out, part, z_target, dx_part);
+                const auto launch = [&](auto waves) {
+                    constexpr int WAVES = decltype(waves)::value;
+                    hipLaunchKernelGGL((narrow_rows_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(dx)::value, WAVES>),
+                                       dim3((unsigned)(n.x_groups * n.x_splits)), dim3(WAVES * 64), 0, s, p, (int)n.x_splits, n.x_per, (int)width_out, part,
+                                       z_target, dx_part);
+                };
+                if constexpr (ONE_WAVE<T, decltype(dp)::value>)
+                    if (n.x_waves == 1) {
+                        launch(std::integral_constant<int, 1>());
+                        RECO_CHECK_LAUNCH();
+                        return RECO_OK;
+                    }
+                launch(std::integral_constant<int, 4>());
                 RECO_CHECK_LAUNCH();
                 return RECO_OK;
             });

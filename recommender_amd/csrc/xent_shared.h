@@ -66,7 +66,7 @@ __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 
 // The form for narrow rows (xent_narrow.h).  x: groups of held rows, times splits of `per` vocabulary rows.  w: groups of held
 // vocabulary rows, times tiles of x rows, in shares of consecutive (group, tile) units; shared: some group has parts in several.
 struct NarrowPlan {
-    int64_t x_groups, x_splits, x_per, w_groups, w_tiles, w_share, w_shares;
+    int64_t x_waves, x_groups, x_splits, x_per, w_groups, w_tiles, w_share, w_shares;
     bool w_shared;
 };
 template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D);
