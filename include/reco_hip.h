@@ -143,8 +143,9 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
  * [0, V) are clamped and counted in *oob (nullable).  bias may hold -inf (items that are never offered) or the type's lowest value.
  * reduction: RECO_XENT_NONE (loss [T]), _MEAN over the rows that count (loss [1]; NaN when none does), _SUM.  loss and state are fp32.
  * state [3 T + 1] is written by the forward call and read by the gradient call, which takes the same operands.
- * dx_unit: where reco_linear_xent_dx_floats() is not 0 (narrow rows), the forward call can write that many floats, dx for an incoming
- * gradient of one, in the same pass (NULL: no gradient of x will be asked for); the gradient call needs them for dx.
+ * kept: the forward call can keep reco_linear_xent_kept_floats() floats for the gradient call (NULL: nothing), 16-byte aligned.  Narrow rows
+ * (up to 128 values in 32 bits, 256 in 16): dx for an incoming gradient of one, from the same pass; the gradient call needs it for dx.
+ * Wider ones: the logits, where that saves time and they are few (up to 512 MB); without them the gradient call computes them again.
  * dloss fp32: [T] for RECO_XENT_NONE, else [1].  dx [T, D], dw [V, D], db [V] dense, of `dtype`; NULL = not wanted.
  * Sums run in an order that depends on the sizes alone: the same bits on every run.  Work is enqueued only; calls that overlap need a
  * workspace each (*_workspace_bytes looks at x and w for their alignment, never through them), 16-byte aligned.
@@ -153,14 +154,14 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
 #define RECO_XENT_MEAN 1
 #define RECO_XENT_SUM  2
 size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D,
-                                        int with_dx);
-int64_t reco_linear_xent_dx_floats(int dtype, int64_t T, int64_t D);
+                                        int keep);
+int64_t reco_linear_xent_kept_floats(int dtype, int64_t T, int64_t V, int64_t D, int with_dx);
 int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                     const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, float* dx_unit, int32_t* oob,
+                     const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, float* kept, int32_t* oob,
                      void* ws, size_t ws_bytes, void* stream);
 size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D);
 int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                          const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dx_unit, const float* dloss,
+                          const int64_t* target, int64_t ignore, int reduction, const float* state, const float* kept, const float* dloss,
                           void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
 
 /* Linear layer over a SPARSE input given as CSR -- the "masked-observed" form of the AutoRec / Hybrid encoders, whose input

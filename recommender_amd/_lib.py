@@ -45,7 +45,7 @@ _SIGNATURES = {
     "reco_embedding_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int64, c_float, c_int64, c_void_p, c_void_p,
                                     c_size_t, c_void_p]),
     "reco_linear_xent_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, c_int]),
-    "reco_linear_xent_dx_floats": (c_int64, [c_int, c_int64, c_int64]),
+    "reco_linear_xent_kept_floats": (c_int64, [c_int, c_int64, c_int64, c_int64, c_int]),
     "reco_linear_xent": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "reco_linear_xent_grad_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64]),

@@ -132,6 +132,27 @@ __device__ __forceinline__ void pair_of(int64_t place, int64_t na, int64_t nb, i
 
 template <int B> using Acc = f32x16[Shape<B>::MB][Shape<B>::NB];
 
+// Whether the logits of the statistics may be kept for G: in 32 bits a product costs 2 D / 125 TFLOP/s per logit and its 8 bytes of traffic
+// 2 ps (f32 4096 x 20,000 x 768, with gradients: 3.18 ms, 4.01 with a second product; 3706 x 6040 x 500 0.70 ms, 0.87).  In 16 bits the two
+// are alike up to some 1000 values (bf16 4096 x 20,000 x 768: 0.86 both; 1000 x 60,000 x 2048: 1.34, 1.46), not worth the memory.
+template <typename T> constexpr bool KEEPS = sizeof(T) == 4;
+
+// A tile's logits as its lanes hold them (kept from the statistics for G): tile (token, vocabulary), then wave, register group, lane
+template <int B> __device__ __forceinline__ int64_t kept_at(int64_t token_tile, int64_t tiles_v, int64_t v_tile)
+{
+    return (token_tile * tiles_v + v_tile) * (B * B) + (threadIdx.x >> 6) * (B * B / (Shape<B>::THREADS / 64)) + (threadIdx.x & 63) * 4;
+}
+
+template <int B, typename F> __device__ __forceinline__ void each_kept(F&& fn)          // fn(i, j, first register, offset)
+{
+#pragma unroll
+    for (int i = 0; i < Shape<B>::MB; ++i)
+#pragma unroll
+        for (int j = 0; j < Shape<B>::NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) fn(i, j, r, ((i * Shape<B>::NB + j) * 4 + r / 4) * 256);
+}
+
 // All of this wave's loads and LDS accesses are done, then the workgroup's
 __device__ __forceinline__ void drain_and_meet()
 {
@@ -212,7 +233,8 @@ __device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, c
 }
 
 template <typename T, int B>
-__global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, int64_t splits, int64_t tiles_per_split, Running* __restrict__ part, float* __restrict__ z_target)
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, int64_t splits, int64_t tiles_per_split, Running* __restrict__ part,
+                                                                     float* __restrict__ z_target, float* __restrict__ kept)
 {
     typedef Shape<B> S;
     int64_t token_tile, split;
@@ -247,6 +269,12 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
 #pragma unroll
                     for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
                 }
+        if (KEEPS<T> && kept) {
+            float* to = kept + kept_at<B>(token_tile, (p.V + B - 1) / B, m0 / B);
+            each_kept<B>([&](int i, int j, int r, int at) {
+                *reinterpret_cast<f32x4*>(to + at) = f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+            });
+        }
         const bool tail = m0 + B > p.V;
 #pragma unroll
         for (int j = 0; j < S::NB; ++j) {
@@ -488,10 +516,10 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ unit,
         dx[i] = (T)(unit[i] * (gn ? gn[i / D] * f : f));
 }
 
-// G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero
-template <typename T, int B>
-__global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int64_t v0, const float* __restrict__ lse, const float* __restrict__ rest,
-                                                                 const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
+// G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero.  KEPT: from the logits of the statistics
+template <typename T, int B, bool KEPT>
+__global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int64_t v0, const float* __restrict__ kept, const float* __restrict__ lse,
+                                                                 const float* __restrict__ rest, const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
 {
     typedef Shape<B> S;
     int64_t token_tile, panel;
@@ -502,17 +530,28 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
     const int64_t n0 = token_tile * B, m0 = v0 + panel * B;
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     Acc<B> acc = {};
-    tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
-    if (bias)
+    if constexpr (KEPT) {
+        if (m0 < p.V) {
+            const float* from = kept + kept_at<B>(token_tile, (p.V + B - 1) / B, m0 / B);
+            each_kept<B>([&](int i, int j, int r, int at) {
+                const f32x4 z = *reinterpret_cast<const f32x4*>(from + at);
 #pragma unroll
-        for (int i = 0; i < S::MB; ++i)
+                for (int u = 0; u < 4; ++u) acc[i][j][r + u] = z[u];
+            });
+        }
+    } else {
+        tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
+        if (bias)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
-                const float z = v < p.V ? (float)bias[v] : 0.f;
+            for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-                for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
+                    const float z = v < p.V ? (float)bias[v] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
+                }
+    }
     // through LDS, so that a row's values leave 16 bytes a lane: a wave's 64 rows (tokens) of WM values, chunks changing places by the row
     drain_and_meet();
     constexpr int ROW = S::WM, CH = ROW * (int)sizeof(T) / 16, VEC = Traits<T>::VEC, PER_ARRAY = Stage<T, true, B>::SIZE / (S::WN * ROW);
@@ -828,10 +867,13 @@ int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t 
     });
 }
 
+// The most logits that are kept for the gradient: 512 MB of them
+constexpr int64_t KEPT_FLOATS = (int64_t)1 << 27;
+
 constexpr int REDUCE_ROWS = 16384;            // rows that one workgroup reduces by itself
 
 template <typename T>
-int forward(const Args& a, int reduction, float* loss, float* state, float* dx_unit, bool with_dx, int32_t* oob, char* ws, size_t* need, hipStream_t s)
+int forward(const Args& a, int reduction, float* loss, float* state, float* kept, bool keep, int32_t* oob, char* ws, size_t* need, hipStream_t s)
 {
     Carve c{ws};
     Problem p;
@@ -844,7 +886,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     float* z_target = (float*)c.take((size_t)a.T * 4);
     float* rows = (float*)c.take((size_t)a.T * 4);
     float2* sums = (float2*)c.take(256 * sizeof(float2));
-    float* dx_part = narrow && with_dx ? (float*)c.take((size_t)splits * a.T * a.D * 4) : nullptr;
+    float* dx_part = narrow && keep ? (float*)c.take((size_t)splits * a.T * a.D * 4) : nullptr;
     const int rc = pack_rows<T>(a, p, false, c, launch, s);
     if (rc) return rc;
     *need = c.used;
@@ -857,7 +899,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
         const int rs = with_tile<T>(tile, [&](auto t) -> int {
             constexpr int B = decltype(t)::value;
             hipLaunchKernelGGL((stats_kernel<T, B>), dim3((unsigned)(ceil_div64(a.T, B) * splits)), dim3(Shape<B>::THREADS), 0, s, p, splits, f.tiles_per_split,
-                               part, z_target);
+                               part, z_target, kept);
             return RECO_OK;
         });
         if (rs) return rs;
@@ -865,7 +907,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
     const auto join = [&](auto waves) {
         constexpr int WAVES = decltype(waves)::value;
         hipLaunchKernelGGL((rows_kernel<T, WAVES>), dim3((unsigned)(WAVES > 1 ? a.T : ceil_div64(a.T, 4))), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, s, p, part,
-                           splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D, dx_part ? dx_unit : nullptr);
+                           splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D, dx_part ? kept : nullptr);
     };
     if (splits > 64) join(std::integral_constant<int, 8>());
     else join(std::integral_constant<int, 1>());
@@ -880,7 +922,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* dx_u
 }
 
 template <typename T>
-int backward(const Args& a, int reduction, const float* state, const float* dx_unit, const float* dloss, void* dx, void* dw, void* db, char* ws, size_t* need,
+int backward(const Args& a, int reduction, const float* state, const float* kept, const float* dloss, void* dx, void* dw, void* db, char* ws, size_t* need,
              hipStream_t s)
 {
     Carve c{ws};
@@ -924,15 +966,22 @@ int backward(const Args& a, int reduction, const float* state, const float* dx_u
             const int rn = narrow_cols_of<T>(p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
             if (rn) return rn;
         }
-        if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, dx_unit, a.T, a.D, gn, scale, (T*)dx);
+        if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, kept, a.T, a.D, gn, scale, (T*)dx);
         RECO_CHECK_LAUNCH();
         return RECO_OK;
     }
     for (int64_t v0 = 0; v0 < a.V; v0 += b.width) {
         const int64_t width = a.V - v0 < b.width ? a.V - v0 : b.width, ldg = ceil_div64(width, 256) * 256;
-        int rl = with_tile<T>(tile_of(sizeof(T), a.T, b.width), [&](auto t) -> int {
+        int rl = with_tile<T>(tile_of(sizeof(T), a.T, a.V), [&](auto t) -> int {
             constexpr int B = decltype(t)::value;
-            hipLaunchKernelGGL((g_kernel<T, B>), dim3((unsigned)(ceil_div64(a.T, B) * (ldg / B))), dim3(Shape<B>::THREADS), 0, s, p, v0, lse, rest, gn, G, ldg);
+            const dim3 grid((unsigned)(ceil_div64(a.T, B) * (ldg / B))), block(Shape<B>::THREADS);
+            if constexpr (KEEPS<T>)
+                if (kept) {
+                    hipLaunchKernelGGL((g_kernel<T, B, true>), grid, block, 0, s, p, v0, kept, lse, rest, gn, G, ldg);
+                    RECO_CHECK_LAUNCH();
+                    return RECO_OK;
+                }
+            hipLaunchKernelGGL((g_kernel<T, B, false>), grid, block, 0, s, p, v0, nullptr, lse, rest, gn, G, ldg);
             RECO_CHECK_LAUNCH();
             return RECO_OK;
         });
@@ -965,31 +1014,39 @@ int check_args(const char* what, const Args& a, int reduction)
 }  // namespace
 
 extern "C" size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D,
-                                                   int with_dx)
+                                                   int keep)
 {
     if (T <= 0 || V <= 0 || D <= 0) return 0;
     const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr};
     size_t need = 0;
     (void)reco_with_type(dtype, [&](auto z) -> int {
-        return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, with_dx != 0, nullptr, nullptr, &need, nullptr);
+        return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, keep != 0, nullptr, nullptr, &need, nullptr);
     });
     return need;
 }
 
-extern "C" int64_t reco_linear_xent_dx_floats(int dtype, int64_t T, int64_t D)
+extern "C" int64_t reco_linear_xent_kept_floats(int dtype, int64_t T, int64_t V, int64_t D, int with_dx)
 {
-    return T > 0 && D > 0 && dtype >= RECO_DT_F32 && dtype <= RECO_DT_F16 && narrow_fits(dtype, D) ? T * D : 0;
+    if (dtype < RECO_DT_F32 || dtype > RECO_DT_F16 || T <= 0 || T >= (int64_t)1 << 31 || V <= 0 || V >= (int64_t)1 << 31 || D <= 0) return 0;
+    if (narrow_fits(dtype, D)) return with_dx ? T * D : 0;
+    if (dtype != RECO_DT_F32) return 0;                  // KEEPS
+    const int64_t tile = tile_of(4, T, V);
+    if (ceil_div64(T, tile) > KEPT_FLOATS / (tile * tile)) return 0;
+    const int64_t n = ceil_div64(T, tile) * ceil_div64(V, tile) * tile * tile;
+    return n <= KEPT_FLOATS ? n : 0;
 }
 
 extern "C" int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                                const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, float* dx_unit, int32_t* oob,
+                                const int64_t* target, int64_t ignore, int reduction, float* loss, float* state, float* kept, int32_t* oob,
                                 void* ws, size_t ws_bytes, void* stream)
 {
     const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
     const int rc = check_args("linear_xent", a, reduction);
     if (rc) return rc;
     RECO_REQUIRE(loss && state && ws && (uintptr_t)ws % 16 == 0, "linear_xent: null or misaligned loss, state or workspace");
-    const size_t need = reco_linear_xent_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D, dx_unit != nullptr);
+    RECO_REQUIRE((uintptr_t)kept % 16 == 0, "linear_xent: misaligned room for what is kept");
+    if (reco_linear_xent_kept_floats(dtype, T, V, D, 1) == 0) kept = nullptr;
+    const size_t need = reco_linear_xent_workspace_bytes(x, ldx, w, ldw, dtype, T, V, D, kept != nullptr);
     if (ws_bytes < need) {
         reco_set_error("linear_xent: workspace of %zu bytes, %zu needed", ws_bytes, need);
         return RECO_ENOMEM;
@@ -997,7 +1054,7 @@ extern "C" int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64
     ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
     size_t used = 0;
     return reco_with_type(dtype, [&](auto z) -> int {
-        return forward<decltype(z)>(a, reduction, loss, state, dx_unit, dx_unit != nullptr, oob, (char*)ws, &used, (hipStream_t)stream);
+        return forward<decltype(z)>(a, reduction, loss, state, kept, kept != nullptr, oob, (char*)ws, &used, (hipStream_t)stream);
     });
 }
 
@@ -1013,7 +1070,7 @@ extern "C" size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t l
 }
 
 extern "C" int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int dtype, int64_t T, int64_t V, int64_t D,
-                                     const int64_t* target, int64_t ignore, int reduction, const float* state, const float* dx_unit, const float* dloss,
+                                     const int64_t* target, int64_t ignore, int reduction, const float* state, const float* kept, const float* dloss,
                                      void* dx, void* dw, void* db, void* ws, size_t ws_bytes, void* stream)
 {
     const Args a{x, ldx, w, ldw, bias, dtype, T, V, D, target, ignore};
@@ -1025,11 +1082,13 @@ extern "C" int reco_linear_xent_grad(const void* x, int64_t ldx, const void* w, 
         reco_set_error("linear_xent_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
         return RECO_ENOMEM;
     }
-    RECO_REQUIRE(!dx || dx_unit || !narrow_fits(dtype, D), "linear_xent_grad: dx needs the dx_unit that the forward call wrote");
+    RECO_REQUIRE((uintptr_t)kept % 16 == 0, "linear_xent_grad: what was kept is misaligned");
+    if (reco_linear_xent_kept_floats(dtype, T, V, D, 1) == 0) kept = nullptr;
+    RECO_REQUIRE(!dx || kept || !narrow_fits(dtype, D), "linear_xent_grad: dx needs what the forward call kept");
     if (!dx && !dw && !db) return RECO_OK;
     ProfScope prof((hipStream_t)stream, RECO_PROF_XENT);
     size_t used = 0;
     return reco_with_type(dtype, [&](auto z) -> int {
-        return backward<decltype(z)>(a, reduction, state, dx_unit, dloss, dx, dw, db, (char*)ws, &used, (hipStream_t)stream);
+        return backward<decltype(z)>(a, reduction, state, kept, dloss, dx, dw, db, (char*)ws, &used, (hipStream_t)stream);
     });
 }

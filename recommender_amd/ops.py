@@ -530,16 +530,16 @@ def _xent_args(x, weight, target, bias, reduction, ignore_index):
     return x, weight, target, bias
 
 
-def _xent(x, weight, target, bias, reduction, ignore_index, check_ids, with_dx):
-    """(loss, state) of checked operands; with_dx: a gradient of x will be asked for (state begins with dx_unit, see
-    reco_linear_xent)."""
+def _xent(x, weight, target, bias, reduction, ignore_index, check_ids, keep, with_dx):
+    """(loss, state) of checked operands; keep: gradients will be asked for, with_dx: that of x too (state begins with what is kept for
+    them, see reco_linear_xent)."""
     T, D = x.shape
     dev, dtype, V = x.device, DTYPES[x.dtype], weight.shape[0]
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev)
     if T == 0:
         return loss.fill_(float("nan")) if reduction == "mean" else loss.zero_(), None
     L = _lib.lib()
-    floats = L.reco_linear_xent_dx_floats(dtype, T, D) if with_dx else 0
+    floats = L.reco_linear_xent_kept_floats(dtype, T, V, D, 1 if with_dx else 0) if keep else 0
     state = torch.empty(floats + 3 * T + 1, dtype=torch.float32, device=dev)
     at = state.data_ptr()
     oob = torch.zeros(1, dtype=torch.int32, device=dev) if check_ids else None
@@ -578,7 +578,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, rows, target, reduction, ignore_index, check_ids):
         xr, wr, br = rows
-        loss, state = _xent(xr, wr, target, br, reduction, ignore_index, check_ids, ctx.needs_input_grad[0])
+        loss, state = _xent(xr, wr, target, br, reduction, ignore_index, check_ids, True, ctx.needs_input_grad[0])
         ctx.save_for_backward(xr, wr, target, br, state)
         ctx.args = reduction, ignore_index
         return loss
@@ -610,7 +610,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         _no_captured_graph("linear_cross_entropy", "linear_cross_entropy_grad")
         return _LinearCrossEntropy.apply(x, weight, bias, (xr, wr, br), target, reduction, ignore_index, check_ids)
-    return _xent(xr, wr, target, br, reduction, ignore_index, check_ids, False)[0]
+    return _xent(xr, wr, target, br, reduction, ignore_index, check_ids, False, False)[0]
 
 
 def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ignore_index=-100, grad=None):
@@ -622,7 +622,7 @@ def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ig
         grad = torch.ones(shape, dtype=torch.float32, device=x.device)
     elif not isinstance(grad, torch.Tensor) or grad.dtype != torch.float32 or grad.device != x.device or tuple(grad.shape) != shape:
         raise ValueError("grad must be a float32 tensor of shape %s on %s" % (shape, x.device))
-    loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False, True)
+    loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False, True, True)
     return (loss, *_xent_grad(x, weight, target, bias, state, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
 
 

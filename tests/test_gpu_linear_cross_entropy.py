@@ -384,6 +384,67 @@ def test_gradients_against_differences(T, V, D):
             assert abs((up - down) / (2 * step) - slope) <= T * (size ** 3 * step ** 2 / 6 + 20 * 2.0 ** -20 / (2 * step)), (k, slope)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(70, 900, 129), (1, 5000, 300), (300, 20000, 260)])
+def test_kept_logits_change_no_bit(dtype, T, V, D):
+    """The C entries with and without the room that the forward call may keep its logits in."""
+    from recommender_amd import _lib
+    x, w, t, b = _problem(T, V, D, dtype, True, 5)
+    L, ops = _lib.lib(), _ops()
+    dt, s = ops.DTYPES[dtype], torch.cuda.current_stream().cuda_stream
+    what = (x.data_ptr(), D, w.data_ptr(), D)
+    floats = L.reco_linear_xent_kept_floats(dt, T, V, D, 1)
+    assert (floats > 0) == (dtype == torch.float32 or D <= 256)
+    got = []
+    for keep in ([True, False] if D > 256 or dtype == torch.float32 else [True]):
+        kept = torch.full((floats,), math.nan, device="cuda") if keep and floats else None
+        state, loss, one = torch.empty(3 * T + 1, device="cuda"), torch.empty((), device="cuda"), torch.ones((), device="cuda")
+        out = [torch.full((n,), math.nan, dtype=dtype, device="cuda") for n in (T * D, V * D, V)]
+        ws = torch.empty(max(L.reco_linear_xent_workspace_bytes(*what, dt, T, V, D, int(keep)), L.reco_linear_xent_grad_workspace_bytes(*what, dt, T, V, D)),
+                         dtype=torch.uint8, device="cuda")
+        at = None if kept is None else kept.data_ptr()
+        _lib.check(L.reco_linear_xent(*what, b.data_ptr(), dt, T, V, D, t.data_ptr(), -100, _lib.XENT_MEAN, loss.data_ptr(), state.data_ptr(), at, None,
+                                      ws.data_ptr(), ws.numel(), s))
+        for _ in range(2):                                    # what is kept serves more than one gradient call
+            _lib.check(L.reco_linear_xent_grad(*what, b.data_ptr(), dt, T, V, D, t.data_ptr(), -100, _lib.XENT_MEAN, state.data_ptr(), at, one.data_ptr(),
+                                               *(o.data_ptr() for o in out), ws.data_ptr(), ws.numel(), s))
+            got.append([loss.clone()] + [o.clone() for o in out])
+    for other in got[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(got[0], other)), "other bits"
+    auto = ops.linear_cross_entropy_grad(x, w, t, b)
+    assert all(torch.equal(p.view(-1), q.view(-1)) for p, q in zip(got[0], auto))
+
+
+@pytest.mark.parametrize("T,V,D", [(1, 9001, 65), (31, 40000, 128), (32, 700, 100), (33, 700, 100), (5, 3, 128)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_few_rows_in_32_bits(T, V, D, bias):
+    x, w, target, b = _problem(T, V, D, torch.float32, bias, masked=0.1)
+    _check(x, w, target, b, "mean")
+
+
+def test_outputs_of_any_alignment():
+    """The C entries write rows to where they are asked to: 2 bytes off every wider access."""
+    from recommender_amd import _lib
+    for dtype, T, V, D in ((torch.bfloat16, 40, 500, 64), (torch.float32, 40, 500, 64), (torch.float16, 300, 700, 320)):
+        x, w, t, b = _problem(T, V, D, dtype, True, 6)
+        L, ops = _lib.lib(), _ops()
+        dt, s = ops.DTYPES[dtype], torch.cuda.current_stream().cuda_stream
+        want = ops.linear_cross_entropy_grad(x, w, t, b)
+        what = (x.data_ptr(), D, w.data_ptr(), D)
+        floats = L.reco_linear_xent_kept_floats(dt, T, V, D, 1)
+        kept, state, loss, one = torch.empty(floats, device="cuda"), torch.empty(3 * T + 1, device="cuda"), torch.empty((), device="cuda"), torch.ones((), device="cuda")
+        ws = torch.empty(max(L.reco_linear_xent_workspace_bytes(*what, dt, T, V, D, 1), L.reco_linear_xent_grad_workspace_bytes(*what, dt, T, V, D)),
+                         dtype=torch.uint8, device="cuda")
+        out = [torch.zeros(n + 2, dtype=dtype, device="cuda") for n in (T * D, V * D, V)]
+        at = kept.data_ptr() if floats else None
+        _lib.check(L.reco_linear_xent(*what, b.data_ptr(), dt, T, V, D, t.data_ptr(), -100, _lib.XENT_MEAN, loss.data_ptr(), state.data_ptr(), at, None,
+                                      ws.data_ptr(), ws.numel(), s))
+        _lib.check(L.reco_linear_xent_grad(*what, b.data_ptr(), dt, T, V, D, t.data_ptr(), -100, _lib.XENT_MEAN, state.data_ptr(), at, one.data_ptr(),
+                                           *(o[1:].data_ptr() for o in out), ws.data_ptr(), ws.numel(), s))
+        for o, e in zip(out, want[1:]):
+            assert torch.equal(o[1:-1], e.view(-1)) and o[0] == 0 and o[-1] == 0
+
+
 def test_two_streams_at_once():
     ops = _ops()
     a, b = _problem(300, 900, 64, torch.bfloat16, True, 1), _problem(300, 900, 64, torch.bfloat16, True, 2)

@@ -61,3 +61,19 @@ def test_workspace_does_not_hold_the_logits():
     aligned = L.reco_linear_xent_workspace_bytes(some, D, some, D, 1, T, V, D, 0)
     assert L.reco_linear_xent_workspace_bytes(ctypes.c_void_p(258), D, some, D, 1, T, V, D, 0) >= aligned + 2 * T * D       # a copy of x
     assert L.reco_linear_xent_workspace_bytes(some, D, some, D + 1, 1, T, V, D, 0) >= aligned + 2 * V * D                  # a copy of w
+
+
+def test_what_is_kept_for_the_gradient():
+    from recommender_amd import _lib
+    kept = _lib.lib().reco_linear_xent_kept_floats
+    assert kept(0, 70, 900, 128, 1) == 70 * 128 and kept(0, 70, 900, 128, 0) == 0                 # narrow rows: dx
+    assert kept(1, 70, 900, 256, 1) == 70 * 256
+    assert kept(0, 70, 900, 129, 1) == kept(0, 70, 900, 129, 0) == 128 * 1024                     # the logits, in whole tiles
+    assert kept(1, 70, 900, 257, 1) == kept(2, 70, 900, 600, 1) == 0
+    assert kept(0, 16384, 8192, 300, 1) == 2 ** 27 and kept(0, 16384, 8193, 300, 1) == kept(0, 16385, 8192, 300, 1) == 0
+    assert kept(0, 2 ** 31 - 1, 2 ** 31 - 1, 300, 1) == 0 and kept(3, 70, 900, 8, 1) == kept(0, 0, 900, 8, 1) == 0
+    some = ctypes.c_void_p(256)
+    assert _lib.lib().reco_linear_xent(some, 200, some, 200, None, 0, 4, 9, 200, some, -100, 1, some, some, ctypes.c_void_p(264), None, some, 1 << 30,
+                                       None) == _lib.EINVAL
+    assert _lib.lib().reco_linear_xent_grad(some, 200, some, 200, None, 0, 4, 9, 200, some, -100, 1, some, ctypes.c_void_p(264), some, some, some, None, some,
+                                            1 << 30, None) == _lib.EINVAL
