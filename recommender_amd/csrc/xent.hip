@@ -232,6 +232,65 @@ __device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, c
     } while (left > 0);
 }
 
+// acc: logits of vocabulary rows v0 .. (32 per i) and 32 tokens per j, plus the rows' bias
+template <typename T, int MB, int NB> __device__ __forceinline__ void add_bias(const Problem& p, f32x16 (&acc)[MB][NB], int64_t v0)
+{
+    const T* bias = (const T*)p.bias;
+    const int half = threadIdx.x >> 5 & 1;
+    if (bias)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t v = v0 + 32 * i + acc_row(r, half);
+                const float z = v < p.V ? (float)bias[v] : 0.f;
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j][r] += z;
+            }
+}
+
+// The block's logits go into this lane's running maxima and sums, the targets' into z_target.  t0: this lane's first token
+template <int MB, int NB>
+__device__ __forceinline__ void fold(const Problem& p, f32x16 (&acc)[MB][NB], int64_t v0, int64_t t0, const int64_t (&y)[NB], Running (&run)[NB],
+                                     float* __restrict__ z_target)
+{
+    const int half = threadIdx.x >> 5 & 1;
+    const bool tail = v0 + 32 * MB > p.V;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int64_t here = y[j] - v0;
+        if (tail || __any(here >= 0 && here < 32 * MB)) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t v = v0 + 32 * i + acc_row(r, half);
+                    if (v == y[j]) z_target[t0 + 32 * j] = acc[i][j][r];
+                    if (v == y[j] || v >= p.V) acc[i][j][r] = -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+        const float m = fmaxf(run[j].m, top), base = m == -INFINITY ? 0.f : m;
+        float s = run[j].s * exp2f((run[j].m - base) * LOG2E);
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
+        run[j] = Running{m, s};
+    }
+}
+
+// Both halves of a wave hold sums of the same 32 columns
+__device__ __forceinline__ Running halves_joined(const Running& mine)
+{
+    const Running o{__shfl_xor(mine.m, 32, 64), __shfl_xor(mine.s, 32, 64)};
+    return threadIdx.x & 32 ? joined(o, mine) : joined(mine, o);
+}
+
 template <typename T, int B>
 __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, int64_t splits, int64_t tiles_per_split, Running* __restrict__ part,
                                                                      float* __restrict__ z_target, float* __restrict__ kept)
@@ -241,7 +300,6 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
     pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, splits, token_tile, split);
     TILE_LDS(T, true, true, B);
     const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
-    const T* bias = (const T*)p.bias;
     const int64_t n0 = token_tile * B;
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     int64_t y[S::NB];
@@ -259,62 +317,263 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
     for (int64_t m0 = first; m0 < end; m0 += B) {
         Acc<B> acc = {};
         tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
-        if (bias)
-#pragma unroll
-            for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
-                    const float z = v < p.V ? (float)bias[v] : 0.f;
-#pragma unroll
-                    for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
-                }
+        add_bias<T>(p, acc, m0 + wm);
         if (KEEPS<T> && kept) {
             float* to = kept + kept_at<B>(token_tile, (p.V + B - 1) / B, m0 / B);
             each_kept<B>([&](int i, int j, int r, int at) {
                 *reinterpret_cast<f32x4*>(to + at) = f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
             });
         }
-        const bool tail = m0 + B > p.V;
-#pragma unroll
-        for (int j = 0; j < S::NB; ++j) {
-            const int64_t t = n0 + wn + 32 * j + (lane & 31);
-            const int64_t here = y[j] - m0;
-            if (tail || __any(here >= 0 && here < B)) {
-#pragma unroll
-                for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
-                        if (v == y[j]) z_target[t] = acc[i][j][r];
-                        if (v == y[j] || v >= p.V) acc[i][j][r] = -INFINITY;
-                    }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
-            const float m = fmaxf(run[j].m, top), base = m == -INFINITY ? 0.f : m;
-            float s = run[j].s * exp2f((run[j].m - base) * LOG2E);
-#pragma unroll
-            for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
-            run[j] = Running{m, s};
-        }
+        fold(p, acc, m0 + wm, n0 + wn + (lane & 31), y, run, z_target);
     }
     __syncthreads();
     Running* sh = reinterpret_cast<Running*>(lds_a0);              // [2 waves along the vocabulary][B tokens]
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
-        const Running o{__shfl_xor(run[j].m, 32, 64), __shfl_xor(run[j].s, 32, 64)};
-        const Running both = half ? joined(o, run[j]) : joined(run[j], o);
+        const Running both = halves_joined(run[j]);
         if (half == 0) sh[(wm ? B : 0) + wn + 32 * j + lane] = both;
     }
     __syncthreads();
     const int64_t t = n0 + threadIdx.x;
     if (threadIdx.x < B && t < p.T) part[split * p.T + t] = joined(sh[threadIdx.x], sh[B + threadIdx.x]);
+}
+
+// The statistics of up to 64 rows (tokens): a tile of 128 would multiply mostly padding, and the one large operand is read once whatever is
+// done.  A wave takes 64 vocabulary rows at a time, its operands straight from memory, two chunks of 128 bytes a row under way: lane l
+// reads 64 consecutive bytes of row l % 32, the first or the second half of the chunk, for either operand -- the order of k is free --
+// so every line is read whole.  No alignment is asked for and nothing is copied: the last pieces of a row are read from where the row
+// ends, and what the piece before has had of them is cleared, in both operands.
+template <typename T, int NB, int MB, int BYTES, int WAVES>
+__global__ __launch_bounds__(64, WAVES) void few_kernel(Problem p, int64_t per, Running* __restrict__ part, float* __restrict__ z_target, float* __restrict__ kept)
+{
+    constexpr int ROWS = 32 * MB, VEC = Traits<T>::VEC, KC = BYTES / (int)sizeof(T), PIECES = KC / 2 / VEC;
+    typedef typename Traits<T>::frag frag;
+    typedef frag loose __attribute__((aligned(sizeof(T))));
+    const int lane = threadIdx.x, l31 = lane & 31, half = lane >> 5, D = (int)p.D;
+    const int64_t blocks = (p.V + ROWS - 1) / ROWS, b0 = blockIdx.x * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+    const int last = D - VEC, chunks = (D + 2 * KC - 1) / (2 * KC) * 2;
+    const T *wp[MB], *xp[NB];
+    int64_t y[NB];
+    Running run[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int64_t t = 32 * j + l31;
+        xp[j] = (const T*)p.x + (t < p.T ? t : p.T - 1) * p.ldx;
+        y[j] = t < p.T && p.target[t] != p.ignore ? clamp_target(p.target[t], p.V) : -1;
+        run[j] = Running{-INFINITY, 0.f};
+    }
+    struct Chunk { frag w[MB][PIECES], x[NB][PIECES]; } a, b;
+    auto rows = [&](int64_t block) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            const int64_t v = block * ROWS + 32 * i + l31;
+            wp[i] = (const T*)p.w + (v < p.V ? v : p.V - 1) * p.ldw;
+        }
+    };
+    auto load = [&](Chunk& c, int chunk) {
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            const int k = chunk * KC + half * (KC / 2) + n * VEC, at = k < last ? k : last;
+#pragma unroll
+            for (int i = 0; i < MB; ++i) c.w[i][n] = *reinterpret_cast<const loose*>(wp[i] + at);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) c.x[j][n] = *reinterpret_cast<const loose*>(xp[j] + at);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x16 acc[MB][NB];
+    auto multiply = [&](Chunk& c, int chunk) {
+        if ((chunk + 1) * KC > D)
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n) {
+                const int k = chunk * KC + half * (KC / 2) + n * VEC, had = k - (k < last ? k : last);
+#pragma unroll
+                for (int u = 0; u < VEC; ++u) {
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) c.w[i][n][u] = u < had ? (T)0.f : c.w[i][n][u];
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) c.x[j][n][u] = u < had ? (T)0.f : c.x[j][n][u];
+                }
+            }
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n)
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+#pragma unroll
+                        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(c.w[i][n][u], c.x[j][n][u], acc[i][j], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) mma(acc[i][j], c.w[i][n], c.x[j][n]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    rows(b0);
+    load(a, 0);
+#pragma unroll 1
+    for (int64_t block = b0; block < b1; ++block) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = f32x16{};
+#pragma unroll 1
+        for (int c = 0; c < chunks; c += 2) {
+            load(b, c + 1);
+            multiply(a, c);
+            if (c + 2 == chunks) rows(block + 1);              // behind the last block: the last row, read for nothing
+            load(a, c + 2 == chunks ? 0 : c + 2);
+            multiply(b, c + 1);
+        }
+        add_bias<T>(p, acc, block * ROWS);
+        if (KEEPS<T> && kept) {                                // as kept_at lays out tiles of 128
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                const int64_t v = block * ROWS + 32 * i;
+                float* to = kept + v / 64 * (2 * 64 * 64) + (v & 32) / 32 * (2 * 4 * 256) + lane * 4;
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        *reinterpret_cast<f32x4*>(to + (j * 4 + r / 4) * 256) = f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
+            }
+        }
+        fold(p, acc, block * ROWS, l31, y, run, z_target);
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const Running both = halves_joined(run[j]);
+        if (half == 0 && 32 * j + l31 < p.T) part[blockIdx.x * p.T + 32 * j + l31] = both;
+    }
+}
+
+// The statistics of up to four rows (tokens): nothing to multiply but the memory's stream.  A wave takes eight vocabulary rows at a time, 64
+// lanes beside each other in a row, so that whole lines are read whatever the alignment is (32 rows at 128 bytes, as above, reach 2.6
+// TB/s with rows off the lines); each lane adds its products of the rows, and the lanes' sums are added so that the number of values halves
+// with each of the first three exchanges: lane l ends with row l % 8.
+template <typename T, int NT>
+__global__ __launch_bounds__(64, (NT == 1 && sizeof(T) == 4 ? 4 : NT <= 2 ? 3 : 2)) void dot_kernel(Problem p, int64_t per, Running* __restrict__ part, float* __restrict__ z_target,
+                                                                 float* __restrict__ kept)
+{
+    constexpr int ROWS = 8, VEC = Traits<T>::VEC, STEP = 64 * VEC;
+    typedef typename Traits<T>::frag frag;
+    typedef frag loose __attribute__((aligned(sizeof(T))));
+    const int lane = threadIdx.x, D = (int)p.D, last = D - VEC, steps = (D + STEP - 1) / STEP;
+    const int64_t blocks = (p.V + ROWS - 1) / ROWS, b0 = blockIdx.x * per, b1 = b0 + per < blocks ? b0 + per : blocks;
+    const T* bias = (const T*)p.bias;
+    const T *wp[ROWS], *xp[NT];
+    int64_t y[NT];
+    Running run[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t t = j < p.T ? j : p.T - 1;
+        xp[j] = (const T*)p.x + t * p.ldx;
+        y[j] = p.target[t] != p.ignore ? clamp_target(p.target[t], p.V) : -1;
+        run[j] = Running{-INFINITY, 0.f};
+    }
+    frag a[ROWS], b[ROWS];
+    auto rows = [&](int64_t block) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t v = block * ROWS + i;
+            wp[i] = (const T*)p.w + (v < p.V ? v : p.V - 1) * p.ldw;
+        }
+    };
+    auto load = [&](frag (&c)[ROWS], int step) {
+        const int k = step * STEP + lane * VEC, at = k < last ? k : last;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) c[i] = *reinterpret_cast<const loose*>(wp[i] + at);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    float acc[NT][ROWS];
+    auto multiply = [&](frag (&c)[ROWS], int step) {
+        // the last pieces of a row are read from where it ends: what the piece before has had of them is cleared, in both operands
+        const int k = step * STEP + lane * VEC, at = k < last ? k : last, had = k - at;
+        frag x[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j] = *reinterpret_cast<const loose*>(xp[j] + at);
+        if ((step + 1) * STEP > D)
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) {
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) c[i][u] = u < had ? (T)0.f : c[i][u];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) x[j][u] = u < had ? (T)0.f : x[j][u];
+            }
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) acc[j][i] = fmaf((float)c[i][u], (float)x[j][u], acc[j][i]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    rows(b0);
+    load(a, 0);
+#pragma unroll 1
+    for (int64_t block = b0; block < b1; ++block) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) acc[j][i] = 0.f;
+        auto step = [&](frag (&now)[ROWS], frag (&next)[ROWS], int s) {
+            if (s + 1 == steps) rows(block + 1);               // behind the last block: the last row, read for nothing
+            load(next, s + 1 == steps ? 0 : s + 1);
+            multiply(now, s);
+        };
+        int s = 0;
+#pragma unroll 1
+        for (; s + 2 <= steps; s += 2) {
+            step(a, b, s);
+            step(b, a, s + 1);
+        }
+        if (s < steps) {
+            step(a, b, s);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) a[i] = b[i];
+        }
+        const int64_t v = block * ROWS + (lane & 7);
+        const float more = bias && v < p.V ? (float)bias[v] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float mine = lane & 4 ? acc[j][i + 4] : acc[j][i], other = lane & 4 ? acc[j][i] : acc[j][i + 4];
+                f[i] = mine + __shfl_xor(other, 4, 64);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float mine = lane & 2 ? f[i + 2] : f[i], other = lane & 2 ? f[i] : f[i + 2];
+                f[i] = mine + __shfl_xor(other, 2, 64);
+            }
+            const float mine = lane & 1 ? f[1] : f[0], other = lane & 1 ? f[0] : f[1];
+            float z = mine + __shfl_xor(other, 1, 64);
+#pragma unroll
+            for (int d = 8; d < 64; d <<= 1) z += __shfl_xor(z, d, 64);
+            z += more;
+            if (lane < ROWS && j < p.T && v < p.V) {
+                if (KEEPS<T> && kept) {                        // as kept_at lays out tiles of 128
+                    const int in = (int)(v & 31);
+                    kept[v / 64 * (2 * 64 * 64) + (v & 32) / 32 * (2 * 4 * 256) + in / 8 * 256 + ((in & 4) * 8 + j) * 4 + (in & 3)] = z;
+                }
+                if (v == y[j]) z_target[j] = z;
+                else run[j] = joined(run[j], Running{z, 1.f});
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int d = 1; d < ROWS; d <<= 1) {
+            const Running o{__shfl_xor(run[j].m, d, 64), __shfl_xor(run[j].s, d, 64)};
+            run[j] = lane & d ? joined(o, run[j]) : joined(run[j], o);
+        }
+        if (lane == 0 && j < p.T) part[blockIdx.x * p.T + j] = run[j];
+    }
 }
 
 // WAVES waves per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
@@ -526,7 +785,6 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
     pair_of(place_of(blockIdx.x, gridDim.x), (p.T + B - 1) / B, ldg / B, token_tile, panel);
     TILE_LDS(T, true, true, B);
     const Operand<T> W{(const T*)p.w, p.ldw, p.V}, X{(const T*)p.x, p.ldx, p.T};
-    const T* bias = (const T*)p.bias;
     const int64_t n0 = token_tile * B, m0 = v0 + panel * B;
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     Acc<B> acc = {};
@@ -541,16 +799,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
         }
     } else {
         tile_product<T, true, true, B>(acc, W, X, m0, n0, 0, p.D, TILE_LDS_ARGS);
-        if (bias)
-#pragma unroll
-            for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int64_t v = m0 + wm + 32 * i + acc_row(r, half);
-                    const float z = v < p.V ? (float)bias[v] : 0.f;
-#pragma unroll
-                    for (int j = 0; j < S::NB; ++j) acc[i][j][r] += z;
-                }
+        add_bias<T>(p, acc, m0 + wm);
     }
     // through LDS, so that a row's values leave 16 bytes a lane: a wave's 64 rows (tokens) of WM values, chunks changing places by the row
     drain_and_meet();
@@ -870,6 +1119,34 @@ int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t 
 // The most logits that are kept for the gradient: 512 MB of them
 constexpr int64_t KEPT_FLOATS = (int64_t)1 << 27;
 
+// The forms for few rows (dot_kernel, few_kernel): vocabulary rows a wave takes at a time, how often, and the waves
+struct FewPlan {
+    int64_t rows, per, splits;
+};
+
+FewPlan few_plan(int64_t T, int64_t V, int64_t D, int size)
+{
+    // dot_kernel where a row keeps enough of the lanes beside each other at work.  With 33 tokens or more, 128 vocabulary rows read x half
+    // as often as 64, once there are enough of them for the chip's 1024 places (64 x 131,071 x 1024 f32: 205 us, 256 with 64; at 65,536
+    // 142, 97)
+    const int64_t pieces = D * size / 16;
+    const bool dot = T == 1 ? pieces >= 32 || size == 4 : T <= 4 && pieces >= (size == 4 ? 48 : 96);
+    const int64_t rows = dot ? 8 : T <= 32 || V < 128 * 960 ? 64 : 128;
+    const int64_t waves = 1024 * (rows == 128 ? 1 : rows == 64 ? 3 : T == 1 && size == 4 ? 4 : T <= 2 ? 3 : 2);
+    const int64_t blocks = ceil_div64(V, rows), per = ceil_div64(blocks, waves);
+    return FewPlan{rows, per, ceil_div64(blocks, per)};
+}
+
+// Where rows are wide.  Narrow ones that leave nothing for the gradient: where the narrow form would copy W first; in 32 bits a single
+// token (1 x 1 M: x 64 84 us instead of 102, x 128 130 instead of 160) and 33 to 64, of which the narrow form keeps half its waves at
+// work (64 x 1 M x 100: 255 us instead of 338; 64 x 50,000 x 128 35 both).
+bool is_few(const Args& a, bool narrow, bool keep)
+{
+    const int size = a.dtype == RECO_DT_F32 ? 4 : 2;
+    if (a.T > 64 || a.D * size < 16) return false;
+    return !narrow || (!keep && (must_pack(a.w, a.ldw, a.D, size) || (size == 4 && a.D > 32 && (a.T == 1 || a.T > 32))));
+}
+
 constexpr int REDUCE_ROWS = 16384;            // rows that one workgroup reduces by itself
 
 template <typename T>
@@ -881,18 +1158,33 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* kept
     const int tile = tile_of(sizeof(T), a.T, a.V);
     const ForwardPlan f = forward_plan(a.T, a.V, tile);
     const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
-    const int64_t splits = narrow ? n.x_splits : f.splits;
+    const bool few = is_few(a, narrow, keep);
+    const FewPlan fp = few_plan(a.T, a.V, a.D, sizeof(T));
+    const int64_t splits = few ? fp.splits : narrow ? n.x_splits : f.splits;
     Running* part = (Running*)c.take((size_t)splits * a.T * sizeof(Running));
     float* z_target = (float*)c.take((size_t)a.T * 4);
     float* rows = (float*)c.take((size_t)a.T * 4);
     float2* sums = (float2*)c.take(256 * sizeof(float2));
     float* dx_part = narrow && keep ? (float*)c.take((size_t)splits * a.T * a.D * 4) : nullptr;
-    const int rc = pack_rows<T>(a, p, false, c, launch, s);
-    if (rc) return rc;
+    if (few) {
+        p = Problem{a.T, a.V, a.D, a.ldx, a.ldw, a.x, a.w, a.bias, a.target, a.ignore};
+    } else {
+        const int rc = pack_rows<T>(a, p, false, c, launch, s);
+        if (rc) return rc;
+    }
     *need = c.used;
     if (!launch) return RECO_OK;
     if (reduction == REDUCE_NONE) rows = loss;
-    if (narrow) {
+    if (few) {
+        const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)splits), dim3(64), 0, s, p, fp.per, part, z_target, kept); };
+        if (fp.rows == 8) {
+            if (a.T == 1) launch(dot_kernel<T, 1>);
+            else if (a.T == 2) launch(dot_kernel<T, 2>);
+            else launch(dot_kernel<T, 4>);
+        } else if (a.T <= 32) launch(few_kernel<T, 1, 2, 64, 3>);
+        else if (fp.rows == 64) launch(few_kernel<T, 2, 2, 64, 3>);
+        else launch(few_kernel<T, 2, 4, 128, 1>);
+    } else if (narrow) {
         const int rn = narrow_rows_of<T>(p, n, a.D, part, z_target, dx_part, s);
         if (rn) return rn;
     } else {

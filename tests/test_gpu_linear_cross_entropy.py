@@ -385,7 +385,7 @@ def test_gradients_against_differences(T, V, D):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,V,D", [(70, 900, 129), (1, 5000, 300), (300, 20000, 260)])
+@pytest.mark.parametrize("T,V,D", [(70, 900, 129), (65, 5000, 300), (300, 20000, 260)])
 def test_kept_logits_change_no_bit(dtype, T, V, D):
     """The C entries with and without the room that the forward call may keep its logits in."""
     from recommender_amd import _lib
@@ -420,6 +420,32 @@ def test_kept_logits_change_no_bit(dtype, T, V, D):
 def test_few_rows_in_32_bits(T, V, D, bias):
     x, w, target, b = _problem(T, V, D, torch.float32, bias, masked=0.1)
     _check(x, w, target, b, "mean")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 1, 300), (1, 7, 129), (2, 9, 1001), (3, 4099, 640), (4, 700, 257), (5, 63, 300), (31, 65, 700), (32, 130, 2000), (33, 64, 513),
+                                   (50, 5003, 300), (64, 129, 1024), (64, 3000, 260), (40, 123001, 264), (1, 40000, 9), (1, 5000, 65), (64, 30001, 40),
+                                   (1, 20000, 2049), (4, 9001, 1000)])
+def test_few_rows(dtype, T, V, D):
+    x, w, target, b = _problem(T, V, D, dtype, True, masked=0.05)
+    _check(x, w, target, b, "none", g=torch.linspace(-2.0, 2.0, T, device="cuda"), what="few")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,D", [(1, 301), (2, 999), (3, 260), (20, 77), (33, 263), (64, 515)])
+def test_few_rows_off_every_alignment(dtype, T, D):
+    """Rows that begin anywhere, among others whose values must not be read into them."""
+    x, w, target, b = _problem(T, 1500, D, dtype, True)
+    wide_x, wide_w = torch.full((T, D + 5), math.nan, dtype=dtype, device="cuda"), torch.full((1500, D + 3), math.inf, dtype=dtype, device="cuda")
+    for wide, like in ((wide_x, x), (wide_w, w)):
+        wide[:, 1:D + 1] = like
+    x, w = wide_x[:, 1:D + 1], wide_w[:, 1:D + 1]
+    want = Exact(x, w, target, b, "none", -100)
+    _close(_ops().linear_cross_entropy(x, w, target, b, "none"), want.loss, want.loss_tol, "loss")
+    if T > 1:
+        x[1, 0] = math.nan
+        loss = _ops().linear_cross_entropy(x, w, target, b, "none")
+        assert bool(loss[1].isnan()) and int(loss.isnan().sum()) == 1
 
 
 def test_outputs_of_any_alignment():
