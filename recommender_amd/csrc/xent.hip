@@ -581,16 +581,13 @@ __global__ __launch_bounds__(64, (NT == 1 && sizeof(T) == 4 ? 4 : NT <= 2 ? 3 : 
 // what it waits for is memory: with one wave to a row, 505 splits of 16 rows x 128 took 40 to 72 us, with eight 15; up to 64 splits the
 // further waves only cost (6038 rows x 32: 11 us with one, 25 with four; 8192 x 128: 15, 34).
 template <typename T, int WAVES>
-__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits,
-                                                                            const float* __restrict__ z_target, float* __restrict__ loss,
-                                                                            float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
-                                                                            const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
+__device__ __forceinline__ void one_row(const Problem& p, int64_t t, const Running* __restrict__ part, int64_t splits, const float* __restrict__ z_target,
+                                        float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
+                                        const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
 {
     __shared__ Running runs[WAVES];
     __shared__ float sums[WAVES > 1 ? WAVES : 1][WAVES > 1 ? 256 : 1];
     const int lane = threadIdx.x & 63, wave = WAVES > 1 ? threadIdx.x >> 6 : 0;
-    const int64_t t = WAVES > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= p.T) return;
     const int64_t y = p.target[t];
     if (y == p.ignore) {
         if (wave) return;
@@ -666,6 +663,21 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void rows_kernel(Prob
     for (int k = 0; k < 4; ++k) {
         const int c = 64 * k + lane;
         if (c < D_out) dx_unit[t * D_out + c] = none ? NAN : fmaf(-q, (float)w[c], total[k] / sum);
+    }
+}
+
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void rows_kernel(Problem p, const Running* __restrict__ part, int64_t splits,
+                                                                            const float* __restrict__ z_target, float* __restrict__ loss,
+                                                                            float* __restrict__ lse, float* __restrict__ rest, int32_t* oob,
+                                                                            const float* __restrict__ dx_part, int64_t D_out, float* __restrict__ dx_unit)
+{
+    if constexpr (WAVES > 1) {
+        one_row<T, WAVES>(p, blockIdx.x, part, splits, z_target, loss, lse, rest, oob, dx_part, D_out, dx_unit);
+    } else {
+#pragma unroll 1
+        for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < p.T; t += (int64_t)gridDim.x * 4)
+            one_row<T, 1>(p, t, part, splits, z_target, loss, lse, rest, oob, dx_part, D_out, dx_unit);
     }
 }
 
@@ -1198,7 +1210,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* kept
     }
     const auto join = [&](auto waves) {
         constexpr int WAVES = decltype(waves)::value;
-        hipLaunchKernelGGL((rows_kernel<T, WAVES>), dim3((unsigned)(WAVES > 1 ? a.T : ceil_div64(a.T, 4))), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, s, p, part,
+        hipLaunchKernelGGL((rows_kernel<T, WAVES>), dim3((unsigned)(WAVES > 1 ? a.T : clamp64(ceil_div64(a.T, 4), 1, 1 << 20))), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, s, p, part,
                            splits, z_target, rows, state, state + 2 * a.T, oob, dx_part, a.D, dx_part ? kept : nullptr);
     };
     if (splits > 64) join(std::integral_constant<int, 8>());
@@ -1236,8 +1248,12 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
         }
     } else {
         G = (T*)c.take((size_t)a.T * b.width * sizeof(T));
-        const size_t xf = product_plan(sizeof(T), a.T, a.D, b.width).floats, wf = product_plan(sizeof(T), b.width, a.D, a.T).floats;
-        w_part = (float*)c.take((xf > wf ? xf : wf) * 4);
+        // the last piece may be narrower, and fewer units can mean shorter shares and more workgroups
+        size_t places = 0;
+        for (const int64_t width : {b.width < a.V ? b.width : a.V, (a.V - 1) % b.width + 1})
+            for (const ProductPlan& q : {product_plan(sizeof(T), a.T, a.D, width), product_plan(sizeof(T), width, a.D, a.T)})
+                if (q.floats > places) places = q.floats;
+        w_part = (float*)c.take(places * 4);
         if (b.width < a.V) x_part = (float*)c.take((size_t)a.T * a.D * 4);
         b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
     }

@@ -5,6 +5,7 @@ product path.  torch is used for allocation (torch.empty), streams and device gu
 """
 import contextlib
 import ctypes
+import operator
 import os
 
 import torch
@@ -155,9 +156,10 @@ def _padding(padding_idx, rows):
     """nn.Embedding's rule: an index into the table, negative ones from its end; -1 for none."""
     if padding_idx is None:
         return -1
+    padding_idx = operator.index(padding_idx)
     if not -rows <= padding_idx < rows:
         raise ValueError("padding_idx must be within the %d rows of the table, got %d" % (rows, padding_idx))
-    return int(padding_idx) % rows
+    return padding_idx % rows
 
 
 def _no_captured_graph(what, instead):
@@ -245,7 +247,7 @@ def embedding_grad(ids, grad, rows, scale=1.0, padding_idx=None):
 
     ids: integers of any shape, clamped to the table; grad: ids' shape + [dim].  May be captured into a HIP graph.
     """
-    scale, rows = _number(scale, "scale"), int(rows)
+    scale, rows = _number(scale, "scale"), operator.index(rows)
     if isinstance(grad, torch.Tensor) and grad.dim() != 2 and grad.dim() > 0:
         grad = grad.reshape(-1, grad.shape[-1]) if grad.numel() else grad.new_empty((0, grad.shape[-1]))
     grad = _rows(grad, "grad")

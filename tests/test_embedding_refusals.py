@@ -59,3 +59,13 @@ def test_workspace_holds_both_lists_and_the_partial_rows(n, rows, dim):
     from recommender_amd import _lib
     got = _lib.lib().reco_embedding_grad_workspace_bytes(n, rows, dim)
     assert got >= 8 * n + 2 * 4 * dim * (n // 128)
+
+
+def test_whole_numbers_are_asked_for():
+    from recommender_amd import ops
+    for bad in (1.0, 0.5, "1", torch.tensor([1, 2])):
+        with pytest.raises(TypeError):
+            ops._padding(bad, 4)
+    assert ops._padding(torch.tensor(3), 4) == 3
+    with pytest.raises(TypeError):
+        ops.embedding_grad(torch.zeros(2, dtype=torch.int64), torch.zeros(2, 3), 4.5)

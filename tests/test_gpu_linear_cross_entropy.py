@@ -448,6 +448,24 @@ def test_few_rows_off_every_alignment(dtype, T, D):
         assert bool(loss[1].isnan()) and int(loss.isnan().sum()) == 1
 
 
+def test_more_rows_than_a_launch_has_waves():
+    T, V, D = 2 ** 26 + 37, 3, 8
+    w = torch.randn(V, D, device="cuda").bfloat16()
+    x = torch.empty(T, D, dtype=torch.bfloat16, device="cuda").normal_()
+    target = torch.randint(0, V, (T,), device="cuda")
+    loss, dx, _, _ = _ops().linear_cross_entropy_grad(x, w, target, reduction="none")
+    for at in (slice(0, 500), slice(T // 2, T // 2 + 500), slice(T - 500, T)):
+        want = Exact(x[at], w, target[at], None, "none", -100)
+        _close(loss[at], want.loss, want.loss_tol, "loss")
+        _close(dx[at], want.dx, want.dx_tol, "dx")
+
+
+@pytest.mark.parametrize("dtype,T,V,D", [(torch.float32, 7296, 600, 384), (torch.float32, 3648, 1100, 300), (torch.bfloat16, 9000, 16000, 520)])
+def test_pieces_of_uneven_width(dtype, T, V, D):
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    _check(x, w, target, b, "mean")
+
+
 def test_outputs_of_any_alignment():
     """The C entries write rows to where they are asked to: 2 bytes off every wider access."""
     from recommender_amd import _lib

@@ -77,3 +77,13 @@ def test_what_is_kept_for_the_gradient():
                                        None) == _lib.EINVAL
     assert _lib.lib().reco_linear_xent_grad(some, 200, some, 200, None, 0, 4, 9, 200, some, -100, 1, some, ctypes.c_void_p(264), some, some, some, None, some,
                                             1 << 30, None) == _lib.EINVAL
+
+
+def test_the_last_piece_of_the_vocabulary_has_room():
+    """Fewer units of work can mean shorter shares and more workgroups, each of which has two places of 128 x 128 sums."""
+    from recommender_amd import _lib
+    L = _lib.lib()
+    some = ctypes.c_void_p(256)
+    # 600 columns: 5 x 3 tiles of dw with 57 steps each are 855 units, 2 to each of 428 workgroups (768 would be 1026, 3 to each of 342)
+    T, V, D = 7296, 600, 384
+    assert L.reco_linear_xent_grad_workspace_bytes(some, D, some, D, 0, T, V, D) >= 428 * 2 * 128 * 128 * 4 + T * V * 4 + T * D * 4
