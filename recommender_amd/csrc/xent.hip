@@ -163,7 +163,8 @@ __device__ __forceinline__ void drain_and_meet()
 // acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end).  Fragments are read one KSTEP before they are multiplied.  The barrier
 // stands before the last quarter of a step, whose fragments are in registers already: behind it nobody reads this half of LDS any
 // more, the step after next sets out for it, and the other half has arrived.
-template <typename T, bool AKC, bool BKC, int B>
+// DIRECT: whose tiles these are (product_kernel); the same work either way
+template <typename T, bool AKC, bool BKC, int B, bool DIRECT = false>
 __device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, const Operand<T>& Bm, int64_t m0, int64_t n0, int64_t k0, int64_t k_end, T* a0, T* a1,
                                              T* b0, T* b1)
 {
@@ -854,9 +855,10 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
 
 // A B in equal shares: the units are (tile, step of TB in k), the steps of a tile together, tiles of one row of tiles beside each other;
 // every workgroup takes `share` consecutive units and writes the sums of each tile it touches, in 32 bits, to a place of its own: place
-// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.  With `out` [M, N] a tile that lies in one share is finished
-// here: times scale / G_SCALE, rounded to T.
-template <typename T, bool AKC, bool BKC, int B>
+// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.  DIRECT: a tile of `out` [M, N] that lies in one share is
+// finished here: times scale / G_SCALE, rounded to T; in 16 bits through LDS, in whole lines (2 bytes a lane took 366 us for 131,072 x
+// 1024 values of 8 tokens, and 174 instead of 130 per 16,384 x 1024 of 4096).
+template <typename T, bool AKC, bool BKC, int B, bool DIRECT>
 __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T> A, Operand<T> Bm, int64_t tiles_n, int64_t M, int64_t N, int64_t K, int64_t steps,
                                                                        int64_t units, int64_t share, const float* __restrict__ scale, float* __restrict__ part,
                                                                        T* __restrict__ out)
@@ -866,6 +868,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
     const int64_t worker = place_of(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     const int64_t end = (worker + 1) * share < units ? (worker + 1) * share : units;
+    const bool whole16 = N * sizeof(T) % 16 == 0 && (uintptr_t)out % 16 == 0;
 #pragma unroll 1
     for (int64_t u = worker * share; u < end;) {
         const int64_t tile = u / steps, step = u - tile * steps, n = end - u < steps - step ? end - u : steps - step;
@@ -873,19 +876,53 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
         u += n;
         Acc<B> acc = {};
         const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
-        tile_product<T, AKC, BKC, B>(acc, A, Bm, m0, n0, k0, k1, TILE_LDS_ARGS);
-        if (out && n == steps) {
+        tile_product<T, AKC, BKC, B, DIRECT>(acc, A, Bm, m0, n0, k0, k1, TILE_LDS_ARGS);
+        if (DIRECT && n == steps) {
             const float f = *scale / Traits<T>::G_SCALE;
-#pragma unroll
-            for (int j = 0; j < S::NB; ++j) {
-                const int64_t c = n0 + wn + 32 * j + (lane & 31);
+            if constexpr (sizeof(T) == 2) {
+                // a wave's WM rows of 64 values, chunks changing places by the row
+                drain_and_meet();
+                constexpr int VEC = Traits<T>::VEC, CH = S::WN / VEC, PER_ARRAY = Stage<T, AKC, B>::SIZE / (S::WM * S::WN);
+                static_assert(PER_ARRAY * 4 >= S::THREADS / 64, "the waves' blocks fit the four arrays");
+                const int wave = threadIdx.x >> 6, array = wave / PER_ARRAY;
+                T* const mine = (array == 0 ? lds_a0 : array == 1 ? lds_a1 : array == 2 ? lds_b0 : lds_b1) + wave % PER_ARRAY * (S::WM * S::WN);
 #pragma unroll
                 for (int i = 0; i < S::MB; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int64_t m = m0 + wm + 32 * i + acc_row(r, half);
-                        if (m < M && c < N) out[m * N + c] = (T)(acc[i][j][r] * f);
+                        const int row = 32 * i + acc_row(r, half);
+#pragma unroll
+                        for (int j = 0; j < S::NB; ++j) {
+                            const int c = 32 * j + (lane & 31);
+                            mine[row * S::WN + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC] = (T)(acc[i][j][r] * f);
+                        }
                     }
+                drain_and_meet();
+                for (int at = lane; at < S::WM * CH; at += 64) {
+                    const int row = at / CH, c = at % CH;
+                    const int64_t m = m0 + wm + row, col = n0 + wn + c * VEC;
+                    if (m >= M) break;
+                    const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(mine + row * S::WN + (c ^ (row & (CH - 1))) * VEC);
+                    if (whole16) {
+                        if (col < N) *reinterpret_cast<Pack<T, VEC>*>(out + m * N + col) = v;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k)
+                            if (col + k < N) out[m * N + col + k] = v.v[k];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < S::NB; ++j) {
+                    const int64_t c = n0 + wn + 32 * j + (lane & 31);
+#pragma unroll
+                    for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int64_t m = m0 + wm + 32 * i + acc_row(r, half);
+                            if (m < M && c < N) out[m * N + c] = acc[i][j][r] * f;
+                        }
+                }
             }
             continue;
         }
@@ -909,19 +946,32 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
     if (direct && a == b) return;
     const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
     const float f = out ? *scale / Traits<T>::G_SCALE : 1.f;
+    const bool fours = N % 4 == 0 && (uintptr_t)out % sizeof(Pack<T, 4>) == 0;
     for (int i = (blockIdx.y * 256 + threadIdx.x) * 4; i < B * B; i += gridDim.y * 1024) {
         const int64_t m = m0 + i / B, n = n0 + i % B;
         if (m >= M || n >= N) continue;
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
         for (int64_t w = a; w <= b; ++w) s += *reinterpret_cast<const f32x4*>(part + (w * 2 + (w == a ? 1 : 0)) * (B * B) + i);
+        const int64_t at = m * N + n;
+        const int left = N - n < 4 ? (int)(N - n) : 4;
+        if (sum && !first)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (n + j >= N) break;
-            float v = s[j];
-            if (sum && !first) v += sum[m * N + n + j];
-            if (out) out[m * N + n + j] = (T)(v * f);
-            else sum[m * N + n + j] = v;
+            for (int j = 0; j < 4; ++j)
+                if (j < left) s[j] += sum[at + j];
+        if (!out) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < left) sum[at + j] = s[j];
+            continue;
         }
+        Pack<T, 4> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[j] = (T)(s[j] * f);
+        if (fours) *reinterpret_cast<Pack<T, 4>*>(out + at) = o;
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < left) out[at + j] = o.v[j];
     }
 }
 
@@ -1118,10 +1168,13 @@ int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t 
     return with_tile<T>(q.tile, [&](auto t) -> int {
         constexpr int W = decltype(t)::value;
         const bool direct = out && !sum;
-        hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W>), dim3((unsigned)q.workers), dim3(Shape<W>::THREADS), 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share,
-                           scale, part, direct ? out : nullptr);
+        const dim3 grid((unsigned)q.workers), block(Shape<W>::THREADS);
+        if (direct)
+            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, true>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, out);
+        else
+            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, false>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, out);
         if (!direct || q.share % q.steps)
-            hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / 4096)), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
+            hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / (q.tiles_m * q.tiles_n <= 64 ? 1024 : 4096))), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
                            scale, first, direct, sum, out);
         RECO_CHECK_LAUNCH();
         return RECO_OK;
