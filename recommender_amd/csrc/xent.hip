@@ -233,21 +233,25 @@ __device__ __forceinline__ void tile_product(Acc<B>& acc, const Operand<T>& A, c
     } while (left > 0);
 }
 
+// The rows of a block's registers: row_of(i, r) behind this half's first, so that one number is compared with constants
+__device__ __forceinline__ constexpr int row_of(int i, int r) { return 32 * i + acc_row(r, 0); }
+__device__ __forceinline__ int rows_behind(int64_t v, int64_t V, int most) { return V - v < most ? (int)(V - v) : most; }
+
 // acc: logits of vocabulary rows v0 .. (32 per i) and 32 tokens per j, plus the rows' bias
 template <typename T, int MB, int NB> __device__ __forceinline__ void add_bias(const Problem& p, f32x16 (&acc)[MB][NB], int64_t v0)
 {
-    const T* bias = (const T*)p.bias;
-    const int half = threadIdx.x >> 5 & 1;
-    if (bias)
+    if (!p.bias) return;
+    const int64_t first = v0 + 4 * (threadIdx.x >> 5 & 1);
+    const int left = rows_behind(first, p.V, 32 * MB), last = left > 0 ? left - 1 : 0;
+    const T* bias = (const T*)p.bias + (left > 0 ? first : 0);
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t v = v0 + 32 * i + acc_row(r, half);
-                const float z = v < p.V ? (float)bias[v] : 0.f;
+        for (int r = 0; r < 16; ++r) {
+            const float z = (float)bias[row_of(i, r) < last ? row_of(i, r) : last];           // behind the vocabulary: any, it is cleared later
 #pragma unroll
-                for (int j = 0; j < NB; ++j) acc[i][j][r] += z;
-            }
+            for (int j = 0; j < NB; ++j) acc[i][j][r] += z;
+        }
 }
 
 // The block's logits go into this lane's running maxima and sums, the targets' into z_target.  t0: this lane's first token
@@ -255,20 +259,22 @@ template <int MB, int NB>
 __device__ __forceinline__ void fold(const Problem& p, f32x16 (&acc)[MB][NB], int64_t v0, int64_t t0, const int64_t (&y)[NB], Running (&run)[NB],
                                      float* __restrict__ z_target)
 {
-    const int half = threadIdx.x >> 5 & 1;
-    const bool tail = v0 + 32 * MB > p.V;
+    const int64_t first = v0 + 4 * (threadIdx.x >> 5 & 1);
+    const int left = rows_behind(first, p.V, 32 * MB);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int64_t here = y[j] - v0;
-        if (tail || __any(here >= 0 && here < 32 * MB)) {
+        const int64_t off = y[j] - first;
+        const int here = off >= 0 && off < 32 * MB ? (int)off : -1;
+        if (__any(here >= 0 || left < 32 * MB)) {
+            float mine = 0.f;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int64_t v = v0 + 32 * i + acc_row(r, half);
-                    if (v == y[j]) z_target[t0 + 32 * j] = acc[i][j][r];
-                    if (v == y[j] || v >= p.V) acc[i][j][r] = -INFINITY;
+                    mine = row_of(i, r) == here ? acc[i][j][r] : mine;
+                    acc[i][j][r] = row_of(i, r) == here || row_of(i, r) >= left ? -INFINITY : acc[i][j][r];
                 }
+            if (here >= 0 && !(here & 4) && here < left) z_target[t0 + 32 * j] = mine;         // & 4: the other half's row
         }
         float top = -INFINITY;
 #pragma unroll
@@ -820,13 +826,16 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
     const int wave = threadIdx.x >> 6;
     const int array = wave / PER_ARRAY;
     T* const mine = (array == 0 ? lds_a0 : array == 1 ? lds_a1 : array == 2 ? lds_b0 : lds_b1) + wave % PER_ARRAY * (S::WN * ROW);
+    const int64_t first = m0 + wm + 4 * half;
+    const int left = rows_behind(first, p.V, S::WM);
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
         const int row = 32 * j + (lane & 31);
         const int64_t t = n0 + wn + row;
         const int64_t y0 = t < p.T ? p.target[t] : p.ignore;
         const bool in = y0 != p.ignore;
-        const int64_t y = in ? clamp_target(y0, p.V) : -1;
+        const int64_t off = in ? clamp_target(y0, p.V) - first : -1;
+        const int here = off >= 0 && off < S::WM ? (int)off : -1;
         const float l = in ? lse[t] : 0.f, low = in ? -LOG2E * lse[p.T + t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE : 0.f;
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
@@ -836,9 +845,9 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
                 Pack<T, 4> o;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int64_t v = m0 + wm + c + u;
-                    const float e = v == y ? -q : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * r4 + u] - l, LOG2E, low));
-                    o.v[u] = (T)(in && v < p.V ? e * g : 0.f);
+                    const int v = row_of(i, 4 * r4 + u);
+                    const float e = v == here ? -q : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * r4 + u] - l, LOG2E, low));
+                    o.v[u] = (T)(in && v < left ? e * g : 0.f);
                 }
                 *reinterpret_cast<Pack<T, 4>*>(mine + row * ROW + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC) = o;
             }
@@ -886,17 +895,21 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
                 static_assert(PER_ARRAY * 4 >= S::THREADS / 64, "the waves' blocks fit the four arrays");
                 const int wave = threadIdx.x >> 6, array = wave / PER_ARRAY;
                 T* const mine = (array == 0 ? lds_a0 : array == 1 ? lds_a1 : array == 2 ? lds_b0 : lds_b1) + wave % PER_ARRAY * (S::WM * S::WN);
+                static_assert(CH == 8, "a row's place among the chunks goes by its number modulo 8");
+                int spot[4][S::NB];                        // of rows 4 half + u, columns 32 j + lane % 32
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < S::NB; ++j) {
+                        const int row = 4 * half + u, c = 32 * j + (lane & 31);
+                        spot[u][j] = row * S::WN + ((c / VEC) ^ row) * VEC + c % VEC;
+                    }
 #pragma unroll
                 for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = 32 * i + acc_row(r, half);
+                    for (int r = 0; r < 16; ++r)
 #pragma unroll
-                        for (int j = 0; j < S::NB; ++j) {
-                            const int c = 32 * j + (lane & 31);
-                            mine[row * S::WN + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC] = (T)(acc[i][j][r] * f);
-                        }
-                    }
+                        for (int j = 0; j < S::NB; ++j) mine[spot[r & 3][j] + (32 * i + 8 * (r >> 2)) * S::WN] = (T)(acc[i][j][r] * f);
                 drain_and_meet();
                 for (int at = lane; at < S::WM * CH; at += 64) {
                     const int row = at / CH, c = at % CH;
@@ -912,27 +925,27 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
                     }
                 }
             } else {
+                const int left = rows_behind(m0 + wm + 4 * half, M, S::WM), at = (wm + 4 * half) * (int)N + wn + (lane & 31);
 #pragma unroll
                 for (int j = 0; j < S::NB; ++j) {
-                    const int64_t c = n0 + wn + 32 * j + (lane & 31);
+                    const bool in = n0 + wn + 32 * j + (lane & 31) < N;
 #pragma unroll
                     for (int i = 0; i < S::MB; ++i)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int64_t m = m0 + wm + 32 * i + acc_row(r, half);
-                            if (m < M && c < N) out[m * N + c] = acc[i][j][r] * f;
-                        }
+                        for (int r = 0; r < 16; ++r)
+                            if (in && row_of(i, r) < left) (out + (m0 + row_of(i, r)) * N + n0 + 32 * j)[at] = acc[i][j][r] * f;
                 }
             }
             continue;
         }
         float* to = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
+        const int mine = (wm + 4 * half) * B + wn + (lane & 31);
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
 #pragma unroll
             for (int j = 0; j < S::NB; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) to[(wm + 32 * i + acc_row(r, half)) * B + wn + 32 * j + (lane & 31)] = acc[i][j][r];
+                for (int r = 0; r < 16; ++r) (to + (row_of(i, r) * B + 32 * j))[mine] = acc[i][j][r];
     }
 }
 
