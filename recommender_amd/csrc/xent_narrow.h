@@ -291,15 +291,17 @@ __global__ __launch_bounds__(WAVES * 64, (waves_per_simd<T, DP>())) void narrow_
         const int here = y - (int)v0;                                           // the target's place in this block, if it is in it
         const bool tail = !BIAS && v0 + 32 > end, mine = __any((unsigned)here < 32u);
         if (tail || mine) {
-            const int left = (int)(end - v0);
+            const int left = (int)(end - v0), at = here - 4 * half, stop = left - 4 * half;      // registers are compared with constants
+            float own = 0.f;
             top = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int row = acc_row(r, half);
-                if (row == here && row < left) z_target[t] = z[r];
-                if (row == here || row >= left) z[r] = -INFINITY;
+                const int row = acc_row(r, 0);
+                own = row == at ? z[r] : own;
+                z[r] = row == at || row >= stop ? -INFINITY : z[r];
                 top = fmaxf(top, z[r]);
             }
+            if ((unsigned)here < 32u && (here & 4) == 4 * half && here < left) z_target[t] = own;
         }
         if (__any(top > m + lag<T>())) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));                          // both halves of a column keep one reference
