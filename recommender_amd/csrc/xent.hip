@@ -13,7 +13,12 @@
 // rounded to the operands' type to be multiplied (half a step per term, where the result takes one such rounding too); half-precision G
 // is held times 2^14, so that probabilities down to 2^-28 are normal numbers.
 //
-// This file: the form for every width.  A piece of G, [T, piece] in the operands' type, is written and read by two matrix products.
+// This file: the forms for every width and for few rows.  A piece of G, [T, piece] in the operands' type, is written and read by two matrix
+// products.  Bound by the matrix instructions: bf16 4096 x 131,072 x 1024 statistics 1.0 ms (1.1 PFLOP/s), G 0.16 ms and the products 0.12
+// ms each per piece of 16,384 columns (0.84, 1.14, 1.08 PFLOP/s; a large library product reaches 1.34); f32 3706 x 6040 x 500 0.24 ms and
+// 0.21 ms each, matrix instructions busy for 0.81 to 0.85 of the cycles.
+//
+// xent_narrow.h: rows of up to 128 values in 32 bits, 256 in 16 (4097 x 50,021 x 250 f16 with gradients 0.84 ms, 1.89 by this file's form).
 #include "xent_shared.h"
 
 namespace {
