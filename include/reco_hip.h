@@ -133,12 +133,12 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
                     void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * K-g  softmax cross entropy over a whole catalogue, and its gradients, without its logits in memory
+ * K-g  softmax cross entropy over a whole catalogue, and its gradients, without its logits in memory (but see `kept`)
  *   z[t, v] = sum_d x[t, d] w[v, d] + bias[v];   loss_t = log sum_v exp(z[t, v]) - z[t, target_t]
  * the loss over all items that a two-tower / GMF table (src/helpers/ncf_model.py:207-211) or the AutoRec decoder
  * (src/autorec/utils/model.py:31-33) is trained with; no counterpart in the reference, which samples negatives.
  * x [T, D], w [V, D], bias [V] (nullable) of one `dtype`, rows dense with strides ldx / ldw.  Any sizes, strides and alignment
- * (rows that do not start on 16 bytes, or whose width is no whole number of 16-byte groups, are copied into ws first).
+ * (rows that do not start on 16 bytes, or whose width is no whole number of 16-byte groups, may be copied into ws first).
  * target int64 [T]; a row whose target equals `ignore` has no loss and no gradient whatever its x holds; other targets outside
  * [0, V) are clamped and counted in *oob (nullable).  bias may hold -inf (items that are never offered) or the type's lowest value.
  * reduction: RECO_XENT_NONE (loss [T]), _MEAN over the rows that count (loss [1]; NaN when none does), _SUM.  loss and state are fp32.
@@ -146,6 +146,7 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
  * kept: the forward call can keep reco_linear_xent_kept_floats() floats for the gradient call (NULL: nothing), 16-byte aligned.  Narrow rows
  * (up to 128 values in 32 bits, 256 in 16): dx for an incoming gradient of one, from the same pass; the gradient call needs it for dx.
  * Wider ones: the logits, where that saves time and they are few (up to 512 MB); without them the gradient call computes them again.
+ * with_dx: whether a gradient of x will be asked for.  keep: whether the forward call will be given that room (its workspace differs).
  * dloss fp32: [T] for RECO_XENT_NONE, else [1].  dx [T, D], dw [V, D], db [V] dense, of `dtype`; NULL = not wanted.
  * Sums run in an order that depends on the sizes alone: the same bits on every run.  Work is enqueued only; calls that overlap need a
  * workspace each (*_workspace_bytes looks at x and w for their alignment, never through them), 16-byte aligned.

@@ -1037,12 +1037,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ in, int
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void zero_kernel(T* out, int64_t n)
-{
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (T)0.f;
-}
-
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
@@ -1396,7 +1390,7 @@ extern "C" size_t reco_linear_xent_workspace_bytes(const void* x, int64_t ldx, c
                                                    int keep)
 {
     if (T <= 0 || V <= 0 || D <= 0) return 0;
-    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr};
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
     size_t need = 0;
     (void)reco_with_type(dtype, [&](auto z) -> int {
         return forward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, keep != 0, nullptr, nullptr, &need, nullptr);
@@ -1440,7 +1434,7 @@ extern "C" int reco_linear_xent(const void* x, int64_t ldx, const void* w, int64
 extern "C" size_t reco_linear_xent_grad_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t T, int64_t V, int64_t D)
 {
     if (T <= 0 || V <= 0 || D <= 0) return 0;
-    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr};
+    const Args a{x, ldx, w, ldw, nullptr, dtype, T, V, D, nullptr, 0};
     size_t need = 0;
     (void)reco_with_type(dtype, [&](auto z) -> int {
         return backward<decltype(z)>(a, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, &need, nullptr);

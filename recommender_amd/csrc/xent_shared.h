@@ -7,7 +7,6 @@
 namespace xent {
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LN2 = 0.69314718055994530942f;
 
 template <typename T> struct Traits;
 template <> struct Traits<float> {

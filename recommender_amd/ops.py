@@ -600,7 +600,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, check_ids=True):
     """cross_entropy(x @ weight.T + bias, target) over a whole catalogue without its [T, V] logits in memory, differentiable in x,
-    weight and bias.
+    weight and bias (float32 rows of more than 128 values keep their logits for the gradient where these take 512 MB at most).
 
     x [T, D], weight [V, D], bias [V] (may hold -inf: items never offered) of one type, float32 / bfloat16 / float16; target integers
     [T]; rows whose target is ignore_index have no loss and no gradient.  The loss is float32: [T] for reduction "none" (0 for ignored
