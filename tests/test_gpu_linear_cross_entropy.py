@@ -246,6 +246,35 @@ def test_masks(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 200, 20), (1, 200, 700), (2, 200, 1000), (4, 300, 700), (20, 200, 300), (40, 200, 301), (64, 130000, 260), (70, 200, 300), (300, 400, 520),
+                                   (20, 200, 100), (300, 400, 100)])
+def test_masks_in_every_form(dtype, T, V, D):
+    ops = _ops()
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    target[:] = 7
+    ones = torch.ones(T, device="cuda")
+    alone = torch.full_like(b, -math.inf)
+    alone[7] = 0.5                                             # nothing but the target is offered
+    loss, grads = _check(x, w, target, alone, "none", g=ones, what="target alone")
+    assert not bool(loss.any()) and not any(bool(t.any()) for t in grads)
+    assert not bool(ops.linear_cross_entropy(x, w, target, alone, "none").any())
+    if dtype != torch.float16:                                 # (-65504 is no mask against logits of any size)
+        low = b.clone()
+        low[50:] = torch.finfo(dtype).min
+        _check(x, w, target, low, "mean", what="lowest")
+    gone = b.clone()
+    gone[7] = -math.inf                                        # the target is masked
+    loss, dx, dw, db = ops.linear_cross_entropy_grad(x, w, target, gone, "none")
+    assert bool(torch.isposinf(loss).all()) and bool(torch.isposinf(ops.linear_cross_entropy(x, w, target, gone, "none")).all())
+    want = Exact(x, w, target, gone, "none", -100, ones)
+    _close(dx, want.dx, want.dx_tol, "dx, masked target")
+    _close(dw, want.dw, want.dw_tol, "dw, masked target")
+    none = torch.full_like(b, -math.inf)                       # nothing is offered
+    assert bool(ops.linear_cross_entropy(x, w, target, none, "none").isnan().all())
+    assert bool(ops.linear_cross_entropy_grad(x, w, target, none, "none")[0].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("D", [16, 128, 512])
 def test_not_a_number_spreads_to_its_row_alone(dtype, D):
     ops = _ops()
@@ -448,6 +477,36 @@ def test_few_rows_off_every_alignment(dtype, T, D):
         assert bool(loss[1].isnan()) and int(loss.isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("T,V,D", [(3, 17000003, 128), (70, 17000003, 128), (3, 4200003, 520), (70, 4200003, 520)])
+def test_tables_beyond_32_bit_offsets(T, V, D):
+    """V D > 2^31 values.  Bounds: at most V / 256 terms one after the other (relative 4e-3 of a sum), logits within 2e-5, G and the result
+    rounded to bf16 (2^-8 each): 2e-2 of the sum of the terms' sizes."""
+    assert V * D > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(T + D)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    x = (torch.randn(T, D, device="cuda", generator=gen) / math.sqrt(D)).bfloat16()
+    target = torch.randint(0, V, (T,), device="cuda", generator=gen)
+    target[0], target[1] = V - 1, V // 2
+    loss, dx, dw, _ = _ops().linear_cross_entropy_grad(x, w, target, reduction="sum")
+    X, total, mean = x.double(), torch.zeros(T, dtype=torch.float64, device="cuda"), torch.zeros(T, D, dtype=torch.float64, device="cuda")
+    for at in range(0, V, 1 << 20):
+        W = w[at:at + (1 << 20)].double()
+        e = (X @ W.t()).exp()
+        total += e.sum(1)
+        mean += e @ W
+        del W, e
+    zt = (X * w[target].double()).sum(1)
+    want = (total.log() - zt).sum()
+    assert abs(float(loss) - float(want)) <= T * 4e-3 + 1e-6 * abs(float(want))
+    assert abs(float(_ops().linear_cross_entropy(x, w, target, reduction="sum")) - float(want)) <= T * 4e-3 + 1e-6 * abs(float(want))
+    exact = mean / total[:, None] - w[target].double()
+    assert bool(((dx.double() - exact).abs() <= 2e-2 * (w[target].double().abs() + 1)).all())
+    rows = torch.cat([torch.arange(V - 300, V, device="cuda"), target, torch.arange(V // 2 - 5, V // 2 + 5, device="cuda"), torch.arange(0, 10, device="cuda")])
+    G = (X @ w[rows].double().t()).exp() / total[:, None]
+    G = torch.where(rows[None, :] == target[:, None], G - 1, G)
+    assert bool(((dw[rows].double() - G.t() @ X).abs() <= 2e-2 * (G.abs().t() @ X.abs())).all())
+
+
 def test_more_rows_than_a_launch_has_waves():
     T, V, D = 2 ** 26 + 37, 3, 8
     w = torch.randn(V, D, device="cuda").bfloat16()
@@ -505,7 +564,7 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,V,D", [(70, 333, 50), (1, 5000, 64), (40, 200, 600)])
+@pytest.mark.parametrize("T,V,D", [(70, 333, 50), (1, 5000, 64), (40, 200, 600), (3, 900, 700), (300, 700, 300)])
 def test_captured_and_replayed(dtype, T, V, D):
     ops = _ops()
     x, w, target, b = _problem(T, V, D, dtype, True)
