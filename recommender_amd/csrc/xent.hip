@@ -1030,10 +1030,24 @@ template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ in, int64_t rows, int64_t ld, int64_t D, T* __restrict__ out, int64_t ldo,
                                                    const int64_t* __restrict__ target, int64_t ignore)
 {
-    const int64_t n = rows * ldo;
+    constexpr int VEC = Traits<T>::VEC;
+    typedef typename Traits<T>::frag frag;
+    typedef frag loose __attribute__((aligned(sizeof(T))));
+    const int64_t per_row = ldo / VEC, n = rows * per_row;
+#pragma unroll 4
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / ldo, c = i - r * ldo;
-        out[i] = c < D && !(target && target[r] == ignore) ? in[r * ld + c] : (T)0.f;
+        const int64_t r = n < (int64_t)1 << 32 ? (uint32_t)i / (uint32_t)per_row : i / per_row, c = (i - r * per_row) * VEC;
+        const T* src = in + r * ld + c;
+        const bool drop = target && target[r] == ignore;
+        frag v;
+        if (c + VEC <= D) {
+            v = *reinterpret_cast<const loose*>(src);
+            if (drop) v = frag{};
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = c + j < D && !drop ? src[j] : (T)0.f;
+        }
+        *reinterpret_cast<frag*>(out + r * ldo + c) = v;
     }
 }
 
@@ -1154,7 +1168,7 @@ template <typename T> int pack_rows(const Args& a, Problem& p, bool clean, Carve
         if (!(clean && is_x) && !must_pack(*m.p, *m.ld, a.D, sizeof(T))) continue;
         T* to = (T*)c.take((size_t)m.rows * padded * sizeof(T));
         if (launch) {
-            hipLaunchKernelGGL(pack_kernel<T>, dim3(stream_blocks(m.rows * padded)), dim3(256), 0, s, (const T*)*m.p, m.rows, *m.ld, a.D, to, padded,
+            hipLaunchKernelGGL(pack_kernel<T>, dim3(stream_blocks(m.rows * (padded / Traits<T>::VEC))), dim3(256), 0, s, (const T*)*m.p, m.rows, *m.ld, a.D, to, padded,
                                clean && is_x ? a.target : nullptr, a.ignore);
             RECO_CHECK_LAUNCH();
             *m.p = to;
