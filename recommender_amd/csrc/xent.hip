@@ -18,7 +18,7 @@
 // ms each per piece of 16,384 columns (0.84, 1.14, 1.08 PFLOP/s; a large library product reaches 1.34); f32 3706 x 6040 x 500 0.24 ms and
 // 0.21 ms each, matrix instructions busy for 0.81 to 0.85 of the cycles.
 //
-// xent_narrow.h: rows of up to 128 values in 32 bits, 256 in 16 (4097 x 50,021 x 250 f16 with gradients 0.84 ms, 1.89 by this file's form).
+// xent_narrow.h: rows of up to 128 values in 32 bits, 256 in 16 (4097 x 50,021 x 250 f16 with gradients 0.81 ms, 1.89 by this file's form).
 #include "xent_shared.h"
 
 namespace {
