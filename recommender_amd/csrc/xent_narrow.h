@@ -15,8 +15,8 @@
 //
 // What bounds it: a wave issues matrix instructions and exponentials in turn; an exponential per logit and two products of the row's width
 // share a SIMD's issue.  bf16 8192 x 100,003 x 128: rows 0.47 ms, cols 0.51 (0.90, 0.83 PFLOP/s); f16 4097 x 50,021 x 250: 0.41 and 0.36 (0.50,
-// 0.56); f32 6038 x 3533 x 32: 42 us each.  115 x 1 M x 128 without gradient: 69 us, 3.7 TB/s.  Two waves a SIMD, one where rows are 512
-// bytes: three spilled; 64 held rows a wave halved the waves and were slower; so was a ring unrolled over six blocks.
+// 0.56); f32 6038 x 3533 x 32: 42 us each.  115 x 1 M x 128 without gradient: 69 us, 3.7 TB/s.  At rows of 256 bytes three waves a SIMD spilled;
+// 64 held rows a wave halved the waves and were slower; so was a ring unrolled over six blocks.
 #pragma once
 #include "xent_shared.h"
 
@@ -230,8 +230,13 @@ template <typename U> __device__ __forceinline__ void store4(U* row, int c, int 
     if (c + 3 < width) row[c + 3] = (U)v3;
 }
 
-// Waves per SIMD that the registers are cut for
-template <typename T, int DP> constexpr int waves_per_simd() { return DP * (int)sizeof(T) >= 512 ? 1 : 2; }
+// Waves per SIMD that the registers are cut for.  8192 x 100,003 in bf16 with gradients: x 32 500 us with two, 447 with three, 432 with
+// four; x 64 662, 609, 1263 (spills); f32 2000 x 50,000 x 32 296, 287, 318 and 6038 x 3533 x 32 144, 149, 147.
+template <typename T, int DP> constexpr int waves_per_simd()
+{
+    if (sizeof(T) == 4) return DP == 128 ? 1 : 2;
+    return DP == 32 ? 4 : DP == 64 ? 3 : DP == 128 ? 2 : 1;
+}
 
 // ---------------------------------------------------------------------------------------------
 // rows: loss statistics, and with DX the softmax-weighted sums of W
