@@ -1248,7 +1248,7 @@ int forward(const Args& a, int reduction, float* loss, float* state, float* kept
     const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
     const int tile = tile_of(sizeof(T), a.T, a.V);
     const ForwardPlan f = forward_plan(a.T, a.V, tile);
-    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
+    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D, keep) : NarrowPlan{};
     const bool few = is_few(a, narrow, keep);
     const FewPlan fp = few_plan(a.T, a.V, a.D, sizeof(T));
     const int64_t splits = few ? fp.splits : narrow ? n.x_splits : f.splits;
@@ -1316,7 +1316,7 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
     float* tops = (float*)c.take(256 * 4);
     int* y = (int*)c.take((size_t)a.T * 4);
     float* expo = (float*)c.take((size_t)a.T * 8);
-    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D) : NarrowPlan{};
+    const NarrowPlan n = narrow ? narrow_plan_of<T>(a.T, a.V, a.D, true) : NarrowPlan{};
     const BackwardPlan b = narrow ? BackwardPlan{} : backward_plan(a.T, a.V, a.D, sizeof(T));
     T* G = nullptr;
     float *x_part = nullptr, *w_part = nullptr, *b_part = nullptr;

@@ -238,11 +238,15 @@ template <typename T, int DP> constexpr int waves_per_simd()
     return DP == 32 ? 4 : DP == 64 ? 3 : DP == 128 ? 2 : 1;
 }
 
+// of the rows kernel: one more without dx, whose sums are half of the registers (8192 x 100,003 x 128 bf16 326 -> 294 us, 4097 x 50,021 x 256
+// f16 229 -> 167, 115 x 1 M x 128 f32 351 -> 328; f32 2000 x 50,000 x 64 144 -> 147, and below that there are enough)
+template <typename T, int DP, bool DX> constexpr int rows_waves() { return waves_per_simd<T, DP>() + (!DX && DP >= 128 ? 1 : 0); }
+
 // ---------------------------------------------------------------------------------------------
 // rows: loss statistics, and with DX the softmax-weighted sums of W
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DP, bool BIAS, bool DX, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, (waves_per_simd<T, DP>())) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out,
+__global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>())) void narrow_rows_kernel(Problem p, int splits, int64_t rows_per_split, int width_out,
                                                                                    Running* __restrict__ part, float* __restrict__ z_target,
                                                                                    float* __restrict__ dx_part)
 {
@@ -652,14 +656,14 @@ inline void split_plan(int64_t T, int64_t D, int64_t groups, int64_t streamed, i
 
 namespace xent {
 
-template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D)
+template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D, bool dx)
 {
     NarrowPlan n{};
     (void)shape_of<T>(D, [&](auto dp, int64_t tile, int64_t places) -> int {
         constexpr int DP = decltype(dp)::value;
         n.x_waves = ONE_WAVE<T, DP> && T_rows <= 32 ? 1 : 4;
         n.x_groups = ceil_div64(T_rows, 32 * n.x_waves);
-        const int64_t x_places = n.x_waves == 4 ? places : 256 * (160 * 1024 / (3 * tile * (DP * (int)sizeof(T) + 4)));
+        const int64_t x_places = n.x_waves == 4 ? 256 * (dx ? rows_waves<T, DP, true>() : rows_waves<T, DP, false>()) : 256 * (160 * 1024 / (3 * tile * (DP * (int)sizeof(T) + 4)));
         split_plan(T_rows, DP, n.x_groups, V, tile, x_places, sizeof(T) == 2 ? 0.8e15 : 0.12e15, &n.x_splits, &n.x_per);
         n.w_groups = ceil_div64(V, HELD);
         n.w_tiles = ceil_div64(T_rows, tile);
@@ -723,7 +727,7 @@ int narrow_cols_of(const Problem& p, const NarrowPlan& n, int64_t width_out, con
 
 // One source file per element type instantiates these
 #define XENT_NARROW(T)                                                                                                                             \
-    template xent::NarrowPlan xent::narrow_plan_of<T>(int64_t, int64_t, int64_t);                                                                  \
+    template xent::NarrowPlan xent::narrow_plan_of<T>(int64_t, int64_t, int64_t, bool);                                                             \
     template int xent::narrow_rows_of<T>(const xent::Problem&, const xent::NarrowPlan&, int64_t, xent::Running*, float*, float*, hipStream_t);      \
     template int xent::narrow_cols_of<T>(const xent::Problem&, const xent::NarrowPlan&, int64_t, const float*, const int*, const float*,            \
                                          const float*, const float*, void*, void*, float*, float*, hipStream_t)

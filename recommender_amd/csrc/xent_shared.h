@@ -68,7 +68,7 @@ struct NarrowPlan {
     int64_t x_waves, x_groups, x_splits, x_per, w_groups, w_tiles, w_share, w_shares;
     bool w_shared;
 };
-template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D);
+template <typename T> NarrowPlan narrow_plan_of(int64_t T_rows, int64_t V, int64_t D, bool dx);
 template <typename T> int narrow_rows_of(const Problem& p, const NarrowPlan& n, int64_t width_out, Running* part, float* z_target, float* dx_part, hipStream_t s);
 template <typename T>
 int narrow_cols_of(const Problem& p, const NarrowPlan& n, int64_t width_out, const float* expo, const int* y, const float* rest, const float* gn,
