@@ -19,6 +19,7 @@
 // 0.21 ms each, matrix instructions busy for 0.81 to 0.85 of the cycles.
 //
 // xent_narrow.h: rows of up to 128 values in 32 bits, 256 in 16 (4097 x 50,021 x 250 f16 with gradients 0.81 ms, 1.89 by this file's form).
+#include "xent_plan.h"
 #include "xent_shared.h"
 
 namespace {
@@ -29,8 +30,6 @@ using namespace xent;
 // a B x B tile of a matrix product, B = 256 (8 waves, 128 x 64 each) or 128 (4 waves, 64 x 64 each): operands staged through LDS, two
 // steps of k in it; the next one arrives in registers while this one is multiplied; one barrier per step
 // ---------------------------------------------------------------------------------------------
-constexpr int TB = 128;          // sizes of slices and paddings are multiples of this
-
 // A matrix of which B rows r take part: KC: element (r, k) at p[r * ld + k], else at p[k * ld + r].  Row starts are 16-byte aligned;
 // `rows` (the limit of r) and k_end count whole VEC groups along the contiguous side.
 template <typename T> struct Operand {
@@ -867,15 +866,15 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
     }
 }
 
-// A B in equal shares: the units are (tile, step of TB in k), the steps of a tile together, tiles of one row of tiles beside each other;
-// every workgroup takes `share` consecutive units and writes the sums of each tile it touches, in 32 bits, to a place of its own: place
-// 1 if it begins the tile, place 0 if not.  join_kernel adds them in order.  DIRECT: a tile of `out` [M, N] that lies in one share is
-// finished here: times scale / G_SCALE, rounded to T; in 16 bits through LDS, in whole lines (2 bytes a lane took 366 us for 131,072 x
-// 1024 values of 8 tokens, and 174 instead of 130 per 16,384 x 1024 of 4096).
+// A B in equal shares (xent_plan.h), tiles of one row of tiles beside each other.  A tile that lies in one share is finished here: `sum`
+// [M, N], what earlier pieces left, is added to it (first: there is nothing yet), and it goes to `sum`, or with `out` [M, N], times
+// scale / G_SCALE and rounded to T, there; in 16 bits through LDS, in whole lines (2 bytes a lane took 366 us for 131,072 x 1024 values
+// of 8 tokens, and 174 instead of 130 per 16,384 x 1024 of 4096).  The 32-bit sums of a part of a tile go to one of the workgroup's two
+// places, and join_kernel adds those in order.  DIRECT: no `sum`, all of it goes to `out`.
 template <typename T, bool AKC, bool BKC, int B, bool DIRECT>
 __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T> A, Operand<T> Bm, int64_t tiles_n, int64_t M, int64_t N, int64_t K, int64_t steps,
                                                                        int64_t units, int64_t share, const float* __restrict__ scale, float* __restrict__ part,
-                                                                       T* __restrict__ out)
+                                                                       int first, float* __restrict__ sum, T* __restrict__ out)
 {
     typedef Shape<B> S;
     TILE_LDS(T, AKC, BKC, B);
@@ -885,13 +884,33 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
     const bool whole16 = N * sizeof(T) % 16 == 0 && (uintptr_t)out % 16 == 0;
 #pragma unroll 1
     for (int64_t u = worker * share; u < end;) {
-        const int64_t tile = u / steps, step = u - tile * steps, n = end - u < steps - step ? end - u : steps - step;
-        const int64_t k0 = step * TB, k1 = (step + n) * TB < K ? (step + n) * TB : K;
-        u += n;
+        const TilePart q = tile_part(u, end, steps);
+        const int64_t k0 = q.step * TB, k1 = (q.step + q.count) * TB < K ? (q.step + q.count) * TB : K;
+        u += q.count;
         Acc<B> acc = {};
-        const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
+        const int64_t m0 = q.tile / tiles_n * B, n0 = q.tile % tiles_n * B;
         tile_product<T, AKC, BKC, B, DIRECT>(acc, A, Bm, m0, n0, k0, k1, TILE_LDS_ARGS);
-        if (DIRECT && n == steps) {
+        // fn(block i, j and register r of a value, its place in m): the values inside a matrix m [M, N], 32 of a row beside each other
+        const auto each_value = [&](auto* m, auto&& fn) {
+            const int left = rows_behind(m0 + wm + 4 * half, M, S::WM), at = (wm + 4 * half) * (int)N + wn + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j) {
+                const bool in = n0 + wn + 32 * j + (lane & 31) < N;
+#pragma unroll
+                for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (in && row_of(i, r) < left) fn(i, j, r, (m + (m0 + row_of(i, r)) * N + n0 + 32 * j)[at]);
+            }
+        };
+        if (q.count == steps) {
+            if constexpr (!DIRECT) {
+                if (!first) each_value(sum, [&](int i, int j, int r, const float& s) { acc[i][j][r] += s; });
+                if (!out) {
+                    each_value(sum, [&](int i, int j, int r, float& s) { s = acc[i][j][r]; });
+                    continue;
+                }
+            }
             const float f = *scale / Traits<T>::G_SCALE;
             if constexpr (sizeof(T) == 2) {
                 // a wave's WM rows of 64 values, chunks changing places by the row
@@ -930,20 +949,11 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
                     }
                 }
             } else {
-                const int left = rows_behind(m0 + wm + 4 * half, M, S::WM), at = (wm + 4 * half) * (int)N + wn + (lane & 31);
-#pragma unroll
-                for (int j = 0; j < S::NB; ++j) {
-                    const bool in = n0 + wn + 32 * j + (lane & 31) < N;
-#pragma unroll
-                    for (int i = 0; i < S::MB; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (in && row_of(i, r) < left) (out + (m0 + row_of(i, r)) * N + n0 + 32 * j)[at] = acc[i][j][r] * f;
-                }
+                each_value(out, [&](int i, int j, int r, T& o) { o = acc[i][j][r] * f; });
             }
             continue;
         }
-        float* to = part + (worker * 2 + (step ? 0 : 1)) * (B * B);
+        float* to = part + place_of_part(worker, q.step == 0) * (B * B);
         const int mine = (wm + 4 * half) * B + wn + (lane & 31);
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
@@ -954,14 +964,14 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void product_kernel(Operand<T
     }
 }
 
-// The places of every tile added (direct: of those in several shares); with `sum` [M, N] added to (first: written to) it, or with `out` its total (and sum's, if !first)
-// times scale / G_SCALE rounded to T
+// The parts of every tile that several workgroups shared, added; to `sum` [M, N] and `out` as the whole tiles of product_kernel go
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int B, int64_t tiles_n, int64_t steps, int64_t share, int64_t M, int64_t N,
-                                                   const float* __restrict__ scale, int first, int direct, float* __restrict__ sum, T* __restrict__ out)
+                                                   const float* __restrict__ scale, int first, float* __restrict__ sum, T* __restrict__ out)
 {
-    const int64_t tile = blockIdx.x, a = tile * steps / share, b = ((tile + 1) * steps - 1) / share;
-    if (direct && a == b) return;
+    const int64_t tile = blockIdx.x;
+    const Workers from = workers_of(tile, steps, share);
+    if (from.first == from.last) return;
     const int64_t m0 = tile / tiles_n * B, n0 = tile % tiles_n * B;
     const float f = out ? *scale / Traits<T>::G_SCALE : 1.f;
     const bool fours = N % 4 == 0 && (uintptr_t)out % sizeof(Pack<T, 4>) == 0;
@@ -969,7 +979,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
         const int64_t m = m0 + i / B, n = n0 + i % B;
         if (m >= M || n >= N) continue;
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t w = a; w <= b; ++w) s += *reinterpret_cast<const f32x4*>(part + (w * 2 + (w == a ? 1 : 0)) * (B * B) + i);
+        for (int64_t w = from.first; w <= from.last; ++w) s += *reinterpret_cast<const f32x4*>(part + place_of_part(w, w == from.first) * (B * B) + i);
         const int64_t at = m * N + n;
         const int left = N - n < 4 ? (int)(N - n) : 4;
         if (sum && !first)
@@ -1094,13 +1104,6 @@ struct ForwardPlan {
     int64_t splits, tiles_per_split;
 };
 
-// 256-wide tiles in 16 bits (a 128-wide one asks LDS for 1.5 times as much per product), 128-wide ones where one side has no more rows,
-// and in 32 bits, whose matrix instructions are 16 times slower and whose smaller tiles fill the chip more evenly
-int tile_of(int size, int64_t rows_a, int64_t rows_b) { return size == 2 && rows_a > 128 && rows_b > 128 ? 256 : 128; }
-
-// workgroups of these kernels that the chip holds at once: one of 8 waves per compute unit, or two of 4
-int64_t places_of(int tile) { return tile == 256 ? 256 : 512; }
-
 // The split of the vocabulary with the fewest rounds of tiles; the longest runs of tiles among equals
 ForwardPlan forward_plan(int64_t T, int64_t V, int tile)
 {
@@ -1116,27 +1119,6 @@ ForwardPlan forward_plan(int64_t T, int64_t V, int tile)
     // more splits than the sums of a row are worth: at most 2048
     if (ceil_div64(tiles, best) > 2048) best = ceil_div64(tiles, 2048);
     return ForwardPlan{ceil_div64(tiles, best), best};
-}
-
-// A product in shares (product_kernel)
-struct ProductPlan {
-    int tile;
-    int64_t tiles_m, tiles_n, steps, units, share, workers;
-    size_t floats;                    // of the places
-};
-
-ProductPlan product_plan(int size, int64_t M, int64_t N, int64_t K)
-{
-    ProductPlan q;
-    q.tile = tile_of(size, M, N);
-    q.tiles_m = ceil_div64(M, q.tile);
-    q.tiles_n = ceil_div64(N, q.tile);
-    q.steps = ceil_div64(K, TB);
-    q.units = q.tiles_m * q.tiles_n * q.steps;
-    q.share = ceil_div64(q.units, places_of(q.tile));
-    q.workers = ceil_div64(q.units, q.share);
-    q.floats = (size_t)q.workers * 2 * q.tile * q.tile;
-    return q;
 }
 
 struct BackwardPlan {
@@ -1196,12 +1178,12 @@ int launch_product(const Operand<T>& A, const Operand<T>& B, int64_t M, int64_t 
         const bool direct = out && !sum;
         const dim3 grid((unsigned)q.workers), block(Shape<W>::THREADS);
         if (direct)
-            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, true>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, out);
-        else
-            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, false>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, out);
-        if (!direct || q.share % q.steps)
+            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, true>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, first, sum, out);
+        else if constexpr (AKC)                      // dx; dw has no sum of earlier pieces
+            hipLaunchKernelGGL((product_kernel<T, AKC, BKC, W, false>), grid, block, 0, s, A, B, q.tiles_n, M, N, K, q.steps, q.units, q.share, scale, part, first, sum, out);
+        if (q.share % q.steps)
             hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)(W * W / (q.tiles_m * q.tiles_n <= 64 ? 1024 : 4096))), dim3(256), 0, s, part, W, q.tiles_n, q.steps, q.share, M, N,
-                           scale, first, direct, sum, out);
+                           scale, first, sum, out);
         RECO_CHECK_LAUNCH();
         return RECO_OK;
     });

@@ -653,3 +653,14 @@ def test_tables_trained_by_it_are_served_by_the_engine():
 
 
 U0 = U
+
+
+@pytest.mark.parametrize("dtype,T,V,D", [(torch.bfloat16, 8192, 9000, 4096), (torch.float16, 16385, 9000, 1024), (torch.float32, 16384, 6040, 600),
+                                         (torch.float32, 8193, 4100, 1000)])
+def test_more_tiles_of_dx_than_the_chip_has_places(dtype, T, V, D):
+    """Several pieces of the vocabulary, and more tiles of dx (256 x 256 in 16 bits, 128 x 128 in 32) than workgroups that share them out:
+    a workgroup then has tiles of its own between the two that it shares."""
+    tile, places, size = (128, 512, 4) if dtype == torch.float32 else (256, 256, 2)
+    assert -(-T // tile) * -(-D // tile) > places and T * V * size > 128 << 20
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    _check(x, w, target, b, "mean")
