@@ -9,6 +9,7 @@ import operator
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ACT_CLAMP, ACT_NONE, ACT_RATING, ACT_RELU, ACT_SIGMOID, TowerDesc, check  # noqa: F401
@@ -108,6 +109,13 @@ def neumf_gather(eu_g, ei_g, eu_m, ei_m, user, item, check_ids=True, gmf_out=Non
 DTYPES = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
 
 
+def _no_tangent(t, name):
+    """There is no forward mode here: a dual tensor would come back without its tangent.  (Outside of a dual_level no tensor has one; asking
+    for it takes a microsecond, a ninth of a short lookup.)"""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError("%s has a tangent: forward-mode differentiation is not supported" % name)
+
+
 def _rows(t, name):
     """A 2-D float32 / bfloat16 / float16 GPU tensor whose rows are dense: a column block of a wider row-major buffer is read in
     place, anything else is copied."""
@@ -119,6 +127,7 @@ def _rows(t, name):
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
     if t.dim() != 2:
         raise ValueError("%s must be 2-D, got shape %s" % (name, tuple(t.shape)))
+    _no_tangent(t, name)
     t = t.detach()
     if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         t = t.contiguous()
@@ -525,6 +534,7 @@ def _xent_args(x, weight, target, bias, reduction, ignore_index):
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype != x.dtype or bias.device != x.device or tuple(bias.shape) != (weight.shape[0],):
             raise ValueError("bias must be a %s tensor of %d entries on %s" % (x.dtype, weight.shape[0], x.device))
+        _no_tangent(bias, "bias")
         bias = bias.detach().contiguous()
     target = _i64(target, "target", x.device)
     if target.numel() != x.shape[0]:
@@ -590,6 +600,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         _no_captured_graph("linear_cross_entropy's backward pass", "linear_cross_entropy_grad")
         if torch.is_grad_enabled():                     # create_graph: the result refuses to be differentiated again
             return _LinearCrossEntropy.once(ctx, dloss)
+        _no_tangent(dloss, "grad")
         return (*_xent_grad(*ctx.saved_tensors, dloss.contiguous(), *ctx.args, ctx.needs_input_grad[:3]), None, None, None, None, None)
 
     @staticmethod
@@ -624,6 +635,7 @@ def linear_cross_entropy_grad(x, weight, target, bias=None, reduction="mean", ig
         grad = torch.ones(shape, dtype=torch.float32, device=x.device)
     elif not isinstance(grad, torch.Tensor) or grad.dtype != torch.float32 or grad.device != x.device or tuple(grad.shape) != shape:
         raise ValueError("grad must be a float32 tensor of shape %s on %s" % (shape, x.device))
+    _no_tangent(grad, "grad")
     loss, state = _xent(x, weight, target, bias, reduction, ignore_index, False, True, True)
     return (loss, *_xent_grad(x, weight, target, bias, state, grad.detach().contiguous(), reduction, ignore_index, (True, True, bias is not None)))
 

@@ -664,3 +664,31 @@ def test_more_tiles_of_dx_than_the_chip_has_places(dtype, T, V, D):
     assert -(-T // tile) * -(-D // tile) > places and T * V * size > 128 << 20
     x, w, target, b = _problem(T, V, D, dtype, True)
     _check(x, w, target, b, "mean")
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word: the operators have no forward mode."""
+    from torch.autograd import forward_ad
+    ops = _ops()
+    x, w, target, b = _problem(20, 50, 16, torch.float32, True)
+    loss = ops.linear_cross_entropy(x, w, target, b)
+    dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))      # noqa: E731
+    with forward_ad.dual_level():
+        assert torch.equal(ops.linear_cross_entropy(x, w, target, b), loss)                # no dual tensor among them
+        for args in ((dual(x), w, target, b), (x, dual(w), target, b), (x, w, target, dual(b))):
+            for call in (ops.linear_cross_entropy, ops.linear_cross_entropy_grad):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                    call(*args)
+        with pytest.raises(NotImplementedError, match="forward"):
+            ops.linear_cross_entropy_grad(x, w, target, b, grad=dual(torch.ones((), device="cuda")))
+        with pytest.raises(NotImplementedError, match="forward"):
+            ops.embedding(target, dual(w))
+        with pytest.raises(NotImplementedError, match="forward"):
+            ops.embedding_grad(target, dual(x), 50)
+        # a backward pass whose incoming gradient has a tangent
+        leaf = x.clone().requires_grad_()
+        for out in (ops.linear_cross_entropy(leaf, w, target, b), ops.embedding(target[:4] % 20, leaf)):
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.autograd.grad(out, leaf, dual(torch.ones_like(out)))

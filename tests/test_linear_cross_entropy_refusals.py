@@ -87,3 +87,17 @@ def test_the_last_piece_of_the_vocabulary_has_room():
     # 600 columns: 5 x 3 tiles of dw with 57 steps each are 855 units, 2 to each of 428 workgroups (768 would be 1026, 3 to each of 342)
     T, V, D = 7296, 600, 384
     assert L.reco_linear_xent_grad_workspace_bytes(some, D, some, D, 0, T, V, D) >= 428 * 2 * 128 * 128 * 4 + T * V * 4 + T * D * 4
+
+
+def test_a_tangent_is_refused():
+    from torch.autograd import forward_ad
+    from recommender_amd import ops
+    x = torch.zeros(2, 3)
+    ops._no_tangent(x, "input")
+    with forward_ad.dual_level():
+        ops._no_tangent(x, "input")
+        for t in (forward_ad.make_dual(x, x), 2 * forward_ad.make_dual(x, x)):
+            with pytest.raises(NotImplementedError, match="input.*forward"):
+                ops._no_tangent(t, "input")
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+            ops._no_tangent(forward_ad.make_dual(x, x), "input")
