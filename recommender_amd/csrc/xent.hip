@@ -737,14 +737,14 @@ __global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __
 }
 
 // Rows' weights in two factors, gn[t] * scale: |gn| < 2 and scale a power of two where every row has a weight of its own, so that G
-// keeps its digits in 16 bits whatever the weights' size is; gn = 1 (NULL) and scale the incoming gradient, over the count for the
+// keeps its digits in 16 bits whatever the size of those weights is that are numbers; gn = 1 (NULL) and scale the incoming gradient, over the count for the
 // mean, where it is the same for all.
 __global__ __launch_bounds__(256) void top_kernel(Problem p, const float* __restrict__ dloss, float* __restrict__ tops)
 {
     __shared__ float sh[4];
     float top = 0.f;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < p.T; t += (int64_t)gridDim.x * 256)
-        if (p.target[t] != p.ignore) top = fmaxf(top, fabsf(dloss[t]));
+        if (p.target[t] != p.ignore && fabsf(dloss[t]) < INFINITY) top = fmaxf(top, fabsf(dloss[t]));
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, 
         for (int i = threadIdx.x & 63; i < n_tops; i += 64) top = fmaxf(top, tops[i]);
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        if (top > 0.f && top < INFINITY) {
+        if (top > 0.f) {
             int e;
             (void)frexpf(top, &e);                       // top = f 2^e with f in [0.5, 1)
             unit = ldexpf(1.f, e < -120 ? -120 : e > 127 ? 127 : e);

@@ -692,3 +692,19 @@ def test_forward_mode_is_refused():
         for out in (ops.linear_cross_entropy(leaf, w, target, b), ops.embedding(target[:4] % 20, leaf)):
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.autograd.grad(out, leaf, dual(torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [16, 128, 200, 320, 600])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_one_row_of_a_weight_that_is_no_number(dtype, D, bad):
+    """Rows' weights are brought to one size for 16 bits: by the largest that is a number."""
+    x, w, target, b = _problem(50, 90, D, dtype, True)
+    g = 100.0 * torch.randn(50, device="cuda")
+    g[7] = 0.0
+    want = Exact(x, w, target, b, "none", -100, g)
+    g[7] = bad
+    _, dx, _, _ = _ops().linear_cross_entropy_grad(x, w, target, b, "none", grad=g)
+    rest = torch.arange(50, device="cuda") != 7
+    _close(dx[rest], want.dx[rest], want.dx_tol[rest], "dx")
+    assert not bool(dx[7].isfinite().all())
