@@ -736,9 +736,10 @@ __global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __
     }
 }
 
-// Rows' weights in two factors, gn[t] * scale: |gn| < 2 and scale a power of two where every row has a weight of its own, so that G
-// keeps its digits in 16 bits whatever the size of those weights is that are numbers; gn = 1 (NULL) and scale the incoming gradient, over the count for the
-// mean, where it is the same for all.
+// Rows' weights in two factors, gn[t] * scale[0]: |gn| < 2 and scale a power of two where every row has a weight of its own, so that G
+// keeps its digits in 16 bits whatever the size of those weights is that are numbers; gn = 1 (NULL) and scale the incoming gradient, over
+// the count for the mean, where it is the same for all.  scale[0] = scale[1] * scale[2]: a finite factor of the finished sums, and one of
+// G's terms, 1 or what is no number: a row that does not count keeps its zeros.
 __global__ __launch_bounds__(256) void top_kernel(Problem p, const float* __restrict__ dloss, float* __restrict__ tops)
 {
     __shared__ float sh[4];
@@ -772,9 +773,14 @@ __global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, 
     } else if (reduction == REDUCE_MEAN) {
         unit = *count > 0.f ? *dloss / *count : 0.f;
     } else {
-        unit = *dloss;
+        unit = *count > 0.f ? *dloss : 0.f;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *scale = unit;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const bool number = fabsf(unit) < INFINITY;
+        scale[0] = unit;
+        scale[1] = number ? unit : 1.f;
+        scale[2] = number ? 1.f : unit;
+    }
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < p.T; t += (int64_t)gridDim.x * 256) {
         const int64_t target = p.target[t];
         const bool in = target != p.ignore;
@@ -787,21 +793,24 @@ __global__ __launch_bounds__(256) void weights_kernel(Problem p, int reduction, 
     }
 }
 
-// dx = gn * scale * dx_unit
+// dx = gn * scale * dx_unit, and 0 for rows that do not count (y < 0) whatever the scale is
 template <typename T>
 __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ unit, int64_t rows, int64_t D, const float* __restrict__ gn,
-                                                 const float* __restrict__ scale, T* __restrict__ dx)
+                                                 const int* __restrict__ y, const float* __restrict__ scale, T* __restrict__ dx)
 {
     const float f = *scale;
+    const bool number = fabsf(f) < INFINITY;
     const int64_t n = rows * D;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        dx[i] = (T)(unit[i] * (gn ? gn[i / D] * f : f));
+        dx[i] = !number && y[i / D] < 0 ? (T)0.f : (T)(unit[i] * (gn ? gn[i / D] * f : f));
 }
 
-// G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero.  KEPT: from the logits of the statistics
+// G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero.  KEPT: from the logits of the statistics.  gn: the
+// rows' weights, or *unit where it is the same for all
 template <typename T, int B, bool KEPT>
 __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int64_t v0, const float* __restrict__ kept, const float* __restrict__ lse,
-                                                                 const float* __restrict__ rest, const float* __restrict__ gn, T* __restrict__ G, int64_t ldg)
+                                                                 const float* __restrict__ rest, const float* __restrict__ gn, const float* __restrict__ unit,
+                                                                 T* __restrict__ G, int64_t ldg)
 {
     typedef Shape<B> S;
     int64_t token_tile, panel;
@@ -840,7 +849,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
         const bool in = y0 != p.ignore;
         const int64_t off = in ? clamp_target(y0, p.V) - first : -1;
         const int here = off >= 0 && off < S::WM ? (int)off : -1;
-        const float l = in ? lse[t] : 0.f, low = in ? -LOG2E * lse[p.T + t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : 1.f) * Traits<T>::G_SCALE : 0.f;
+        const float l = in ? lse[t] : 0.f, low = in ? -LOG2E * lse[p.T + t] : 0.f, q = in ? rest[t] : 0.f, g = in ? (gn ? gn[t] : *unit) * Traits<T>::G_SCALE : 0.f;
 #pragma unroll
         for (int i = 0; i < S::MB; ++i)
 #pragma unroll
@@ -1294,7 +1303,7 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
     Problem p;
     const bool launch = ws != nullptr, narrow = narrow_fits(a.dtype, a.D);
     float* gn = (float*)c.take((size_t)a.T * 4);
-    float* scale = (float*)c.take(4);
+    float* scale = (float*)c.take(3 * 4);
     float* tops = (float*)c.take(256 * 4);
     int* y = (int*)c.take((size_t)a.T * 4);
     float* expo = (float*)c.take((size_t)a.T * 8);
@@ -1335,7 +1344,7 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
             const int rn = narrow_cols_of<T>(p, n, a.D, expo, y, rest, gn, scale, dw, db, w_part, b_part, s);
             if (rn) return rn;
         }
-        if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, kept, a.T, a.D, gn, scale, (T*)dx);
+        if (dx) hipLaunchKernelGGL(dx_kernel<T>, dim3(stream_blocks(a.T * a.D)), dim3(256), 0, s, kept, a.T, a.D, gn, y, scale, (T*)dx);
         RECO_CHECK_LAUNCH();
         return RECO_OK;
     }
@@ -1346,23 +1355,23 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
             const dim3 grid((unsigned)(ceil_div64(a.T, B) * (ldg / B))), block(Shape<B>::THREADS);
             if constexpr (KEEPS<T>)
                 if (kept) {
-                    hipLaunchKernelGGL((g_kernel<T, B, true>), grid, block, 0, s, p, v0, kept, lse, rest, gn, G, ldg);
+                    hipLaunchKernelGGL((g_kernel<T, B, true>), grid, block, 0, s, p, v0, kept, lse, rest, gn, scale + 2, G, ldg);
                     RECO_CHECK_LAUNCH();
                     return RECO_OK;
                 }
-            hipLaunchKernelGGL((g_kernel<T, B, false>), grid, block, 0, s, p, v0, nullptr, lse, rest, gn, G, ldg);
+            hipLaunchKernelGGL((g_kernel<T, B, false>), grid, block, 0, s, p, v0, nullptr, lse, rest, gn, scale + 2, G, ldg);
             RECO_CHECK_LAUNCH();
             return RECO_OK;
         });
         if (!rl && dx)
-            rl = launch_product<T, true, false>({G, ldg, a.T}, {(const T*)p.w + v0 * p.ldw, p.ldw, p.D}, a.T, a.D, width, scale, v0 == 0, w_part, x_part,
+            rl = launch_product<T, true, false>({G, ldg, a.T}, {(const T*)p.w + v0 * p.ldw, p.ldw, p.D}, a.T, a.D, width, scale + 1, v0 == 0, w_part, x_part,
                                                 v0 + width == a.V ? (T*)dx : nullptr, s);
-        if (!rl && dw) rl = launch_product<T, false, false>({G, ldg, ldg}, {(const T*)p.x, p.ldx, p.D}, width, a.D, a.T, scale, true, w_part, nullptr, (T*)dw + v0 * a.D, s);
+        if (!rl && dw) rl = launch_product<T, false, false>({G, ldg, ldg}, {(const T*)p.x, p.ldx, p.D}, width, a.D, a.T, scale + 1, true, w_part, nullptr, (T*)dw + v0 * a.D, s);
         if (rl) return rl;
         if (db) {
             hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(ldg, 256 * Traits<T>::VEC), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per,
                                b_part);
-            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, ldg, width, scale, (T*)db + v0);
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, ldg, width, scale + 1, (T*)db + v0);
         }
         RECO_CHECK_LAUNCH();
     }

@@ -708,3 +708,19 @@ def test_one_row_of_a_weight_that_is_no_number(dtype, D, bad):
     rest = torch.arange(50, device="cuda") != 7
     _close(dx[rest], want.dx[rest], want.dx_tol[rest], "dx")
     assert not bool(dx[7].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(50, 90, 16), (300, 500, 100), (50, 90, 200), (50, 90, 320), (300, 700, 520), (9000, 16000, 520)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_ignored_rows_take_no_gradient_from_a_loss_that_is_no_number(dtype, T, V, D, bad):
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    target[::3] = -100
+    counts = target != -100
+    for reduction in ("mean", "sum"):
+        _, dx, dw, db = _ops().linear_cross_entropy_grad(x, w, target, b, reduction, grad=torch.tensor(bad, device="cuda"))
+        assert not bool(dx[~counts].any()) and not bool(dx[counts].isfinite().any()) and not bool(dw.isfinite().all()) and not bool(db.isfinite().all())
+    target[:] = -100
+    for reduction in ("mean", "sum"):
+        grads = _ops().linear_cross_entropy_grad(x, w, target, b, reduction, grad=torch.tensor(bad, device="cuda"))[1:]
+        assert not any(bool(t.any()) for t in grads)
