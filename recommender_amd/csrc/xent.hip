@@ -10,8 +10,9 @@
 // which 1 - p would lose.  Ignored rows have no loss and no gradient, whatever their x holds.
 //
 // Everything but the operands of the matrix instructions is 32 bits wide: logits, running maxima and sums, losses, accumulators.  G is
-// rounded to the operands' type to be multiplied (half a step per term, where the result takes one such rounding too); half-precision G
-// is held times 2^14, so that probabilities down to 2^-28 are normal numbers.
+// rounded to the operands' type to be multiplied: half a step of each term of dx and dW, where the result takes one such rounding too; more
+// than that only where the terms cancel, and the matrix instructions take 16-bit operands in 16 bits.  dbias multiplies nothing and adds
+// the terms as they are.  Half-precision G is held times 2^14, so that probabilities down to 2^-28 are normal numbers.
 //
 // This file: the forms for every width and for few rows.  A piece of G, [T, piece] in the operands' type, is written and read by two matrix
 // products.  Bound by the matrix instructions: bf16 4096 x 131,072 x 1024 statistics 1.0 ms (1.1 PFLOP/s), G 0.16 ms and the products 0.12
@@ -805,12 +806,26 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ unit,
         dx[i] = !number && y[i / D] < 0 ? (T)0.f : (T)(unit[i] * (gn ? gn[i / D] * f : f));
 }
 
+// N values of each lane (a multiple of 32), added over the 32 lanes of its half: the number of values halves with each exchange, and lane l
+// ends with the sums of values PER l .. PER l + PER - 1, PER = N / 32, in v[0 .. PER)
+template <int N, int FAR = 16> __device__ __forceinline__ void lanes_added(float* v)
+{
+    const bool up = threadIdx.x & FAR;
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+        const float mine = up ? v[k + N / 2] : v[k], other = up ? v[k] : v[k + N / 2];
+        v[k] = mine + __shfl_xor(other, FAR, 64);
+    }
+    if constexpr (FAR > 1) lanes_added<N / 2, FAR / 2>(v);
+}
+
 // G of the vocabulary rows [v0, v0 + width): [T, ldg], columns behind the vocabulary zero.  KEPT: from the logits of the statistics.  gn: the
-// rows' weights, or *unit where it is the same for all
+// rows' weights, or *unit where it is the same for all.  sums (nullable): dbias takes the terms before they are rounded -- they cancel
+// where an item is the target as often as the model expects -- column sums of 64 tokens each, [tokens / 64, whole tiles][ldg] in 32 bits.
 template <typename T, int B, bool KEPT>
 __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int64_t v0, const float* __restrict__ kept, const float* __restrict__ lse,
                                                                  const float* __restrict__ rest, const float* __restrict__ gn, const float* __restrict__ unit,
-                                                                 T* __restrict__ G, int64_t ldg)
+                                                                 T* __restrict__ G, int64_t ldg, float* __restrict__ sums)
 {
     typedef Shape<B> S;
     int64_t token_tile, panel;
@@ -860,10 +875,27 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void g_kernel(Problem p, int6
                 for (int u = 0; u < 4; ++u) {
                     const int v = row_of(i, 4 * r4 + u);
                     const float e = v == here ? -q : __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * r4 + u] - l, LOG2E, low));
-                    o.v[u] = (T)(in && v < left ? e * g : 0.f);
+                    const float term = in && v < left ? e * g : 0.f;
+                    o.v[u] = (T)term;
+                    acc[i][0][4 * r4 + u] = j ? acc[i][0][4 * r4 + u] + term : term;
                 }
                 *reinterpret_cast<Pack<T, 4>*>(mine + row * ROW + ((c / VEC) ^ (row & (CH - 1))) * VEC + c % VEC) = o;
             }
+    }
+    if (sums) {
+        constexpr int PER = S::MB / 2;                              // of the 16 MB rows in a lane's registers
+        float v[16 * S::MB];
+#pragma unroll
+        for (int i = 0; i < S::MB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[16 * i + r] = acc[i][0][r];
+        lanes_added<16 * S::MB>(v);
+        const int k = (lane & 31) * PER;
+        float* const to = sums + (n0 + wn) / 64 * ldg + (m0 - v0 + wm) + 32 * (k / 16) + acc_row(k % 16, half);
+        Pack<float, PER> own;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) own.v[i] = v[i];
+        *reinterpret_cast<Pack<float, PER>*>(to) = own;
     }
     drain_and_meet();
     for (int at = lane; at < S::WN * CH; at += 64) {
@@ -1025,23 +1057,16 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
     }
 }
 
-// column sums of G, [slices][ldg] in 32 bits: slice blockIdx.y takes rows [y * rows_per, ...); 16 bytes of a row per thread
-template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ G, int64_t ldg, int64_t T_rows, int64_t rows_per, float* __restrict__ out)
+// sums of `rows` rows of in [rows, ld], [slices][ld]: slice blockIdx.y takes rows [y * rows_per, ...); 16 bytes of a row per thread
+__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ in, int64_t ld, int64_t rows, int64_t rows_per, float* __restrict__ out)
 {
-    constexpr int VEC = Traits<T>::VEC;
-    const int64_t v = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
-    const int64_t t0 = blockIdx.y * rows_per, t1 = t0 + rows_per < T_rows ? t0 + rows_per : T_rows;
-    if (v >= ldg) return;
-    float s[VEC] = {};
+    const int64_t v = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t t0 = blockIdx.y * rows_per, t1 = t0 + rows_per < rows ? t0 + rows_per : rows;
+    if (v >= ld) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int64_t t = t0; t < t1; ++t) {
-        const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC>*>(G + t * ldg + v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] += (float)g.v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[blockIdx.y * ldg + v + i] = s[i];
+    for (int64_t t = t0; t < t1; ++t) s += *reinterpret_cast<const f32x4*>(in + t * ld + v);
+    *reinterpret_cast<f32x4*>(out + blockIdx.y * ld + v) = s;
 }
 
 // rows with their width filled up to `ldo` with zeros; rows whose target (nullable) is `ignore` as zeros
@@ -1132,19 +1157,23 @@ ForwardPlan forward_plan(int64_t T, int64_t V, int tile)
 
 struct BackwardPlan {
     int64_t width;                    // vocabulary rows per piece, a multiple of 256
-    int64_t b_slices, b_per;          // row slices of G's column sums
+    int64_t b_sums;                   // rows of 64 tokens' column sums of G
+    int64_t b_slices, b_per;          // more than 64 of them are added in slices first (0: they are not)
 };
 
 constexpr size_t PIECE_BYTES = (size_t)128 << 20;
 
 BackwardPlan backward_plan(int64_t T, int64_t V, int64_t D, int size)
 {
-    BackwardPlan b;
+    BackwardPlan b{};
     const int64_t tiles = ceil_div64(V, 256), by_g = (int64_t)(PIECE_BYTES / ((size_t)T * size)) / 256;
     b.width = clamp64(by_g, 1, tiles < 16384 ? tiles : 16384) * 256;
-    b.b_slices = clamp64(512 / ceil_div64(b.width, 256 * (16 / size)), 1, ceil_div64(T, 32) < 64 ? ceil_div64(T, 32) : 64);
-    b.b_per = ceil_div64(T, b.b_slices);
-    b.b_slices = ceil_div64(T, b.b_per);
+    const int tile = tile_of(size, T, V);
+    b.b_sums = ceil_div64(T, tile) * (tile / 64);
+    if (b.b_sums > 64) {
+        b.b_per = ceil_div64(b.b_sums, 64);
+        b.b_slices = ceil_div64(b.b_sums, b.b_per);
+    }
     return b;
 }
 
@@ -1325,7 +1354,7 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
                 if (q.floats > places) places = q.floats;
         w_part = (float*)c.take(places * 4);
         if (b.width < a.V) x_part = (float*)c.take((size_t)a.T * a.D * 4);
-        b_part = (float*)c.take((size_t)b.b_slices * b.width * 4);
+        b_part = (float*)c.take((size_t)(b.b_sums + b.b_slices) * b.width * 4);
     }
     const int rc = pack_rows<T>(a, p, !narrow, c, launch, s);
     if (rc) return rc;
@@ -1355,11 +1384,13 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
             const dim3 grid((unsigned)(ceil_div64(a.T, B) * (ldg / B))), block(Shape<B>::THREADS);
             if constexpr (KEEPS<T>)
                 if (kept) {
-                    hipLaunchKernelGGL((g_kernel<T, B, true>), grid, block, 0, s, p, v0, kept, lse, rest, gn, scale + 2, G, ldg);
+                    hipLaunchKernelGGL((g_kernel<T, B, true>), grid, block, 0, s, p, v0, kept, lse, rest, gn, scale + 2, G, ldg,
+                                       db ? b_part : nullptr);
                     RECO_CHECK_LAUNCH();
                     return RECO_OK;
                 }
-            hipLaunchKernelGGL((g_kernel<T, B, false>), grid, block, 0, s, p, v0, nullptr, lse, rest, gn, scale + 2, G, ldg);
+            hipLaunchKernelGGL((g_kernel<T, B, false>), grid, block, 0, s, p, v0, nullptr, lse, rest, gn, scale + 2, G, ldg,
+                               db ? b_part : nullptr);
             RECO_CHECK_LAUNCH();
             return RECO_OK;
         });
@@ -1369,9 +1400,14 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
         if (!rl && dw) rl = launch_product<T, false, false>({G, ldg, ldg}, {(const T*)p.x, p.ldx, p.D}, width, a.D, a.T, scale + 1, true, w_part, nullptr, (T*)dw + v0 * a.D, s);
         if (rl) return rl;
         if (db) {
-            hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)ceil_div64(ldg, 256 * Traits<T>::VEC), (unsigned)b.b_slices), dim3(256), 0, s, G, ldg, a.T, b.b_per,
-                               b_part);
-            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, b_part, (int)b.b_slices, ldg, width, scale + 1, (T*)db + v0);
+            const float* from = b_part;
+            if (b.b_slices) {
+                hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)ceil_div64(ldg, 1024), (unsigned)b.b_slices), dim3(256), 0, s, b_part, ldg, b.b_sums, b.b_per,
+                                   b_part + b.b_sums * ldg);
+                from += b.b_sums * ldg;
+            }
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(stream_blocks(width)), dim3(256), 0, s, from, (int)(b.b_slices ? b.b_slices : b.b_sums), ldg, width, scale + 1,
+                               (T*)db + v0);
         }
         RECO_CHECK_LAUNCH();
     }

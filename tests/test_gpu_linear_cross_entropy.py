@@ -724,3 +724,24 @@ def test_ignored_rows_take_no_gradient_from_a_loss_that_is_no_number(dtype, T, V
     for reduction in ("mean", "sum"):
         grads = _ops().linear_cross_entropy_grad(x, w, target, b, reduction, grad=torch.tensor(bad, device="cuda"))[1:]
         assert not any(bool(t.any()) for t in grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(600, 300, 40), (600, 300, 320), (1200, 400, 264), (40, 20, 300), (5, 5, 700), (5000, 16385, 260)])
+def test_gradient_of_the_bias_is_summed_before_any_rounding(dtype, T, V, D):
+    """No product needs the terms of dbias rounded to the type.  Where they cancel (every item is the target as often as the model expects
+    it to be) terms rounded to 16 bits would leave half a step of each; what is left of the bound is 32-bit: Exact's without that part."""
+    ops = _ops()
+    x, w, _, _ = _problem(T, V, D, dtype, False)
+    target = torch.arange(T, device="cuda") % V
+    h = torch.finfo(dtype).eps / 2
+    for x, w in ((torch.zeros_like(x), w), (x, w)):
+        for reduction, g in (("sum", None), ("none", 0.5 + torch.rand(T, device="cuda"))):
+            zero = torch.zeros(V, dtype=dtype, device="cuda")
+            want = Exact(x, w, target, zero, reduction, -100, g)
+            G = torch.softmax(x.double() @ w.double().t(), 1)
+            G[torch.arange(T, device="cuda"), target] -= 1
+            sizes = (G * (1.0 if g is None else g.double()[:, None])).abs().sum(0)
+            tol = want.db_tol - 1.05 * h * sizes
+            assert bool((tol > 0).all())
+            _close(ops.linear_cross_entropy_grad(x, w, target, zero, reduction, grad=g)[3], want.db, tol, "db, %s" % reduction)
