@@ -158,11 +158,14 @@ template <int B, typename F> __device__ __forceinline__ void each_kept(F&& fn)  
             for (int r = 0; r < 16; r += 4) fn(i, j, r, ((i * Shape<B>::NB + j) * 4 + r / 4) * 256);
 }
 
-// All of this wave's loads and LDS accesses are done, then the workgroup's
+// All of this wave's loads and LDS accesses are done, then the workgroup's.  The fences are for the compiler, to which neither the wait nor
+// the barrier is an access to memory; the wait is for the loads from memory to LDS, which the fences leave under way.
 __device__ __forceinline__ void drain_and_meet()
 {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 // acc += A (rows m0 ..) times B (rows n0 ..) over k in [k0, k_end).  Fragments are read one KSTEP before they are multiplied.  The barrier

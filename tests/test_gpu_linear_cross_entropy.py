@@ -745,3 +745,13 @@ def test_gradient_of_the_bias_is_summed_before_any_rounding(dtype, T, V, D):
             tol = want.db_tol - 1.05 * h * sizes
             assert bool((tol > 0).all())
             _close(ops.linear_cross_entropy_grad(x, w, target, zero, reduction, grad=g)[3], want.db, tol, "db, %s" % reduction)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(513, 1500, 384), (300, 70000, 260), (2000, 4000, 1100), (130, 900, 2048), (17000, 9000, 1024)])
+def test_the_wide_form_repeats_bit_for_bit(dtype, T, V, D):
+    """Tiles on their way to LDS while others are read, results that leave through LDS, one piece and several: no wave runs ahead."""
+    p = _problem(T, V, D, dtype, True)
+    first = _ops().linear_cross_entropy_grad(*p)
+    for _ in range(12):
+        assert all(torch.equal(a, b) for a, b in zip(first, _ops().linear_cross_entropy_grad(*p)))
