@@ -524,6 +524,8 @@ def _xent_args(x, weight, target, bias, reduction, ignore_index):
         raise ValueError("reduction must be one of %s, got %r" % (sorted(REDUCTIONS), reduction))
     if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
         raise TypeError("ignore_index must be an int, got %r" % (ignore_index,))
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must fit 64 bits, got %d" % ignore_index)
     x, weight = _rows(x, "input"), _rows(weight, "weight")
     if weight.dtype != x.dtype or weight.device != x.device:
         raise ValueError("weight must be %s on %s like the input, got %s on %s" % (x.dtype, x.device, weight.dtype, weight.device))

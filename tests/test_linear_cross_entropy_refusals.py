@@ -101,3 +101,16 @@ def test_a_tangent_is_refused():
                 ops._no_tangent(t, "input")
         with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
             ops._no_tangent(forward_ad.make_dual(x, x), "input")
+
+
+def test_ignore_index_fits_a_target():
+    """A longer one would be cut to its low 64 bits on its way into the library, and could name a column."""
+    from recommender_amd import ops
+    x, w, t = torch.zeros(4, 8), torch.zeros(9, 8), torch.zeros(4, dtype=torch.int64)
+    for call in (ops.linear_cross_entropy, ops.linear_cross_entropy_grad):
+        for bad in (2 ** 64 + 5, 2 ** 63, -2 ** 63 - 1):
+            with pytest.raises(ValueError, match="ignore_index"):
+                call(x, w, t, ignore_index=bad)
+        for good in (2 ** 63 - 1, -2 ** 63):
+            with pytest.raises(ValueError, match="GPU"):
+                call(x, w, t, ignore_index=good)
