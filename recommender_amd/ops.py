@@ -179,8 +179,14 @@ def _no_captured_graph(what, instead):
                            "in the captured work" % (what, instead))
 
 
+def _width(dim):
+    if dim >= 2 ** 31:                                  # the C entries take it as an int
+        raise ValueError("rows of at most 2^31 - 1 values, got %d" % dim)
+    return dim
+
+
 def _embedding(ids, table, scale, check_ids):
-    dev, (rows, dim), n = table.device, table.shape, ids.numel()
+    dev, rows, dim, n = table.device, table.shape[0], _width(table.shape[1]), ids.numel()
     out = torch.empty((n, dim), dtype=table.dtype, device=dev)
     if out.numel() == 0:
         return out
@@ -194,7 +200,7 @@ def _embedding(ids, table, scale, check_ids):
 
 
 def _embedding_grad(ids, grad, rows, scale, padding):
-    n, dim = grad.shape
+    n, dim = grad.shape[0], _width(grad.shape[1])
     dev = grad.device
     out = torch.empty((rows, dim), dtype=grad.dtype, device=dev)
     if out.numel() == 0:

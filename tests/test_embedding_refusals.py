@@ -69,3 +69,14 @@ def test_whole_numbers_are_asked_for():
     assert ops._padding(torch.tensor(3), 4) == 3
     with pytest.raises(TypeError):
         ops.embedding_grad(torch.zeros(2, dtype=torch.int64), torch.zeros(2, 3), 4.5)
+
+
+def test_rows_too_wide_for_the_library_are_refused():
+    """Refused before anything is allocated (the wide row here is one value, expanded): its width would be cut to 32 bits."""
+    from recommender_amd import ops
+    wide = torch.zeros(1, 1).expand(1, 2 ** 31 + 8)
+    with pytest.raises(ValueError, match="2147483656"):
+        ops._embedding(torch.zeros(1, dtype=torch.int64), wide, 1.0, False)
+    with pytest.raises(ValueError, match="2147483656"):
+        ops._embedding_grad(torch.zeros(1, dtype=torch.int64), wide, 4, 1.0, -1)
+    assert ops._width(2 ** 31 - 1) == 2 ** 31 - 1
