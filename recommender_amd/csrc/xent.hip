@@ -712,7 +712,7 @@ __device__ __forceinline__ float block_sum(float v, float* sh)
     return r;
 }
 
-// in: the rows' losses (of Problem p), or with p.T = 0 the `parts` (sum, count) of an earlier launch
+// rows: the rows' losses (of Problem p); or, where `parts` is given, those (sum, count) that an earlier launch left are joined
 __global__ __launch_bounds__(1024) void reduce_kernel(Problem p, const float* __restrict__ rows, const float2* __restrict__ parts, int n_parts, int reduction,
                                                       float* __restrict__ loss, float* __restrict__ count_out, float2* __restrict__ part_out)
 {

@@ -755,3 +755,25 @@ def test_the_wide_form_repeats_bit_for_bit(dtype, T, V, D):
     first = _ops().linear_cross_entropy_grad(*p)
     for _ in range(12):
         assert all(torch.equal(a, b) for a, b in zip(first, _ops().linear_cross_entropy_grad(*p)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 90, 16), (50, 90, 100), (50, 90, 200), (50, 400, 320), (3, 400, 700), (300, 700, 520)])
+def test_both_forms_agree_beside_what_is_no_number(dtype, T, V, D):
+    """Autograd's gradients and the functional form's have the same bits, value by value, where some rows are NaN or infinite as well."""
+    ops = _ops()
+    x, w, target, b = _problem(T, V, D, dtype, True)
+    target[T // 2] = 3
+    target[T - 1] = -100
+    hidden = b.clone()
+    hidden[3] = -math.inf                                      # an infinite loss
+    spoilt = x.clone()
+    spoilt[0, D // 2] = math.nan
+    for x, b in ((x, hidden), (spoilt, b), (spoilt, hidden)):
+        for reduction in ("none", "mean", "sum"):
+            g = torch.randn(T, device="cuda") if reduction == "none" else torch.tensor(1.5, device="cuda")
+            leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+            loss = ops.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], reduction)
+            auto = (loss.detach(),) + torch.autograd.grad(loss, leaves, g)
+            for p, q in zip(ops.linear_cross_entropy_grad(x, w, target, b, reduction, grad=g), auto):
+                assert bool(((p == q) | (p.isnan() & q.isnan())).all())
