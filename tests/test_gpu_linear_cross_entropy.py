@@ -777,3 +777,20 @@ def test_both_forms_agree_beside_what_is_no_number(dtype, T, V, D):
             auto = (loss.detach(),) + torch.autograd.grad(loss, leaves, g)
             for p, q in zip(ops.linear_cross_entropy_grad(x, w, target, b, reduction, grad=g), auto):
                 assert bool(((p == q) | (p.isnan() & q.isnan())).all())
+
+
+@pytest.mark.parametrize("D", [1, 32, 64, 128, 200])
+def test_gradient_of_the_bias_over_many_rows(D):
+    """Thousands of equal terms: added one after the other their roundings go one way.  With logits of 0 the exponentials and the row sums are
+    whole numbers, so what is left is lse (to 4 u |lse|, an absolute error of the exponent), the exponential (4 u) and the sum: 16 terms one
+    after the other, and a few joins (32 u): within 80 u of the terms' sizes."""
+    T, V = 16000, 43808
+    x = torch.randn(T, D, device="cuda")
+    w, b = torch.zeros(V, D, device="cuda"), torch.zeros(V, device="cuda")
+    target = torch.arange(T, device="cuda") % 1000
+    db = _ops().linear_cross_entropy_grad(x, w, target, b, "sum")[3]
+    hits = torch.bincount(target, minlength=V).double()
+    exact = (T - hits) / V - hits * (1 - 1 / V)
+    sizes = (T - hits) / V + hits * (1 - 1 / V)
+    assert 4 * math.log(V) + 4 + 32 < 80
+    _close(db, exact, 80 * U * sizes, "db")
