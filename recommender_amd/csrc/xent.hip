@@ -262,10 +262,10 @@ template <typename T, int MB, int NB> __device__ __forceinline__ void add_bias(c
         }
 }
 
-// The block's logits go into this lane's running maxima and sums, the targets' into z_target.  t0: this lane's first token
+// The block's logits go into this lane's running maxima and sums (over: as in Sum), the targets' into z_target.  t0: this lane's first token
 template <int MB, int NB>
 __device__ __forceinline__ void fold(const Problem& p, f32x16 (&acc)[MB][NB], int64_t v0, int64_t t0, const int64_t (&y)[NB], Running (&run)[NB],
-                                     float* __restrict__ z_target)
+                                     float (&over)[NB], float* __restrict__ z_target)
 {
     const int64_t first = v0 + 4 * (threadIdx.x >> 5 & 1);
     const int left = rows_behind(first, p.V, 32 * MB);
@@ -290,12 +290,16 @@ __device__ __forceinline__ void fold(const Problem& p, f32x16 (&acc)[MB][NB], in
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
         const float m = fmaxf(run[j].m, top), base = m == -INFINITY ? 0.f : m;
-        float s = run[j].s * exp2f((run[j].m - base) * LOG2E);
+        float block = 0.f;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
-        run[j] = Running{m, s};
+            for (int r = 0; r < 16; ++r) block += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
+        Sum sum{run[j].s, over[j]};
+        sum.scale(exp2f((run[j].m - base) * LOG2E));
+        sum.add(block);
+        run[j] = Running{m, sum.s};
+        over[j] = sum.over;
     }
 }
 
@@ -319,6 +323,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
     const int lane = threadIdx.x & 63, half = lane >> 5, wm = S::wm(), wn = S::wn();
     int64_t y[S::NB];
     Running run[S::NB];
+    float over[S::NB] = {};
 #pragma unroll
     for (int j = 0; j < S::NB; ++j) {
         const int64_t t = n0 + wn + 32 * j + (lane & 31);
@@ -339,7 +344,7 @@ __global__ __launch_bounds__(Shape<B>::THREADS, 2) void stats_kernel(Problem p, 
                 *reinterpret_cast<f32x4*>(to + at) = f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
             });
         }
-        fold(p, acc, m0 + wm, n0 + wn + (lane & 31), y, run, z_target);
+        fold(p, acc, m0 + wm, n0 + wn + (lane & 31), y, run, over, z_target);
     }
     __syncthreads();
     Running* sh = reinterpret_cast<Running*>(lds_a0);              // [2 waves along the vocabulary][B tokens]
@@ -370,6 +375,7 @@ __global__ __launch_bounds__(64, WAVES) void few_kernel(Problem p, int64_t per, 
     const T *wp[MB], *xp[NB];
     int64_t y[NB];
     Running run[NB];
+    float over[NB] = {};
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         const int64_t t = 32 * j + l31;
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(64, WAVES) void few_kernel(Problem p, int64_t per, 
                         *reinterpret_cast<f32x4*>(to + (j * 4 + r / 4) * 256) = f32x4{acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]};
             }
         }
-        fold(p, acc, block * ROWS, l31, y, run, z_target);
+        fold(p, acc, block * ROWS, l31, y, run, over, z_target);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {

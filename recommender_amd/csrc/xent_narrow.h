@@ -267,7 +267,8 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
     me.init((const T*)p.x, p.ldx, p.T, (int)p.D, h0);
     int y = -1;
     if (t < p.T && p.target[t] != p.ignore) y = (int)clamp_target(p.target[t], p.V);
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY;
+    Sum sum;
     f32x16 o[DX ? W::BLOCKS : 1];
     if constexpr (DX)
 #pragma unroll
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
             if (top > m + lag<T>()) {
                 const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * LOG2E);
                 m = top;
-                sum *= f;
+                sum.scale(f);
                 if constexpr (DX)
 #pragma unroll
                     for (int d = 0; d < W::BLOCKS; ++d) o[d] *= f;
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
         if (active) {
             // nothing above -inf yet: any finite reference leaves the sum at 0
             const float base = m == -INFINITY ? 0.f : m, shift = e_shift<T>() - base * LOG2E;
-            float top = -INFINITY;
+            float top = -INFINITY, here = 0.f;
             init(&biases[0][0] + after * 32, next);
             if (NS == 1) me.read_ahead(ring + after * BLOCK_BYTES);
             me.template block<DX, (NS > 1)>(
@@ -376,9 +377,10 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
                 [] {},
                 [&](int k, int n) {
 #pragma unroll
-                    for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) sum += s[r];
+                    for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) here += s[r];
                     if (k == n / 2) top = largest(next);
                 });
+            sum.add(here);
             if (i + 1 < n_blocks) settle(first + 32 * (int64_t)(i + 1), next, top);
         }
         if (i % NS == NS - 1) {
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
         if (i + 1 < n_blocks) work(i + 1, s1, s0);
     }
     if (!active) return;
-    const float total = sum + __shfl_xor(sum, 32, 64);
+    const float total = sum.s + __shfl_xor(sum.s, 32, 64);
     if (t >= p.T) return;
     if (half == 0) part[split * p.T + t] = Running{m, total * exp2f(-e_shift<T>())};
     if constexpr (DX) {
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     u += n_tiles;
 
     const float bias = BIAS && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
-    float sum = 0.f, low = 0.f;                                 // dbias, and in 32 bits what rounding has taken from it
+    Sum sum;
     f32x16 o[W::BLOCKS];
 #pragma unroll
     for (int d = 0; d < W::BLOCKS; ++d) o[d] = f32x16{};
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
             const float *expo32 = &expos[0][0] + 4 * half, *gn32 = &gns[0][0] + 4 * half;
             const int* y32 = &ys[tile & 3][i % NS * 32];
             const int mine = y32[l31];
-            float here = W::WIDE ? 0.f : sum;
+            float here = 0.f;
             next = f32x16{};
             if (NS == 1) me.read_ahead(ring + after * BLOCK_BYTES);
             me.template block<true, (NS > 1)>(
@@ -548,16 +550,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
 #pragma unroll
                     for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) here += s[r];
                 });
-            if constexpr (W::WIDE) {
-                // Thousands of small terms of one sign, then the targets' of the other: one after the other they left 7e-6 of dbias (11127 x
-                // 43,808 x 32), 150 times what a sum by halves does.  In 16 bits dbias is rounded to 2^-9 or 2^-12 of its size, and the
-                // register that this takes is not free (8192 x 100,003 x 128 bf16 932 -> 941 us).
-                const float add = here - low, total = sum + add;
-                low = (total - sum) - add;
-                sum = total;
-            } else {
-                sum = here;
-            }
+            sum.add(here);
         }
         if (i % NS == NS - 1 && tile + 1 < n_tiles) {
             if (tile + 2 < n_tiles) put(tile + 2);
@@ -574,7 +567,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     if (u < u1) me.init((const T*)p.w, p.ldw, p.V, (int)p.D, ((group + 1) * 4 + wave) * 32);      // on its way during the stores
     if (!active) continue;
     const float f = whole ? *scale / Traits<T>::G_SCALE : 1.f;
-    const float total = (sum + __shfl_xor(sum, 32, 64)) * f;
+    const float total = (sum.s + __shfl_xor(sum.s, 32, 64)) * f;
     if (v >= p.V) continue;
     const int64_t row = ((int64_t)blockIdx.x * 2 + (tile0 ? 0 : 1)) * 128 + wave * 32 + l31;
     if (half == 0) {

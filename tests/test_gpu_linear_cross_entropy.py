@@ -794,3 +794,29 @@ def test_gradient_of_the_bias_over_many_rows(D):
     sizes = (T - hits) / V + hits * (1 - 1 / V)
     assert 4 * math.log(V) + 4 + 32 < 80
     _close(db, exact, 80 * U * sizes, "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(16384, 600007, 24), (16384, 400003, 64), (16384, 200003, 128), (8192, 300007, 256), (65536, 300007, 264), (50, 8000009, 264), (3, 4000003, 700),
+                                   (33, 2000003, 100), (40, 8000009, 8)])
+def test_many_items_of_one_logit(dtype, T, V, D):
+    """A catalogue most of whose items have no vector yet: hundreds of thousands of equal terms in every row's sum.  Added one after the other
+    their roundings go one way.  Bounds: the terms are within (2 |z - max| + 4) u, the logits of the others within (D + 2) u of their
+    products' sizes; 128 terms one after the other, then compensated sums of them, rescaled at most once per new maximum, and 64 joins: 256 u.
+    The loss adds 4 u of itself and of the target's logit."""
+    ops = _ops()
+    gen = torch.Generator(device="cuda").manual_seed(V + D)
+    warm = 100
+    w = torch.zeros(V, D, dtype=dtype, device="cuda")
+    w[:warm] = (torch.randn(warm, D, device="cuda", generator=gen) / math.sqrt(D)).to(dtype)
+    x = torch.randn(T, D, device="cuda", generator=gen).to(dtype)
+    target = torch.randint(0, warm, (T,), device="cuda", generator=gen)
+    z = x.double() @ w[:warm].double().t()
+    others = z.scatter(1, target[:, None], -math.inf).exp().sum(1) + (V - warm)
+    zt = z.gather(1, target[:, None])[:, 0]
+    want = (others.log() - zt).exp().log1p()
+    span = z.max(1).values.clamp(min=0) - z.min(1).values.clamp(max=0)
+    tol = U * (2 * span + 4 + (D + 2) * (x.double().abs() @ w[:warm].double().abs().t()).max(1).values + 256 + 4 * want + 4 * zt.abs())
+    _close(ops.linear_cross_entropy(x, w, target, reduction="none"), want, tol, "loss without gradient")
+    leaf = x.clone().requires_grad_()
+    _close(ops.linear_cross_entropy(leaf, w, target, reduction="none").detach(), want, tol, "loss")
