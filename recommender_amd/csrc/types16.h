@@ -10,6 +10,23 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 // N consecutive values of T moved as one access (N * sizeof(T) a power of two up to 16)
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
+// A sum of many values and what rounding has put into it too much: its error does not grow with their number.  MAY_BE_INFINITE: an infinite
+// sum stays so, as a plain one does (else it is NaN from the next value on).
+struct Sum {
+    float s = 0.f, over = 0.f;
+    template <bool MAY_BE_INFINITE> __device__ __forceinline__ void add(float v)
+    {
+        const float part = v - over, total = s + part;
+        over = !MAY_BE_INFINITE || fabsf(total) < INFINITY ? (total - s) - part : 0.f;
+        s = total;
+    }
+    __device__ __forceinline__ void scale(float f)
+    {
+        s *= f;
+        over *= f;
+    }
+};
+
 // Calls fn with a value of the element type that `dtype` (RECO_DT_*) names; fn returns the call's status.
 template <typename F> static int reco_with_type(int dtype, F&& fn)
 {

@@ -297,7 +297,7 @@ __device__ __forceinline__ void fold(const Problem& p, f32x16 (&acc)[MB][NB], in
             for (int r = 0; r < 16; ++r) block += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * LOG2E);
         Sum sum{run[j].s, over[j]};
         sum.scale(exp2f((run[j].m - base) * LOG2E));
-        sum.add(block);
+        sum.add<false>(block);
         run[j] = Running{m, sum.s};
         over[j] = sum.over;
     }

@@ -380,7 +380,7 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
                     for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) here += s[r];
                     if (k == n / 2) top = largest(next);
                 });
-            sum.add(here);
+            sum.add<false>(here);
             if (i + 1 < n_blocks) settle(first + 32 * (int64_t)(i + 1), next, top);
         }
         if (i % NS == NS - 1) {
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
 #pragma unroll
                     for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) here += s[r];
                 });
-            sum.add(here);
+            sum.add<EACH>(here);                                   // rows' weights may be infinite
         }
         if (i % NS == NS - 1 && tile + 1 < n_tiles) {
             if (tile + 2 < n_tiles) put(tile + 2);

@@ -48,27 +48,11 @@ struct Problem {
 
 __device__ __forceinline__ int64_t clamp_target(int64_t y, int64_t V) { return y < 0 ? 0 : y >= V ? V - 1 : y; }
 
-// (m, s): running maximum and sum of exp(z - m) of the logits that are not the target's
+// (m, s): running maximum and sum of exp(z - m) of the logits that are not the target's.  A lane adds the terms of a block one after the
+// other and the blocks' sums as a Sum: hundreds of thousands of equal terms, as of items that have no vector yet, round the same way each
+// time (16384 x 600,007 x 24: a loss 2e-4 off), and dbias has thousands of small terms of one sign before the targets' of the other (11127 x
+// 43,808 x 32: 7e-6 off, now 4e-8).
 struct Running { float m, s; };
-
-// A sum of many parts and what rounding has put into it too much.  Rows add hundreds of thousands of terms in a lane: equal ones, as of items
-// that have no vector yet, round the same way each time (16384 x 600,007 x 24: a loss 2e-4 off), and dbias adds thousands of small terms of
-// one sign before the targets' of the other (11127 x 43,808 x 32: 7e-6 off, now 4e-8).  A lane adds a block's terms one after the other, and
-// the blocks to this.
-struct Sum {
-    float s = 0.f, over = 0.f;
-    __device__ __forceinline__ void add(float v)
-    {
-        const float part = v - over, total = s + part;
-        over = (total - s) - part;
-        s = total;
-    }
-    __device__ __forceinline__ void scale(float f)
-    {
-        s *= f;
-        over *= f;
-    }
-};
 
 __device__ __forceinline__ Running joined(Running a, Running b)
 {

@@ -820,3 +820,21 @@ def test_many_items_of_one_logit(dtype, T, V, D):
     _close(ops.linear_cross_entropy(x, w, target, reduction="none"), want, tol, "loss without gradient")
     leaf = x.clone().requires_grad_()
     _close(ops.linear_cross_entropy(leaf, w, target, reduction="none").detach(), want, tol, "loss")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(300, 90, 16), (3000, 900, 100), (3000, 90, 200), (3000, 900, 320)])
+def test_an_infinite_weight_gives_an_infinite_gradient_of_the_bias(dtype, T, V, D):
+    """As a plain sum does: the target's entry is -inf, the others are +inf (none is NaN: no probability here is 0)."""
+    ops = _ops()
+    x, w, target, b = _problem(T, V, D, dtype, True, learned=False)
+    x = (0.01 * x.float()).to(dtype)
+    g = torch.rand(T, device="cuda")
+    for row in (0, T // 2, T - 1):
+        h = g.clone()
+        h[row] = math.inf
+        db = ops.linear_cross_entropy_grad(x, w, target, b, "none", grad=h)[3]
+        hit = torch.zeros(V, dtype=torch.bool, device="cuda")
+        hit[target[row]] = True
+        assert bool(torch.isneginf(db[hit]).all()) and bool(torch.isposinf(db[~hit]).all())
+
