@@ -267,3 +267,28 @@ def test_offsets_past_32_bits():
     assert torch.equal(grad[far], values)
     grad[far] = 0
     assert not any(bool(part.any()) for part in grad.split(1 << 22))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,dim", [(300000, 1), (300000, 7), (1000003, 64), (500001, 512), (200003, 1030)])
+def test_gradient_of_a_very_frequent_id(dtype, n, dim):
+    """Equal rows' roundings all go one way.  At most 64 rows are added one after the other, and the joins' error does not grow: within 80 u."""
+    grad = torch.full((n, dim), 0.1, device="cuda").to(dtype)
+    ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+    ids[::7] = 2
+    hits = torch.bincount(ids, minlength=4).double()[:, None]
+    exact = (hits * float(grad[0, 0]) * 2.0 ** -6).expand(4, dim)
+    _close(_ops().embedding_grad(ids, grad, 4, scale=2.0 ** -6), exact, exact * (80 * U + torch.finfo(dtype).eps / 2), "gradient")
+
+
+@pytest.mark.parametrize("n", [3, 50, 5000, 200000])
+def test_gradient_of_infinite_rows(n):
+    """What a plain sum gives: infinite where one sign of it came in, NaN where both did or a NaN."""
+    grad = torch.full((n, 5), 0.5, device="cuda")
+    grad[0, 1] = grad[n // 2, 2] = grad[n - 1, 3] = math.inf
+    grad[0, 4], grad[n - 1, 4] = math.inf, -math.inf
+    got = _ops().embedding_grad(torch.zeros(n, dtype=torch.int64, device="cuda"), grad, 2)
+    assert float(got[0, 0]) == 0.5 * n and bool(torch.isposinf(got[0, 1:4]).all()) and bool(got[0, 4].isnan()) and not bool(got[1].any())
+    grad[1, 0] = math.nan
+    assert bool(_ops().embedding_grad(torch.zeros(n, dtype=torch.int64, device="cuda"), grad, 2)[0, 0].isnan())
+
