@@ -487,18 +487,31 @@ __global__ __launch_bounds__(256) void join_kernel(SumArgs a, int per, T* __rest
         }
         Sum acc[N];
         if (col < a.packs) {
-#pragma unroll 4
-            for (int64_t p = c + group; p <= e; p += groups) {
-                const float* src = a.part + (2 * p + (p == c ? 1 : 0)) * (int64_t)a.dim + col * N;
+            // four rows at a time, all on their way at once (behind the end the last one, not used)
+            for (int64_t p = c + group; p <= e; p += 4 * groups) {
+                float v[4][N], four[N];
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i].template add<true>(src[i]);
+                for (int k = 0; k < 4; ++k) {
+                    const int64_t q = p + k * groups < e ? p + k * groups : e;
+                    const float* src = a.part + (2 * q + (q == c ? 1 : 0)) * (int64_t)a.dim + col * N;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[k][i] = src[i];
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    four[i] = v[0][i];
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) four[i] += p + k * groups <= e ? v[k][i] : 0.f;
+                    acc[i].template add<true>(four[i]);
+                }
             }
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) sums[threadIdx.x * N + i] = acc[i].s;
         __syncthreads();
         if (group == 0 && col < a.packs) {
-            for (int g = 1; g < groups; ++g)
+            const int busy = e - c + 1 < groups ? (int)(e - c + 1) : groups;        // most runs have two partial rows
+            for (int g = 1; g < busy; ++g)
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i].template add<true>(sums[(g * lanes + lane) * N + i]);
             float total[N];
