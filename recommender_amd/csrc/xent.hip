@@ -597,6 +597,16 @@ __global__ __launch_bounds__(64, (NT == 1 && sizeof(T) == 4 ? 4 : NT <= 2 ? 3 : 
     }
 }
 
+// a + b as 32 bits round it, and exactly what that leaves (finite values)
+struct Parts {
+    float sum, rest;
+};
+__device__ __forceinline__ Parts exact_sum(float a, float b)
+{
+    const float sum = a + b, of_b = sum - a;
+    return Parts{sum, (a - (sum - of_b)) + (b - of_b)};
+}
+
 // WAVES waves per row: the splits' sums joined, the row's loss, lse and q.  T, dx_part: with the parts of the narrow form's weighted
 // sums of W [splits][T][D_out], D_out <= 256, also dx for an incoming gradient of one, in 32 bits.  A wave takes 64 splits at a time, and
 // what it waits for is memory: with one wave to a row, 505 splits of 16 rows x 128 took 40 to 72 us, with eight 15; up to 64 splits the
@@ -639,10 +649,19 @@ __device__ __forceinline__ void one_row(const Problem& p, int64_t t, const Runni
     if (wave == 0 && lane == 0) {
         if (oob && (y < 0 || y >= p.V)) atomicAdd(oob, 1);
         loss[t] = none ? NAN : target_less ? d + l : l;
-        // lse in two parts: as 32 bits round it, and what that leaves
-        const float base = target_less ? r.m : zt, more = target_less ? ls + l : l, whole = base + more;
-        lse[t] = none ? NAN : whole;
-        lse[p.T + t] = none ? NAN : (base - whole) + more;
+        // lse in two parts: as 32 bits round it, and what that leaves.  Its summands are exact (the maximum or the target's logit, and k log 2
+        // to 12 bits of it) or below 1.1, so that lse is within 2^-23 whatever its size is.
+        int k;
+        float f = frexpf(r.s, &k);
+        if (f < 0.70710678f) {
+            f *= 2.f;
+            --k;
+        }
+        constexpr float LN2_HIGH = 0x1.62ep-1f, LN2_LOW = 3.19461832987e-05f;
+        const Parts a = exact_sum(target_less ? r.m : zt, target_less ? k * LN2_HIGH : 0.f);
+        const Parts b = exact_sum(a.sum, target_less ? fmaf(k, LN2_LOW, logf(f)) + l : l);
+        lse[t] = none ? NAN : b.sum;
+        lse[p.T + t] = none ? NAN : a.rest + b.rest;
         rest[t] = q;
     }
     if (!dx_unit) return;

@@ -838,3 +838,15 @@ def test_an_infinite_weight_gives_an_infinite_gradient_of_the_bias(dtype, T, V, 
         hit[target[row]] = True
         assert bool(torch.isneginf(db[hit]).all()) and bool(torch.isposinf(db[~hit]).all())
 
+
+@pytest.mark.parametrize("D", [8, 128, 200])
+def test_probabilities_of_equal_logits(D):
+    """Every p is 1 / V, as exp(0 - lse) of an lse near 10.  Held to 2^-23 in its two parts, an exponent below 16 in powers of two rounded
+    to 32 bits (2^-21, times log 2), the exponential to 2 u, the result rounded: 11 u."""
+    ops = _ops()
+    assert 2.0 ** -23 + 2.0 ** -21 * math.log(2) + 3 * U <= 11 * U
+    x, target = torch.zeros(1, D, device="cuda"), torch.tensor([5], device="cuda")
+    for V in list(range(3000, 60000, 1999)) + [16018, 42903, 43469, 54789]:
+        assert math.log2(V) < 16
+        db = ops.linear_cross_entropy_grad(x, torch.zeros(V, D, device="cuda"), target, torch.zeros(V, device="cuda"), "sum")[3]
+        _close(db[6:], torch.full_like(db[6:], 1 / V, dtype=torch.float64), torch.full_like(db[6:], 11 * U / V, dtype=torch.float64), "V = %d" % V)
