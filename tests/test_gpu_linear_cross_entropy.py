@@ -850,3 +850,26 @@ def test_probabilities_of_equal_logits(D):
         assert math.log2(V) < 16
         db = ops.linear_cross_entropy_grad(x, torch.zeros(V, D, device="cuda"), target, torch.zeros(V, device="cuda"), "sum")[3]
         _close(db[6:], torch.full_like(db[6:], 1 / V, dtype=torch.float64), torch.full_like(db[6:], 11 * U / V, dtype=torch.float64), "V = %d" % V)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(10, 50, 1), (70, 300, 3), (40, 50, 32), (33, 90, 64), (300, 700, 100), (10, 50, 128), (40, 300, 250), (70, 300, 320)])
+def test_a_row_that_is_sure_of_another_item(dtype, T, V, D):
+    """p of that item is 1 to 2^-57 whatever rounding does to its logit of 50 to 70, as long as both passes round it alike: lse to 2^-23, the
+    exponential 2 u, and the sums of a few terms 4 u, within 8 u of the rows' weights in 32 bits; in 16 the result is rounded."""
+    gen = torch.Generator(device="cuda").manual_seed(T + V + D)
+    way = torch.nn.functional.normalize(torch.randn(D, device="cuda", generator=gen), dim=0)
+    w = (0.01 * torch.randn(V, D, device="cuda", generator=gen))
+    w[7] = 8 * way
+    x = (6.5 + 2 * torch.rand(T, 1, device="cuda", generator=gen)) * way
+    b = 0.5 * torch.randn(V, device="cuda", generator=gen)
+    target = torch.full((T,), 3, device="cuda")
+    x, w, b = x.to(dtype), w.to(dtype), b.to(dtype)
+    z = x.double() @ w.double().t() + b.double()
+    rest = torch.cat([z[:, :7], z[:, 8:]], 1).max(1).values
+    assert bool((z[:, 7] - rest > 40 + math.log(V)).all()) and bool((z[:, 7] > 48).all())
+    g = 0.5 + torch.rand(T, device="cuda", generator=gen)
+    for reduction, h, total in (("sum", None, float(T)), ("none", g, float(g.double().sum()))):
+        db = _ops().linear_cross_entropy_grad(x, w, target, b, reduction, grad=h)[3].double()
+        tol = total * (8 * U + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2))
+        assert abs(float(db[7]) - total) <= tol and abs(float(db[3]) + total) <= tol
