@@ -1394,7 +1394,7 @@ int backward(const Args& a, int reduction, const float* state, const float* kept
         hipLaunchKernelGGL(top_kernel, dim3(row_blocks), dim3(256), 0, s, p, dloss, tops);
     else
         gn = nullptr;
-    hipLaunchKernelGGL(weights_kernel, dim3(row_blocks), dim3(256), 0, s, p, reduction, dloss, state + 3 * a.T, tops, row_blocks, lse, (int)(sizeof(T) == 4),
+    hipLaunchKernelGGL(weights_kernel, dim3(row_blocks), dim3(256), 0, s, p, reduction, dloss, state + 3 * a.T, tops, row_blocks, lse, (int)(sizeof(T) == 4 || db),
                        log2f(Traits<T>::G_SCALE), gn, scale, y, expo);
     if (narrow) {
         if (dw || db) {

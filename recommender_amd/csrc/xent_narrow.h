@@ -412,9 +412,9 @@ __global__ __launch_bounds__(WAVES * 64, (WAVES == 1 ? 1 : rows_waves<T, DP, DX>
 // ---------------------------------------------------------------------------------------------
 // cols: dW and dbias
 // ---------------------------------------------------------------------------------------------
-// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count.  In 32 bits, and with a bias, whose logits may be the type's
+// expo[t]: -lse_t log2(e) + log2(G_SCALE), -inf for rows that do not count.  In 32 bits, and with BIAS, as such logits may be the type's
 // lowest: lse_t itself (+inf), and in 32 bits expo[T + t] minus what rounding left of lse_t, times log2(e).  y[t]: the target, -1 for
-// rows that do not count.  EACH: rows have weights gn[t].
+// rows that do not count.  BIAS: there is one, or its gradient is asked for.  EACH: rows have weights gn[t].
 // The work is groups of 128 held rows times tiles of streamed ones, in that order; every workgroup takes an equal share of consecutive
 // (group, tile) units, so that the groups need not be a multiple of what the chip holds at once (782 groups over 512 places: 0.72 ms
 // with a group to a workgroup).  A group inside one share is finished there; else its parts are written in 32 bits (place 1 of a
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     const bool whole = n_tiles == tiles_in_all, stage = u == u0 || tiles_in_all > 1;     // a single tile stays for every group
     u += n_tiles;
 
-    const float bias = BIAS && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
+    const float bias = BIAS && p.bias && v < p.V ? (float)((const T*)p.bias)[v] : 0.f;
     Sum sum;
     f32x16 o[W::BLOCKS];
 #pragma unroll
@@ -555,9 +555,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
                 },
                 [&](int k, int n) {
 #pragma unroll
-                    for (int r = k * 16 / n; r < (k + 1) * 16 / n; ++r) here += s[r];
+                    for (int r = k * 16 / n; BIAS && r < (k + 1) * 16 / n; ++r) here += s[r];
                 });
-            sum.add<EACH>(here);                                   // rows' weights may be infinite
+            if (BIAS) sum.add<EACH>(here);                         // rows' weights may be infinite
         }
         if (i % NS == NS - 1 && tile + 1 < n_tiles) {
             if (tile + 2 < n_tiles) put(tile + 2);
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void narrow_cols_ke
     const float total = (sum.s + __shfl_xor(sum.s, 32, 64)) * f;
     if (v >= p.V) continue;
     const int64_t row = ((int64_t)blockIdx.x * 2 + (tile0 ? 0 : 1)) * 128 + wave * 32 + l31;
-    if (half == 0) {
+    if (BIAS && half == 0) {
         if (!whole) db_part[row] = total;
         else if (db) db[v] = (T)total;
     }
@@ -719,7 +719,7 @@ int narrow_cols_of(const Problem& p, const NarrowPlan& n, int64_t width_out, con
                    const float* scale, void* dw, void* db, float* dw_part, float* db_part, hipStream_t s)
 {
     return shape_of<T>(p.D, [&](auto dp, int64_t, int64_t) -> int {
-        return with_flag(p.bias != nullptr, [&](auto bias) -> int {
+        return with_flag(p.bias || db, [&](auto bias) -> int {
             return with_flag(gn != nullptr, [&](auto each) -> int {
                 hipLaunchKernelGGL((narrow_cols_kernel<T, decltype(dp)::value, decltype(bias)::value, decltype(each)::value>), dim3((unsigned)n.w_shares), dim3(256),
                                    0, s, p, n.w_groups * n.w_tiles, n.w_share, (int)n.w_tiles, (int)width_out, expo, y, rest, gn, scale, (T*)dw, (T*)db, dw_part,

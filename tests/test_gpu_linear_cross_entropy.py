@@ -873,3 +873,39 @@ def test_a_row_that_is_sure_of_another_item(dtype, T, V, D):
         db = _ops().linear_cross_entropy_grad(x, w, target, b, reduction, grad=h)[3].double()
         tol = total * (8 * U + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2))
         assert abs(float(db[7]) - total) <= tol and abs(float(db[3]) + total) <= tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(40, 90, 16), (300, 1500, 64), (3000, 700, 128), (70, 300, 250), (70, 300, 320)])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_gradient_of_a_bias_that_is_not_there(dtype, T, V, D, reduction):
+    """The C entries give the gradient of a bias of zeros without one, beside the others' or alone; asking for it changes none of their bits in 32
+    bits, and in 16 no more than the exponent's rounding."""
+    from recommender_amd import _lib
+    x, w, t, _ = _problem(T, V, D, dtype, False, 8)
+    t[::5] = -100
+    L, ops = _lib.lib(), _ops()
+    dt, s = ops.DTYPES[dtype], torch.cuda.current_stream().cuda_stream
+    g = torch.rand(T, device="cuda") if reduction == "none" else torch.tensor(0.75, device="cuda")
+    want = Exact(x, w, t, None, reduction, -100, g)
+    what = (x.data_ptr(), D, w.data_ptr(), D)
+    floats = L.reco_linear_xent_kept_floats(dt, T, V, D, 1)
+    kept, state, loss = torch.empty(floats, device="cuda"), torch.empty(3 * T + 1, device="cuda"), torch.empty(T, device="cuda")
+    ws = torch.empty(max(L.reco_linear_xent_workspace_bytes(*what, dt, T, V, D, 1), L.reco_linear_xent_grad_workspace_bytes(*what, dt, T, V, D)),
+                     dtype=torch.uint8, device="cuda")
+    at, red = kept.data_ptr() if floats else None, ops.REDUCTIONS[reduction]
+    _lib.check(L.reco_linear_xent(*what, None, dt, T, V, D, t.data_ptr(), -100, red, loss.data_ptr(), state.data_ptr(), at, None, ws.data_ptr(), ws.numel(), s))
+
+    def grad(*wanted):
+        out = [torch.full((n,), math.nan, dtype=dtype, device="cuda") if k else None for n, k in zip((T * D, V * D, V), wanted)]
+        _lib.check(L.reco_linear_xent_grad(*what, None, dt, T, V, D, t.data_ptr(), -100, red, state.data_ptr(), at, g.data_ptr(),
+                                           *(None if o is None else o.data_ptr() for o in out), ws.data_ptr(), ws.numel(), s))
+        return out
+    dx, dw, db = grad(1, 1, 1)
+    _close(dx.view(T, D), want.dx, want.dx_tol, "dx")
+    _close(dw.view(V, D), want.dw, want.dw_tol, "dw")
+    _close(db, want.db, want.db_tol, "db")
+    assert torch.equal(grad(0, 0, 1)[2], db) and torch.equal(grad(0, 1, 1)[1], dw) and torch.equal(grad(1, 0, 0)[0], dx)
+    other = grad(1, 1, 0)[1]
+    _close(other.view(V, D), want.dw, want.dw_tol, "dw without db")
+    assert dtype != torch.float32 or torch.equal(other, dw)
