@@ -139,7 +139,7 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
  * (src/autorec/utils/model.py:31-33) is trained with; no counterpart in the reference, which samples negatives.
  * x [T, D], w [V, D], bias [V] (nullable) of one `dtype`, rows dense with strides ldx / ldw.  Any sizes, strides and alignment
  * (rows that do not start on 16 bytes, or whose width is no whole number of 16-byte groups, may be copied into ws first).
- * target int64 [T]; a row whose target equals `ignore` has no loss and no gradient whatever its x holds; other targets outside
+ * target int64 [T]; a row whose target equals `ignore` has no loss and no gradient whatever its x or dloss hold; other targets outside
  * [0, V) are clamped and counted in *oob (nullable).  bias may hold -inf (items that are never offered) or the type's lowest value.
  * reduction: RECO_XENT_NONE (loss [T]), _MEAN over the rows that count (loss [1]; NaN when none does), _SUM.  loss and state are fp32.
  * state [3 T + 1] is written by the forward call and read by the gradient call, which takes the same operands.
@@ -148,8 +148,9 @@ int reco_linear_f32(const float* A, int64_t lda, const int64_t* a_rows, int64_t 
  * Wider ones: the logits, where that saves time and they are few (up to 512 MB); without them the gradient call computes them again.
  * with_dx: whether a gradient of x will be asked for.  keep: whether the forward call will be given that room (its workspace differs).
  * dloss fp32: [T] for RECO_XENT_NONE, else [1].  dx [T, D], dw [V, D], db [V] dense, of `dtype`; NULL = not wanted.
- * Sums run in an order that depends on the sizes alone: the same bits on every run.  Work is enqueued only; calls that overlap need a
- * workspace each (*_workspace_bytes looks at x and w for their alignment, never through them), 16-byte aligned.
+ * Arithmetic is fp32; the terms of dx and dw are rounded to `dtype` to be multiplied (half a step each), those of db are not.  Sums run in
+ * an order that depends on the sizes alone: the same bits on every run.  Work is enqueued only; calls that overlap need a workspace each
+ * (*_workspace_bytes looks at x and w for their alignment, never through them), 16-byte aligned.
  * ---------------------------------------------------------------------------------------- */
 #define RECO_XENT_NONE 0
 #define RECO_XENT_MEAN 1

@@ -14,8 +14,8 @@
 // A launch splits the streamed rows where there are few held ones; the parts are joined in order of the splits.
 //
 // What bounds it: a wave issues matrix instructions and exponentials in turn; an exponential per logit and two products of the row's width
-// share a SIMD's issue.  bf16 8192 x 100,003 x 128: rows 0.47 ms, cols 0.51 (0.90, 0.83 PFLOP/s); f16 4097 x 50,021 x 250: 0.41 and 0.36 (0.50,
-// 0.56); f32 6038 x 3533 x 32: 42 us each.  115 x 1 M x 128 without gradient: 64 us, 4.0 TB/s.  At rows of 256 bytes three waves a SIMD spilled;
+// share a SIMD's issue.  bf16 8192 x 100,003 x 128: rows 0.47 ms, cols 0.50 (0.90, 0.84 PFLOP/s); f16 4097 x 50,021 x 250: 0.43 and 0.37 (0.48,
+// 0.55); f32 6038 x 3533 x 32: 43 us each.  115 x 1 M x 128 without gradient: 64 us, 4.0 TB/s.  At rows of 256 bytes three waves a SIMD spilled;
 // 64 held rows a wave halved the waves and were slower; so was a ring unrolled over six blocks.
 #pragma once
 #include "xent_shared.h"
