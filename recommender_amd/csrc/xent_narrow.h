@@ -230,16 +230,16 @@ template <typename U> __device__ __forceinline__ void store4(U* row, int c, int 
     if (c + 3 < width) row[c + 3] = (U)v3;
 }
 
-// Waves per SIMD that the registers are cut for.  8192 x 100,003 in bf16 with gradients: x 32 500 us with two, 447 with three, 432 with
-// four; x 64 662, 609, 1263 (spills); f32 2000 x 50,000 x 32 296, 287, 318 and 6038 x 3533 x 32 144, 149, 147.
+// Waves per SIMD that the registers are cut for.  8192 x 100,003 in bf16 with gradients: x 32 462 us with two, 408 with three, 399 with
+// four; x 64 593, 570, 1206 (spills); f32 2000 x 50,000 x 32 282, 280, 309 and 6038 x 3533 x 32 109, 113, 130.
 template <typename T, int DP> constexpr int waves_per_simd()
 {
     if (sizeof(T) == 4) return DP == 128 ? 1 : 2;
     return DP == 32 ? 4 : DP == 64 ? 3 : DP == 128 ? 2 : 1;
 }
 
-// of the rows kernel: one more without dx, whose sums are half of the registers (8192 x 100,003 x 128 bf16 326 -> 294 us, 4097 x 50,021 x 256
-// f16 229 -> 167, 115 x 1 M x 128 f32 351 -> 328; f32 2000 x 50,000 x 64 144 -> 147, and below that there are enough)
+// of the rows kernel: one more without dx, whose sums are half of the registers (8192 x 100,003 x 128 bf16 311 -> 289 us, 4097 x 50,021 x 256
+// f16 225 -> 154, 115 x 1 M x 128 f32 336 -> 295; f32 2000 x 50,000 x 64 137 both, and below that there are enough)
 template <typename T, int DP, bool DX> constexpr int rows_waves() { return waves_per_simd<T, DP>() + (!DX && DP >= 128 ? 1 : 0); }
 
 // ---------------------------------------------------------------------------------------------
